@@ -9,6 +9,7 @@ Kinds of case:
 
 With `own` false every operator runs in its plain form: elementary torch operations in 32 bits, rounded once at the end.
 """
+import functools
 import math
 
 import numpy as np
@@ -243,10 +244,16 @@ def _few(s):
 
 
 # ------------------------------------------------------------------------------------------------ one pass --
+@functools.lru_cache(maxsize=1)
+def _framework():
+    from radeonflow_kernels_b200 import grouped, quant
+    return grouped, quant
+
+
 def run(state):
     kind = state["kind"]
     if own:
-        from radeonflow_kernels_b200 import grouped, quant
+        grouped, quant = _framework()
         if kind == "quantize":
             return quant.fp8_quantize(state["x"], rows=state["rows"])
         if kind == "blocks":
