@@ -498,6 +498,31 @@ int rf_moe_ep_buffer(RfMoeEp *ep, int which, void **ptr, size_t *bytes);
 int rf_moe_ep_disconnect(RfMoeEp *ep);
 int rf_moe_ep_destroy(RfMoeEp *ep);
 
+/* ------------------------------------------------------- FP8 operands and experts -- */
+/* None of these has a counterpart in the reference, whose FP8 operands arrive quantised and whose experts are fp16. */
+
+enum { RF_F16 = 0, RF_BF16 = 1, RF_F32 = 2 };   /* element types of the matrices below */
+
+/* Rows to e4m3fn with one fp32 scale per 1 x 128 block, the A operand of rf_fp8_gemm and rf_fp8_grouped_gemm:
+ * a = max(largest magnitude of the block, 2^-100), scale = a / 448, q = e4m3(x * (448 / a)).  A block with a NaN is NaN
+ * throughout, one with an infinity has an infinite scale.
+ * x: `dtype` [*, k], rows `row_stride` elements apart; with rows != NULL row i of the result is row rows[i] mod n_src of x.
+ * q [m, k] (16-byte aligned), scale [m, k/128], both dense.  k % 128 == 0.  x needs its element's alignment; rows that start
+ * at multiples of 16 bytes are read faster.                                                     */
+int rf_fp8_quantize(const void *x, int dtype, long long row_stride, const int *rows, int n_src, int m, int k, void *q,
+                    float *scale, rf_stream_t stream);
+
+/* gate_up: `dtype` [m, 2f], rows `row_stride` elements apart; h = SiLU(gate_up[:, :f]) * gate_up[:, f:] in fp32, quantised as
+ * rf_fp8_quantize does: q [m, f], scale [m, f/128].  f % 128 == 0.                              */
+int rf_fp8_swiglu_quantize(const void *gate_up, int dtype, long long row_stride, int m, int f, void *q, float *scale,
+                           rf_stream_t stream);
+
+/* e matrices [n, k] to e4m3fn with one scale per 128 x 128 block (the last of n may be shorter), the B operand:
+ * element (n, k) of matrix i at w[i * stride_e + n * stride_n + k * stride_k]; stride_n or stride_k is 1 (a weight stored
+ * [k, n] is turned round on the way).  q [e, n, k] and scale [e, ceil(n/128), k/128], dense.  k % 128 == 0.  */
+int rf_fp8_quantize_blocks(const void *w, int dtype, int e, int n, int k, long long stride_e, long long stride_n,
+                           long long stride_k, void *q, float *scale, rf_stream_t stream);
+
 /* Library / build identification: "rf_b200 <version> sm_100a".               */
 const char *rf_version(void);
 

@@ -94,6 +94,7 @@ def lib() -> ctypes.CDLL:
         _lib = ctypes.CDLL(LIB_PATH)
         _declare(_lib)
         _declare_ep(_lib)
+        _declare_fp8(_lib)
     return _lib
 
 
@@ -231,6 +232,16 @@ def _declare(L: ctypes.CDLL) -> None:
     L.rf_moe_grouped_gemm_scatter.argtypes = [vp, ci, pvp, vp, ci, ci, ci, vp, pvp, ci, vp]
     L.rf_moe_ep_combine.restype = ci
     L.rf_moe_ep_combine.argtypes = [pvp, vp, vp, vp, vp, vp, ci, ci, ci, ci, vp, vp]
+
+
+def _declare_fp8(L: ctypes.CDLL) -> None:
+    vp, ci, ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
+    L.rf_fp8_quantize.restype = ci
+    L.rf_fp8_quantize.argtypes = [vp, ci, ll, vp, ci, ci, ci, vp, vp, vp]
+    L.rf_fp8_swiglu_quantize.restype = ci
+    L.rf_fp8_swiglu_quantize.argtypes = [vp, ci, ll, ci, ci, vp, vp, vp]
+    L.rf_fp8_quantize_blocks.restype = ci
+    L.rf_fp8_quantize_blocks.argtypes = [vp, ci, ci, ci, ci, ll, ll, ll, vp, vp, vp]
 
 
 class RfMoeEpConfig(ctypes.Structure):

@@ -1,0 +1,286 @@
+// FP8 operands of the block-scaled GEMMs: e4m3fn values with one fp32 scale per 1 x 128 block of a row (activations) or per
+// 128 x 128 block (weights).  No counterpart in the reference, whose operands arrive quantised.
+//
+//   a = max(largest magnitude of the block, 2^-100),  scale = a / 448,  q = e4m3(x * (448 / a)), to nearest, ties to even
+//
+// 448 is e4m3's largest value; the floor keeps 448 / a finite for blocks of zeros.  A NaN makes its whole block NaN, scale
+// included, and an infinity makes the scale infinite: an overflow stays visible behind the product.
+//
+// All three are one pass over the data, held in registers between the block's maximum and its conversion; HBM bounds them.
+#include "ptx.cuh"
+#include "host_util.h"
+#include "launch.h"
+#include "../../include/rf_b200.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace rf {
+
+namespace {
+
+constexpr int kBlock = 128;
+constexpr float kE4m3Max = 448.0f;
+constexpr float kAmaxFloor = 7.888609052210118e-31f;      // 2^-100
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// Four values to four e4m3 bytes, the first in the lowest.
+__device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d) {
+    uint16_t lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+    return (uint32_t)lo | ((uint32_t)hi << 16);
+}
+
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ __half zero_of(__half) { return __ushort_as_half(0); }
+__device__ __forceinline__ __nv_bfloat16 zero_of(__nv_bfloat16) { return __ushort_as_bfloat16(0); }
+__device__ __forceinline__ float zero_of(float) { return 0.f; }
+
+// Eight consecutive elements, as they lie in memory: 16-byte loads (VEC: the address is a multiple of 16) or element by
+// element, those from `n` on zero.
+template <class T>
+struct Eight {
+    static constexpr int kVecs = sizeof(T) / 2;
+    union {
+        uint4 v[kVecs];
+        T e[8];
+    };
+    __device__ __forceinline__ Eight() {}
+    template <bool VEC>
+    __device__ __forceinline__ void load(const T* p, int n = 8) {
+        if (VEC && n >= 8) {
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) v[i] = ld_global_cg_v4(reinterpret_cast<const uint4*>(p) + i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = i < n ? p[i] : zero_of(T());
+        }
+    }
+    __device__ __forceinline__ float f(int i) const { return to_f32(e[i]); }
+};
+
+// The half warp's largest value (16 lanes hold one block of 128).
+__device__ __forceinline__ float half_warp_max(float a) {
+#pragma unroll
+    for (int s = 8; s > 0; s >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, s));
+    return a;
+}
+
+// This lane's eight of a block's 128 values -> its eight bytes, and the block's scale.
+__device__ __forceinline__ uint2 quantize_eight(const float (&x)[8], float* scale) {
+    float a = fabsf(x[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) a = max_nan(a, fabsf(x[i]));
+    a = max_nan(half_warp_max(a), kAmaxFloor);
+    *scale = __fdiv_rn(a, kE4m3Max);
+    const float r = __fdiv_rn(kE4m3Max, a);
+    return make_uint2(to_e4m3x4(x[0] * r, x[1] * r, x[2] * r, x[3] * r), to_e4m3x4(x[4] * r, x[5] * r, x[6] * r, x[7] * r));
+}
+
+// ------------------------------------------------------------------------------------------------- rows --
+// 16 lanes per block of 128 columns, kPerHalf blocks in a row per half warp: all their loads are in flight before the first
+// is used.  Row i of the result is row i of x, or row rows[i] mod n_src (as an unsigned number, so that no index leaves x).
+constexpr int kRowThreads = 256;
+constexpr int kPerHalf = 4;
+constexpr int kBlocksPerCta = kRowThreads / 16 * kPerHalf;
+
+// SWIGLU: x is [gate | up], 2 k columns, and what is quantised is SiLU(gate) * up = gate / (1 + exp(-gate)) * up in fp32.
+template <class T, bool VEC, bool SWIGLU>
+__global__ void __launch_bounds__(kRowThreads)
+quantize_rows_kernel(const T* x, long long row_stride, const int* rows, int n_src, int m, int kb, uint8_t* q, float* scale) {
+    griddep_launch_dependents();
+    griddep_wait();
+    const int lane = threadIdx.x & 15;
+    const long long total = (long long)m * kb;
+    const long long first = ((long long)blockIdx.x * (kRowThreads / 16) + (threadIdx.x >> 4)) * kPerHalf;
+    if (first - (threadIdx.x & 16 ? kPerHalf : 0) >= total) return;       // whole warps leave: the shuffles need all lanes
+    int row = (int)(first / kb), col = (int)(first - (long long)row * kb);
+    Eight<T> g[kPerHalf], u[SWIGLU ? kPerHalf : 1];
+#pragma unroll
+    for (int i = 0; i < kPerHalf; ++i) {
+        if (first + i < total) {
+            const long long src = rows != nullptr ? (long long)((uint32_t)ld_global_s32(rows + row) % (uint32_t)n_src) : row;
+            const T* p = x + src * row_stride + col * kBlock + lane * 8;
+            g[i].template load<VEC>(p);
+            if (SWIGLU) u[i].template load<VEC>(p + (long long)kb * kBlock);
+        }
+        if (++col == kb) {
+            col = 0;
+            ++row;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kPerHalf; ++i) {
+        const bool valid = first + i < total;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[j] = valid ? g[i].f(j) : 0.f;
+            if (SWIGLU && valid) v[j] = __fdividef(v[j], 1.0f + expf(-v[j])) * u[i].f(j);
+        }
+        float s;
+        const uint2 o = quantize_eight(v, &s);
+        if (valid) {
+            *reinterpret_cast<uint2*>(q + (first + i) * kBlock + lane * 8) = o;
+            if (lane == 0) scale[first + i] = s;
+        }
+    }
+}
+
+// ----------------------------------------------------------------------------------------------- blocks --
+// One CTA per 128 x 128 block; element (n, k) of matrix e lies at w[e * stride_e + n * stride_n + k * stride_k].  A thread
+// holds 64 values: with k contiguous (KMAJOR) eight runs of eight along k, written as they are read; with n contiguous two
+// pieces of 4 k x 8 n, whose bytes, four along k to a word, are turned round in shared memory.  Word (n, k/4) lies at
+// word n * 32 + (k/4 ^ 2 (n/8 mod 16)): conflict-free for the 16 x 2 pieces that a warp writes, and pairs of words stay together.
+constexpr int kBlockThreads = 256;
+
+template <class T, bool VEC, bool KMAJOR>
+__global__ void __launch_bounds__(kBlockThreads)
+quantize_blocks_kernel(const T* w, long long stride_e, long long stride_n, long long stride_k, int n, int kb, uint8_t* q,
+                       float* scale) {
+    __shared__ float warp_max[kBlockThreads / 32];
+    __shared__ uint32_t turned[KMAJOR ? 1 : kBlock * kBlock / 4];
+    griddep_launch_dependents();
+    griddep_wait();
+    const int tid = threadIdx.x, k0 = blockIdx.x * kBlock, nb = blockIdx.y, e = blockIdx.z, n0 = nb * kBlock;
+    const int left = n - n0;                                   // rows of w that the block still has
+    w += e * stride_e + (long long)n0 * stride_n + (long long)k0 * stride_k;
+    const long long k = (long long)kb * kBlock;
+    q += ((long long)e * n + n0) * k + k0;
+    Eight<T> v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (KMAJOR) {
+            const int r = i * 16 + (tid >> 4);
+            v[i].template load<VEC>(w + r * stride_n + (tid & 15) * 8, r < left ? 8 : 0);
+        } else {
+            // piece i / 4: k rows 4 (tid / 16 + 16 (i / 4)) + i % 4, columns 8 (tid % 16) ..
+            const int r = 4 * ((tid >> 4) + 16 * (i >> 2)) + (i & 3), c = 8 * (tid & 15);
+            v[i].template load<VEC>(w + r * stride_k + c, left - c);
+        }
+    }
+    float a = kAmaxFloor;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a = max_nan(a, fabsf(v[i].f(j)));
+    a = half_warp_max(a);
+    a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 16));
+    if ((tid & 31) == 0) warp_max[tid >> 5] = a;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kBlockThreads / 32; ++i) a = max_nan(a, warp_max[i]);
+    const float r = __fdiv_rn(kE4m3Max, a);
+    if (tid == 0) scale[((long long)e * gridDim.y + nb) * kb + blockIdx.x] = __fdiv_rn(a, kE4m3Max);
+    if (KMAJOR) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int row = i * 16 + (tid >> 4);
+            if (row < left)
+                *reinterpret_cast<uint2*>(q + row * k + (tid & 15) * 8) =
+                    make_uint2(to_e4m3x4(v[i].f(0) * r, v[i].f(1) * r, v[i].f(2) * r, v[i].f(3) * r),
+                               to_e4m3x4(v[i].f(4) * r, v[i].f(5) * r, v[i].f(6) * r, v[i].f(7) * r));
+        }
+    } else {
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                turned[(8 * (tid & 15) + j) * 32 + (((tid >> 4) + 16 * p) ^ (2 * (tid & 15)))] =
+                    to_e4m3x4(v[4 * p].f(j) * r, v[4 * p + 1].f(j) * r, v[4 * p + 2].f(j) * r, v[4 * p + 3].f(j) * r);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int row = i * 16 + (tid >> 4), pair = (tid & 15) ^ (row >> 3);
+            if (row < left)
+                *reinterpret_cast<uint2*>(q + row * k + (tid & 15) * 8) =
+                    *reinterpret_cast<const uint2*>(&turned[row * 32 + 2 * pair]);
+        }
+    }
+}
+
+template <class T>
+cudaError_t launch_rows(bool vec, bool swiglu, const void* x, long long row_stride, const int* rows, int n_src, int m, int k,
+                        void* q, float* scale, cudaStream_t stream) {
+    auto kernel = swiglu ? (vec ? quantize_rows_kernel<T, true, true> : quantize_rows_kernel<T, false, true>)
+                         : (vec ? quantize_rows_kernel<T, true, false> : quantize_rows_kernel<T, false, false>);
+    const long long blocks = (long long)m * (k / kBlock);
+    return launch_kernel(kernel, dim3((unsigned)((blocks + kBlocksPerCta - 1) / kBlocksPerCta)), kRowThreads, 0, stream, true,
+                         static_cast<const T*>(x), row_stride, rows, n_src, m, k / kBlock, static_cast<uint8_t*>(q), scale);
+}
+
+template <class T>
+cudaError_t launch_blocks(bool vec, bool k_major, const void* w, int e, int n, int k, long long stride_e, long long stride_n,
+                          long long stride_k, void* q, float* scale, cudaStream_t stream) {
+    auto kernel = k_major ? (vec ? quantize_blocks_kernel<T, true, true> : quantize_blocks_kernel<T, false, true>)
+                          : (vec ? quantize_blocks_kernel<T, true, false> : quantize_blocks_kernel<T, false, false>);
+    const dim3 grid((unsigned)(k / kBlock), (unsigned)((n + kBlock - 1) / kBlock), (unsigned)e);
+    return launch_kernel(kernel, grid, kBlockThreads, 0, stream, true, static_cast<const T*>(w), stride_e, stride_n, stride_k, n,
+                         k / kBlock, static_cast<uint8_t*>(q), scale);
+}
+
+int element_bytes(int dtype) { return dtype == RF_F16 || dtype == RF_BF16 ? 2 : dtype == RF_F32 ? 4 : 0; }
+
+// x's rows can be read 16 bytes at a time
+bool rows_aligned(const void* x, long long row_stride, int bytes) {
+    return !misaligned({x}, 16) && (row_stride * bytes) % 16 == 0;
+}
+
+int quantize_rows(bool swiglu, const void* x, int dtype, long long row_stride, const int* rows, int n_src, int m, int k,
+                  void* q, float* scale, rf_stream_t stream) {
+    const int bytes = element_bytes(dtype);
+    if (bytes == 0) return RF_ERR_UNSUPPORTED;
+    if (m < 0 || k <= 0 || k % kBlock != 0 || (long long)m * (k / kBlock) > 0x7fffffffLL) return RF_ERR_BAD_SHAPE;
+    if (rows != nullptr && n_src <= 0 && m > 0) return RF_ERR_BAD_SHAPE;
+    if (m == 0) return RF_OK;
+    if (!x || !q || !scale) return RF_ERR_NULL_POINTER;
+    if (misaligned({q}, 16) || misaligned({scale, rows}, 4) || misaligned({x}, (unsigned)bytes)) return RF_ERR_MISALIGNED;
+    if (!device_state()) return RF_ERR_CUDA;
+    const bool vec = rows_aligned(x, row_stride, bytes);
+    auto run = dtype == RF_F16 ? launch_rows<__half> : dtype == RF_BF16 ? launch_rows<__nv_bfloat16> : launch_rows<float>;
+    return run(vec, swiglu, x, row_stride, rows, n_src, m, k, q, scale, reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess
+               ? RF_OK : RF_ERR_CUDA;
+}
+
+}  // namespace
+
+}  // namespace rf
+
+extern "C" {
+
+int rf_fp8_quantize(const void* x, int dtype, long long row_stride, const int* rows, int n_src, int m, int k, void* q,
+                    float* scale, rf_stream_t stream) {
+    return rf::quantize_rows(false, x, dtype, row_stride, rows, n_src, m, k, q, scale, stream);
+}
+
+int rf_fp8_swiglu_quantize(const void* gate_up, int dtype, long long row_stride, int m, int f, void* q, float* scale,
+                           rf_stream_t stream) {
+    return rf::quantize_rows(true, gate_up, dtype, row_stride, nullptr, 0, m, f, q, scale, stream);
+}
+
+int rf_fp8_quantize_blocks(const void* w, int dtype, int e, int n, int k, long long stride_e, long long stride_n,
+                           long long stride_k, void* q, float* scale, rf_stream_t stream) {
+    const int bytes = rf::element_bytes(dtype);
+    if (bytes == 0) return RF_ERR_UNSUPPORTED;
+    // (the grid's second and third dimension hold 65535 blocks)
+    if (e < 0 || e > 65535 || n < 0 || n > 65535 * 128 || k <= 0 || k % 128 != 0) return RF_ERR_BAD_SHAPE;
+    if (stride_k != 1 && stride_n != 1) return RF_ERR_UNSUPPORTED;
+    if (e == 0 || n == 0) return RF_OK;
+    if (!w || !q || !scale) return RF_ERR_NULL_POINTER;
+    if (rf::misaligned({q}, 16) || rf::misaligned({scale}, 4) || rf::misaligned({w}, (unsigned)bytes)) return RF_ERR_MISALIGNED;
+    if (!rf::device_state()) return RF_ERR_CUDA;
+    const bool k_major = stride_k == 1;
+    const bool vec = rf::rows_aligned(w, k_major ? stride_n : stride_k, bytes) && (e == 1 || (stride_e * bytes) % 16 == 0);
+    auto run = dtype == RF_F16 ? rf::launch_blocks<__half> : dtype == RF_BF16 ? rf::launch_blocks<__nv_bfloat16> : rf::launch_blocks<float>;
+    return run(vec, k_major, w, e, n, k, stride_e, stride_n, stride_k, q, scale, reinterpret_cast<cudaStream_t>(stream)) ==
+                   cudaSuccess ? RF_OK : RF_ERR_CUDA;
+}
+
+}  // extern "C"

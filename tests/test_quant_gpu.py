@@ -1,0 +1,190 @@
+"""FP8 quantisation against a plain computation in 64 bits.
+
+Tolerances.  scale = a / 448 is one correctly rounded fp32 division: off by at most eps32 / 2 = 2^-24 relative.  q is
+e4m3(x * r) with r = fl(448 / a): x * r is off by at most 2 * 2^-24 relative before the conversion, which rounds by half a
+step: 2^-4 relative for normal values (|v| >= 2^-6), 2^-10 absolute below.  So |q - v| <= 2^-4 |v| (1 + 2^-22) + 2^-10.
+SwiGLU: h in fp32 has an exponential (2 ulp), a sum, a division (2 ulp) and a product: 2^-21 relative is more than their sum.
+"""
+import numpy as np
+import pytest
+import torch
+
+from radeonflow_kernels_b200 import gemm, quant
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+DTYPES = [torch.float16, torch.bfloat16, torch.float32]
+
+
+def blocks_of(x):                 # [..., k] -> [..., k/128, 128]
+    return x.reshape(*x.shape[:-1], -1, 128)
+
+
+def check(q, scale, x, a, slack=0.0):
+    """q, scale (device) against x in blocks [..., 128] (float64 numpy) whose largest magnitudes are a."""
+    a = np.maximum(a, 2.0 ** -100)
+    s = scale.double().cpu().numpy()
+    np.testing.assert_allclose(s, a / 448, rtol=2.0 ** -24 * 1.01 + slack)
+    v = x * (448 / a)[..., None]
+    got = blocks_of(q.float().double().cpu().numpy())
+    bad = np.abs(got - v) > 2.0 ** -4 * np.abs(v) * (1 + 2.0 ** -22 + 2 * slack) + 2.0 ** -10
+    assert not bad.any(), (int(bad.sum()), got[bad][:4], v[bad][:4])
+
+
+def data(shape, dtype, seed):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(*shape, generator=g, device=DEV) * torch.exp(2 * torch.randn(shape[0], *[1] * (len(shape) - 1), generator=g, device=DEV))
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,k", [(1, 128), (3, 128), (1, 7168), (7, 384), (130, 1152), (2049, 2048)])
+def test_rows(dtype, m, k):
+    x = data((m, k), dtype, m + k)
+    q, s = quant.fp8_quantize(x)
+    assert q.shape == (m, k) and s.shape == (m, k // 128)
+    xb = blocks_of(x.double().cpu().numpy())
+    check(q, s, xb, np.abs(xb).max(-1))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_strided_unaligned_and_no_write_outside(dtype):
+    big = data((40, 1000), dtype, 5)
+    x = big[3:24, 5:5 + 384]                       # rows 1000 elements apart, starting at odd addresses
+    q = torch.full((30, 384), 1.0, device=DEV).to(torch.float8_e4m3fn)
+    s = torch.full((30, 3), 7.0, device=DEV)
+    quant.fp8_quantize(x, out=(q[4:25], s[4:25]))
+    xb = blocks_of(x.double().cpu().numpy())
+    check(q[4:25], s[4:25], xb, np.abs(xb).max(-1))
+    assert (q.float()[:4] == 1).all() and (q.float()[25:] == 1).all() and (s[:4] == 7).all() and (s[25:] == 7).all()
+    # a broadcast row
+    q, s = quant.fp8_quantize(x[:1].expand(9, 384))
+    assert (q.view(torch.uint8) == q.view(torch.uint8)[:1]).all() and (s == s[:1]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_gather(dtype):
+    x = data((50, 640), dtype, 6)
+    rows = torch.randint(0, 50, (333,), device=DEV, dtype=torch.int32)
+    rows[0], rows[1], rows[2] = 49, 49, 0
+    q, s = quant.fp8_quantize(x, rows=rows + 50 * 3)              # indices count modulo the number of rows
+    q1, s1 = quant.fp8_quantize(x[rows.long()].contiguous())
+    assert torch.equal(q.view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s, s1)
+    q, s = quant.fp8_quantize(x, rows=rows[:0])
+    assert q.shape == (0, 640) and s.shape == (0, 5)
+    # no index, whatever its value, reads outside x
+    wild = torch.tensor([-1, -2 ** 31, 2 ** 31 - 1], device=DEV, dtype=torch.int32)
+    q, s = quant.fp8_quantize(x, rows=wild)
+    i = [(v % 2 ** 32) % 50 for v in (-1, -2 ** 31, 2 ** 31 - 1)]
+    q1, s1 = quant.fp8_quantize(x[i].contiguous())
+    assert torch.equal(q.view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s, s1)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_special_values(dtype):
+    x = torch.randn(6, 384, device=DEV).to(dtype)
+    x[0] = 0
+    x[1, :128] = 0
+    x[2, 5] = float("nan")
+    x[3, 130] = float("inf")
+    x[4] = torch.finfo(dtype).max
+    x[5] = torch.finfo(dtype).smallest_normal / 4
+    q, s = quant.fp8_quantize(x)
+    f = q.float()
+    assert (f[0] == 0).all() and (f[1, :128] == 0).all() and torch.isfinite(s[:2]).all()
+    assert f[2, :128].isnan().all() and s[2, 0].isnan() and torch.isfinite(f[2, 128:]).all()
+    assert s[3, 1].isinf() and f[3, 130].isnan() and (f[3, 128:130] == 0).all() and torch.isfinite(f[3, :128]).all()
+    assert (f[4] == 448).all()
+    xb = blocks_of(x[5:].double().cpu().numpy())
+    check(q[5:], s[5:], xb, np.abs(xb).max(-1))
+    # blocks take the same care of them
+    w = x.repeat(1, 1)
+    q, s = quant.fp8_quantize_blocks(w[2:3])
+    assert q.float()[0, :128].isnan().all() and s[0, 0].isnan() and torch.isfinite(q.float()[0, 128:]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,f", [(1, 128), (5, 384), (131, 2048)])
+def test_swiglu(dtype, m, f):
+    gu = data((m, 2 * f), dtype, m + f).clamp_(-60, 60)
+    gu = torch.cat([gu, gu[:, :8]], 1)[:, :2 * f]               # rows 2f + 8 apart
+    q, s = quant.fp8_swiglu_quantize(gu)
+    x = gu.double().cpu().numpy()
+    h = x[:, :f] / (1 + np.exp(-x[:, :f])) * x[:, f:]
+    hb = blocks_of(h)
+    check(q, s, hb, np.abs(hb).max(-1), slack=2.0 ** -21)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("e,n,k", [(1, 1, 128), (1, 127, 256), (1, 128, 128), (3, 576, 384), (2, 200, 1024), (5, 130, 128)])
+def test_blocks(dtype, turned, e, n, k):
+    w = data((e, k, n) if turned else (e, n, k), dtype, n + k)
+    if turned:
+        w = w.transpose(1, 2)
+    q, s = quant.fp8_quantize_blocks(w)
+    assert q.shape == (e, n, k) and q.is_contiguous() and s.shape == (e, (n + 127) // 128, k // 128)
+    x = w.double().cpu().numpy()
+    for i in range(e):
+        for b in range((n + 127) // 128):
+            xb = blocks_of(x[i, 128 * b:128 * b + 128])                       # [rows, k/128, 128]
+            a = np.abs(xb).max((0, 2))
+            check(q[i, 128 * b:128 * b + 128], s[i, b][None].expand(xb.shape[0], -1), xb, np.broadcast_to(a, xb.shape[:2]))
+    one = quant.fp8_quantize_blocks(w[0])
+    assert torch.equal(one[0].view(torch.uint8), q[0].view(torch.uint8)) and torch.equal(one[1], s[0])
+
+
+def test_blocks_of_views():
+    """Rows further apart than they are long, odd starts, experts in another order."""
+    big = torch.randn(4, 150, 700, device=DEV)
+    for w in (big[1:3, 7:140, 3:3 + 512], big[::2, :130, :384], big.flip(0)[:, 2:4, :128],
+              torch.randn(3, 256, 77, device=DEV).transpose(1, 2)[:, 3:70], big[:, :128, 9:300].transpose(1, 2)):
+        q, s = quant.fp8_quantize_blocks(w)
+        q1, s1 = quant.fp8_quantize_blocks(w.contiguous())
+        assert torch.equal(q.view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s, s1)
+
+
+def test_offsets_beyond_32_bits():
+    """The last rows of a matrix of more than 2^32 bytes (and elements)."""
+    m, k = 4_300_000, 1024
+    x = torch.zeros(m, k, device=DEV, dtype=torch.float16)
+    x[-3:] = torch.randn(3, k, device=DEV, dtype=torch.float16)
+    q, s = quant.fp8_quantize(x)
+    q1, s1 = quant.fp8_quantize(x[-3:])
+    assert torch.equal(q[-3:].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s[-3:], s1)
+    assert not q[:-3].view(torch.uint8).any()
+
+
+def test_on_another_stream_and_in_a_graph():
+    x = torch.randn(64, 512, device=DEV)
+    want = quant.fp8_quantize(x)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = quant.fp8_quantize(x)
+    side.synchronize()
+    assert torch.equal(got[0].view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(got[1], want[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = quant.fp8_quantize(x)
+        twice = quant.fp8_swiglu_quantize(x)
+    x.mul_(-3)
+    graph.replay()
+    want = quant.fp8_quantize(x), quant.fp8_swiglu_quantize(x)
+    for a, b in ((got, want[0]), (twice, want[1])):
+        assert torch.equal(a[0].view(torch.uint8), b[0].view(torch.uint8)) and torch.equal(a[1], b[1])
+
+
+def test_operands_of_the_gemm():
+    """Quantised operands through the GEMM: each factor is off by at most 2^-4 relative plus 2^-10 of its block's 448 steps."""
+    m, n, k = 70, 192, 512
+    x, w = torch.randn(m, k, device=DEV, dtype=torch.bfloat16), torch.randn(k, n, device=DEV, dtype=torch.float16) * k ** -0.5
+    a, a_s = quant.fp8_quantize(x)
+    b, b_s = quant.fp8_quantize_blocks(w.t())
+    c = gemm.fp8_mm(a, b, a_s, b_s, torch.empty(m, n, device=DEV, dtype=torch.bfloat16))
+    da = (blocks_of(a.float().double().cpu().numpy()) * a_s.double().cpu().numpy()[..., None]).reshape(m, k)
+    sb = b_s.double().cpu().numpy().repeat(128, 0)[:n]
+    db = (blocks_of(b.float().double().cpu().numpy()) * sb[..., None]).reshape(n, k)
+    ref = da @ db.T
+    # bf16 rounding 2^-8 of the value; the fp32 sum over k blocks and the tensor cores' sums inside one: 2^-12 of the terms
+    assert (np.abs(c.double().cpu().numpy() - ref) <= 2.0 ** -8 * np.abs(ref) + 2.0 ** -12 * (np.abs(da) @ np.abs(db).T)).all()
