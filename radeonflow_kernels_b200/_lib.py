@@ -242,6 +242,8 @@ def _declare_fp8(L: ctypes.CDLL) -> None:
     L.rf_fp8_swiglu_quantize.argtypes = [vp, ci, ll, ci, ci, vp, vp, vp]
     L.rf_fp8_quantize_blocks.restype = ci
     L.rf_fp8_quantize_blocks.argtypes = [vp, ci, ci, ci, ci, ll, ll, ll, vp, vp, vp]
+    L.rf_fp8_grouped_gemm.restype = ci
+    L.rf_fp8_grouped_gemm.argtypes = [vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, vp]
 
 
 class RfMoeEpConfig(ctypes.Structure):
