@@ -531,6 +531,36 @@ int rf_fp8_quantize_blocks(const void *w, int dtype, int e, int n, int k, long l
 int rf_fp8_grouped_gemm(const void *a, const void *b, const float *as, const float *bs, const int *offsets, void *c,
                         int c_dtype, int m, int n_groups, int n, int k, rf_stream_t stream);
 
+/* A whole MoE layer for 1 to 32 tokens in one kernel: the layer of rf_moe_forward (router with optional bias, softmax, top-k,
+ * SwiGLU experts, shared expert, weighted sum) for a decode step, with fp16 experts or block-scaled FP8 ones.  Experts are
+ * chosen by the same rule (fp16 logits and probabilities, ties to the lowest index); between the logits and the result only
+ * the vector between an expert's two products is rounded, to fp16.  n_routed_experts: a power of two, at most 256;
+ * n_experts_per_token at most 8; n_shared_experts 0 .. 64 (the shared expert is d_expert * n_shared_experts wide).
+ * d_hidden and d_expert: multiples of 64 (fp16) or 128 (FP8).                                       */
+typedef struct RfMoeFew RfMoeFew;
+enum { RF_MOE_FEW_F16 = 0,    /* gate, up [d_hidden, d_expert], down [d_expert, d_hidden], fp16, as in MoEInputRaw        */
+       RF_MOE_FEW_E4M3 = 1 }; /* gate, up [d_expert, d_hidden], down [d_hidden, d_expert], e4m3fn, one fp32 scale per 128 x 128 */
+typedef struct {
+    int d_hidden, d_expert, n_routed_experts, n_experts_per_token, n_shared_experts;
+    int weight_type;
+} RfMoeFewConfig;
+/* HOST arrays of n_routed_experts device pointers, and the shared expert's behind them if there is one; the scale arrays
+ * only for RF_MOE_FEW_E4M3 (else NULL).  Weights, router_weight (fp16 [E, d_hidden]) and router_bias (fp32 [E] or NULL) are kept by
+ * reference.  Allocates a table on the current device and copies to it: call it outside stream capture.  */
+int rf_moe_few_create(const RfMoeFewConfig *config, const void *router_weight, const float *router_bias,
+                      const void *const *expert_gate, const void *const *expert_up, const void *const *expert_down,
+                      const float *const *gate_scale, const float *const *up_scale, const float *const *down_scale,
+                      RfMoeFew **out);
+/* Synchronises the device (it frees the table).                                                     */
+int rf_moe_few_destroy(RfMoeFew *few);
+/* Workspace of a call with n_tokens tokens.  Its first *zeroed_bytes (the same for every n_tokens) have to be zero at the first
+ * call; each call leaves them zero.  Calls that may overlap need a workspace each.  A call that loses a bounded wait
+ * (rf_device_status) marks its workspace; until it is zeroed again, calls with it write no result and report a lost wait.  */
+size_t rf_moe_few_workspace_bytes(const RfMoeFewConfig *config, int n_tokens, size_t *zeroed_bytes);
+/* x fp16 [n_tokens, d_hidden] -> out fp16 [n_tokens, d_hidden], 16-byte aligned, workspace 256.  One kernel, asynchronous.  */
+int rf_moe_few_forward(RfMoeFew *few, const void *x, int n_tokens, void *out, void *workspace, size_t workspace_bytes,
+                       rf_stream_t stream);
+
 /* Library / build identification: "rf_b200 <version> sm_100a".               */
 const char *rf_version(void);
 

@@ -8,7 +8,8 @@ from . import _lib  # noqa: F401
 from .gemm import custom_kernel as gemm_custom_kernel, fp8_mm, fp8_mm_reference_layout  # noqa: F401
 from .grouped import fp8_grouped_mm  # noqa: F401
 from .moe import custom_kernel as moe_custom_kernel, moe_forward  # noqa: F401
+from .moe_few import FewTokenMoE  # noqa: F401
 from .quant import fp8_quantize, fp8_quantize_blocks, fp8_swiglu_quantize  # noqa: F401
 
-__all__ = ["fp8_grouped_mm", "fp8_mm", "fp8_mm_reference_layout", "fp8_quantize", "fp8_quantize_blocks", "fp8_swiglu_quantize",
+__all__ = ["FewTokenMoE", "fp8_grouped_mm", "fp8_mm", "fp8_mm_reference_layout", "fp8_quantize", "fp8_quantize_blocks", "fp8_swiglu_quantize",
            "gemm_custom_kernel", "moe_custom_kernel", "moe_forward"]

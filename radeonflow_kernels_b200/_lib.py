@@ -234,6 +234,11 @@ def _declare(L: ctypes.CDLL) -> None:
     L.rf_moe_ep_combine.argtypes = [pvp, vp, vp, vp, vp, vp, ci, ci, ci, ci, vp, vp]
 
 
+class RfMoeFewConfig(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in (
+        "d_hidden", "d_expert", "n_routed_experts", "n_experts_per_token", "n_shared_experts", "weight_type")]
+
+
 def _declare_fp8(L: ctypes.CDLL) -> None:
     vp, ci, ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
     L.rf_fp8_quantize.restype = ci
@@ -244,6 +249,15 @@ def _declare_fp8(L: ctypes.CDLL) -> None:
     L.rf_fp8_quantize_blocks.argtypes = [vp, ci, ci, ci, ci, ll, ll, ll, vp, vp, vp]
     L.rf_fp8_grouped_gemm.restype = ci
     L.rf_fp8_grouped_gemm.argtypes = [vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, vp]
+    sz, config = ctypes.c_size_t, ctypes.POINTER(RfMoeFewConfig)
+    L.rf_moe_few_create.restype = ci
+    L.rf_moe_few_create.argtypes = [config] + [vp] * 8 + [ctypes.POINTER(vp)]
+    L.rf_moe_few_destroy.restype = ci
+    L.rf_moe_few_destroy.argtypes = [vp]
+    L.rf_moe_few_workspace_bytes.restype = sz
+    L.rf_moe_few_workspace_bytes.argtypes = [config, ci, ctypes.POINTER(sz)]
+    L.rf_moe_few_forward.restype = ci
+    L.rf_moe_few_forward.argtypes = [vp, vp, ci, vp, vp, sz, vp]
 
 
 class RfMoeEpConfig(ctypes.Structure):

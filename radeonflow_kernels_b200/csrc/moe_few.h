@@ -1,0 +1,49 @@
+// Internal interface of the MoE layer for a few tokens (moe_few.cu, moe_few_api.cu).
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stddef.h>
+
+namespace rf {
+
+constexpr int kFewMaxTokens = 32;
+constexpr int kFewMaxExperts = 256;
+constexpr int kFewMaxTopK = 8;
+
+// Words in front of the workspace's counters
+enum { kFewTicket = 0, kFewRouterDone = 1, kFewExits = 2, kFewBad = 3, kFewHeadWords = 8 };
+
+struct MoeFewParams {
+    const void* x;                  // fp16 [t, d]
+    const void* router;             // fp16 [experts, d]
+    const float* router_bias;       // fp32 [experts] or nullptr
+    const CUtensorMap* maps;        // device: gate, up, down of every expert, then of the shared one
+    const float* const* scales;     // device: the same order (FP8 weights)
+    void* out;                      // fp16 [t, d]
+    // workspace
+    int* head;                      // kFewHeadWords, then done [experts + 1]: finished column tiles of an expert's first product
+    int* count1;                    // [experts + 1][tiles1_max] finished K chunks of a column tile, first product
+    int* count2;                    // [tiles2] finished items of a column tile of the result
+    float* logits;                  // [router_chunks][t][experts] partial sums
+    float* part1;                   // [chunks1][pairs][2 * width] partial sums of gate | up, 64 + 64 columns per tile
+    void* h;                        // fp16 [pairs][width]
+    float* part2;                   // [chunks2][pairs][d]
+    int t, d, f, fs;                // fs: the shared expert's width, 0 = none
+    int experts, top_k;
+    int width;                      // max(f, fs)
+    int tiles1_max;                 // width / 64
+    int kc1, kc2;                   // K of an item of the first and the second product
+    int router_chunks, router_units;
+    int* status;
+    int launch_tag;
+};
+
+// Rows of the widest MMA group that t tokens need: 1, 2 or 4 groups of 8.
+inline int moe_few_groups(int t) { return t <= 8 ? 1 : t <= 16 ? 2 : 4; }
+// Largest K chunk whose two operand buffers leave room for the weight stages.
+inline int moe_few_max_chunk(int t) { return t <= 16 ? 1024 : 512; }
+constexpr int kFewRouterChunk = 512;
+
+cudaError_t moe_few_launch(const MoeFewParams& p, bool fp8, int num_sms, cudaStream_t stream);
+
+}  // namespace rf

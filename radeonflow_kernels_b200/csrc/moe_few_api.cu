@@ -1,0 +1,215 @@
+// C-ABI of the MoE layer for a few tokens: one object per layer holds what every call needs of its weights (tensor maps,
+// addresses of the scales) on the device; the caller holds the workspace.
+#include "../../include/rf_b200.h"
+#include "host_util.h"
+#include "moe_few.h"
+
+#include <cstdio>
+#include <new>
+#include <vector>
+
+struct RfMoeFew {
+    RfMoeFewConfig cfg;
+    int device;
+    const void* router;
+    const float* router_bias;
+    CUtensorMap* maps;
+    const float** scales;
+};
+
+namespace {
+
+size_t align_up(size_t v) { return (v + 255) / 256 * 256; }
+
+// What a call of t tokens needs: K chunks, and where the parts of the workspace lie.
+struct Plan {
+    int kc1, kc2, router_chunks;
+    size_t zeroed, count1, count2, logits, part1, h, part2, bytes;
+};
+
+// The longest K chunk that still gives `tiles` column tiles enough items for an even load on every SM; chunks below 256 would
+// be all hand-over.
+int choose_chunk(int tiles, int k, int most, int num_sms) {
+    int kc = most;
+    while (kc > 256 && (long long)tiles * ((k + kc - 1) / kc) < 4LL * num_sms) kc /= 2;
+    return kc;
+}
+
+Plan make_plan(const RfMoeFewConfig& c, int t) {
+    const int num_sms = 148;
+    const int fs = c.d_expert * c.n_shared_experts, width = fs > c.d_expert ? fs : c.d_expert;
+    const int hit = c.n_routed_experts < t * c.n_experts_per_token ? c.n_routed_experts : t * c.n_experts_per_token;
+    const int most = rf::moe_few_max_chunk(t);
+    const size_t pairs = (size_t)t * (c.n_experts_per_token + 1), d = c.d_hidden;
+    Plan p;
+    p.kc1 = choose_chunk((hit * c.d_expert + fs) / 64, c.d_hidden, most, num_sms);
+    p.kc2 = choose_chunk((hit + (fs > 0)) * ((c.d_hidden + 127) / 128), c.d_expert, most, num_sms);
+    p.router_chunks = (c.d_hidden + rf::kFewRouterChunk - 1) / rf::kFewRouterChunk;
+    const size_t chunks1 = (d + p.kc1 - 1) / p.kc1, chunks2 = ((size_t)width + p.kc2 - 1) / p.kc2;
+    // counters first: their place does not depend on t
+    size_t b = align_up((rf::kFewHeadWords + c.n_routed_experts + 1) * sizeof(int));
+    auto take = [&](size_t n) { const size_t at = b; b += align_up(n); return at; };
+    p.count1 = take((size_t)(c.n_routed_experts + 1) * (width / 64) * sizeof(int));
+    p.count2 = take((d + 127) / 128 * sizeof(int));
+    p.zeroed = b;
+    p.logits = take((size_t)p.router_chunks * t * c.n_routed_experts * sizeof(float));
+    p.part1 = take(chunks1 * pairs * 2 * width * sizeof(float));
+    p.h = take(pairs * width * 2);
+    p.part2 = take(chunks2 * pairs * d * sizeof(float));
+    p.bytes = b;
+    return p;
+}
+
+int check_config(const RfMoeFewConfig& c) {
+    if (c.weight_type != RF_MOE_FEW_F16 && c.weight_type != RF_MOE_FEW_E4M3) return RF_ERR_UNSUPPORTED;
+    const int step = c.weight_type == RF_MOE_FEW_E4M3 ? 128 : 64;
+    if (c.d_hidden <= 0 || c.d_hidden % step != 0 || c.d_expert <= 0 || c.d_expert % step != 0) return RF_ERR_BAD_SHAPE;
+    if (c.n_shared_experts < 0 || c.n_shared_experts > 64 || c.d_hidden > (1 << 20) || c.d_expert > (1 << 20)) return RF_ERR_BAD_SHAPE;
+    const int e = c.n_routed_experts;
+    if (e < 1 || e > rf::kFewMaxExperts || (e & (e - 1)) != 0) return RF_ERR_UNSUPPORTED;
+    if (c.n_experts_per_token < 1 || c.n_experts_per_token > rf::kFewMaxTopK || c.n_experts_per_token > e) return RF_ERR_UNSUPPORTED;
+    return RF_OK;
+}
+
+bool encode(CUtensorMap* m, bool fp8, const void* base, int k, int n) {
+    return fp8 ? rf::encode_tma_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, (uint64_t)n, (uint64_t)k, (uint64_t)k, 64, 128, true)
+               : rf::encode_tma_2d(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base, (uint64_t)k, (uint64_t)n, (uint64_t)n * 2, 64, 64, true);
+}
+
+}  // namespace
+
+extern "C" {
+
+int rf_moe_few_create(const RfMoeFewConfig* config, const void* router_weight, const float* router_bias,
+                      const void* const* expert_gate, const void* const* expert_up, const void* const* expert_down,
+                      const float* const* gate_scale, const float* const* up_scale, const float* const* down_scale,
+                      RfMoeFew** out) {
+    if (!config || !out) return RF_ERR_NULL_POINTER;
+    *out = nullptr;
+    const int rc = check_config(*config);
+    if (rc != RF_OK) return rc;
+    const RfMoeFewConfig& c = *config;
+    const bool fp8 = c.weight_type == RF_MOE_FEW_E4M3;
+    if (!router_weight || !expert_gate || !expert_up || !expert_down || (fp8 && (!gate_scale || !up_scale || !down_scale)))
+        return RF_ERR_NULL_POINTER;
+    const int sets = c.n_routed_experts + (c.n_shared_experts > 0 ? 1 : 0);
+    for (int e = 0; e < sets; ++e) {
+        if (!expert_gate[e] || !expert_up[e] || !expert_down[e]) return RF_ERR_NULL_POINTER;
+        if (rf::misaligned({expert_gate[e], expert_up[e], expert_down[e]}, 16)) return RF_ERR_MISALIGNED;
+        if (!fp8) continue;
+        if (!gate_scale[e] || !up_scale[e] || !down_scale[e]) return RF_ERR_NULL_POINTER;
+        if (rf::misaligned({gate_scale[e], up_scale[e], down_scale[e]}, 4)) return RF_ERR_MISALIGNED;
+    }
+    if (rf::misaligned({router_weight}, 16) || rf::misaligned({router_bias}, 4)) return RF_ERR_MISALIGNED;
+    if (!rf::device_state()) return RF_ERR_CUDA;
+    std::vector<CUtensorMap> maps;
+    std::vector<const float*> scales;
+    try {
+        maps.resize((size_t)3 * sets);
+        scales.resize((size_t)3 * sets, nullptr);
+    } catch (const std::bad_alloc&) {
+        return RF_ERR_CUDA;
+    }
+    for (int e = 0; e < sets; ++e) {
+        const int f = e < c.n_routed_experts ? c.d_expert : c.d_expert * c.n_shared_experts;
+        if (!encode(&maps[3 * e], fp8, expert_gate[e], c.d_hidden, f) || !encode(&maps[3 * e + 1], fp8, expert_up[e], c.d_hidden, f) ||
+            !encode(&maps[3 * e + 2], fp8, expert_down[e], f, c.d_hidden))
+            return RF_ERR_CUDA;
+        if (fp8) {
+            scales[3 * e] = gate_scale[e];
+            scales[3 * e + 1] = up_scale[e];
+            scales[3 * e + 2] = down_scale[e];
+        }
+    }
+    RfMoeFew* few = new (std::nothrow) RfMoeFew();
+    if (!few) return RF_ERR_CUDA;
+    few->cfg = c;
+    few->router = router_weight;
+    few->router_bias = router_bias;
+    cudaGetDevice(&few->device);
+    const size_t map_bytes = maps.size() * sizeof(CUtensorMap), scale_bytes = scales.size() * sizeof(float*);
+    char* dev = nullptr;
+    if (cudaMalloc(&dev, map_bytes + scale_bytes) != cudaSuccess) {
+        cudaGetLastError();
+        delete few;
+        return RF_ERR_CUDA;
+    }
+    few->maps = reinterpret_cast<CUtensorMap*>(dev);
+    few->scales = reinterpret_cast<const float**>(dev + map_bytes);
+    if (cudaMemcpy(dev, maps.data(), map_bytes, cudaMemcpyHostToDevice) != cudaSuccess ||
+        cudaMemcpy(dev + map_bytes, scales.data(), scale_bytes, cudaMemcpyHostToDevice) != cudaSuccess) {
+        cudaFree(dev);
+        delete few;
+        return RF_ERR_CUDA;
+    }
+    *out = few;
+    return RF_OK;
+}
+
+int rf_moe_few_destroy(RfMoeFew* few) {
+    if (!few) return RF_OK;
+    const cudaError_t e = cudaFree(few->maps);
+    delete few;
+    return e == cudaSuccess ? RF_OK : RF_ERR_CUDA;
+}
+
+size_t rf_moe_few_workspace_bytes(const RfMoeFewConfig* config, int n_tokens, size_t* zeroed_bytes) {
+    if (zeroed_bytes) *zeroed_bytes = 0;
+    if (!config || check_config(*config) != RF_OK || n_tokens < 1 || n_tokens > rf::kFewMaxTokens) return 0;
+    const Plan p = make_plan(*config, n_tokens);
+    if (zeroed_bytes) *zeroed_bytes = p.zeroed;
+    return p.bytes;
+}
+
+int rf_moe_few_forward(RfMoeFew* few, const void* x, int n_tokens, void* out, void* workspace, size_t workspace_bytes,
+                       rf_stream_t stream) {
+    if (!few) return RF_ERR_NULL_POINTER;
+    if (n_tokens < 0 || n_tokens > rf::kFewMaxTokens) return RF_ERR_BAD_SHAPE;
+    if (n_tokens == 0) return RF_OK;
+    if (!x || !out || !workspace) return RF_ERR_NULL_POINTER;
+    if (rf::misaligned({x, out}, 16) || rf::misaligned({workspace}, 256)) return RF_ERR_MISALIGNED;
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev != few->device) return RF_ERR_UNSUPPORTED;
+    const RfMoeFewConfig& c = few->cfg;
+    const Plan plan = make_plan(c, n_tokens);
+    if (workspace_bytes < plan.bytes) return RF_ERR_WORKSPACE;
+    rf::DeviceState* st = rf::device_state();
+    if (!st) return RF_ERR_CUDA;
+    char* ws = static_cast<char*>(workspace);
+    rf::MoeFewParams p;
+    p.x = x;
+    p.router = few->router;
+    p.router_bias = few->router_bias;
+    p.maps = few->maps;
+    p.scales = few->scales;
+    p.out = out;
+    p.head = reinterpret_cast<int*>(ws);
+    p.count1 = reinterpret_cast<int*>(ws + plan.count1);
+    p.count2 = reinterpret_cast<int*>(ws + plan.count2);
+    p.logits = reinterpret_cast<float*>(ws + plan.logits);
+    p.part1 = reinterpret_cast<float*>(ws + plan.part1);
+    p.h = ws + plan.h;
+    p.part2 = reinterpret_cast<float*>(ws + plan.part2);
+    p.t = n_tokens;
+    p.d = c.d_hidden;
+    p.f = c.d_expert;
+    p.fs = c.d_expert * c.n_shared_experts;
+    p.experts = c.n_routed_experts;
+    p.top_k = c.n_experts_per_token;
+    p.width = p.fs > p.f ? p.fs : p.f;
+    p.tiles1_max = p.width / 64;
+    p.kc1 = plan.kc1;
+    p.kc2 = plan.kc2;
+    p.router_chunks = plan.router_chunks;
+    p.router_units = (p.experts + 15) / 16 * p.router_chunks;
+    p.status = st->status;
+    p.launch_tag = rf::next_launch_tag();
+    const cudaError_t e = rf::moe_few_launch(p, c.weight_type == RF_MOE_FEW_E4M3, st->num_sms, reinterpret_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) {
+        fprintf(stderr, "rf_b200: launch of the layer for a few tokens failed: %s\n", cudaGetErrorString(e));
+        return RF_ERR_CUDA;
+    }
+    return RF_OK;
+}
+
+}  // extern "C"

@@ -9,6 +9,7 @@
 //   tile_list_kernel     per-expert row ranges -> list of row tiles for the grouped GEMM
 #include "moe_kernels.h"
 #include "ptx.cuh"
+#include "softmax_exp.cuh"
 
 #include <cuda_fp16.h>
 #include <stdint.h>
@@ -18,25 +19,6 @@ namespace rf {
 // Kernels that may start before the one in front of them has finished take what it writes through plain pointers (a load
 // from const __restrict__ memory may be moved in front of griddep_wait()).
 namespace {
-
-// exp(x), x <= 0, as a fixed sequence of fp32 operations with no fused multiply-add, so a CPU
-// restatement reproduces it bit for bit: t = max(x,-80)*log2e; n = rint(t); f = t-n; degree-7
-// Horner for 2^f; exact scaling by 2^n.
-__device__ __forceinline__ float det_exp(float x) {
-    x = fmaxf(x, -80.0f);
-    const float t = __fmul_rn(x, 1.4426950408889634f);
-    const float n = rintf(t);
-    const float f = __fsub_rn(t, n);
-    float p = 1.5252733804059840e-05f;
-    p = __fadd_rn(__fmul_rn(p, f), 0.0001540353039338161f);
-    p = __fadd_rn(__fmul_rn(p, f), 0.0013333558146428443f);
-    p = __fadd_rn(__fmul_rn(p, f), 0.009618129107628477f);
-    p = __fadd_rn(__fmul_rn(p, f), 0.05550410866482158f);
-    p = __fadd_rn(__fmul_rn(p, f), 0.2402265069591007f);
-    p = __fadd_rn(__fmul_rn(p, f), 0.6931471805599453f);
-    p = __fadd_rn(__fmul_rn(p, f), 1.0f);
-    return __uint_as_float(__float_as_uint(p) + (static_cast<int>(n) << 23));   // p in [0.7, 1.42], result normal
-}
 
 // The sort's blocks: block b of `n_blocks` holds the items [b * items, (b + 1) * items), those of whole tokens where the
 // counts come from topk_kernel.  At most 256 blocks: every block of the scatter reads all blocks' counts.

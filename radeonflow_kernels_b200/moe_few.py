@@ -1,0 +1,144 @@
+"""The MoE layer for a few tokens, a decode step, in one kernel.
+
+``FewTokenMoE`` computes the layer of `moe.moe_forward` (router, softmax and top-k, SwiGLU experts, shared expert, weighted sum)
+for 1 to 32 tokens.  The experts are the layer's fp16 weights or block-scaled FP8 ones (`moe_fp8.quantize_experts`); tokens
+and results are fp16, products are summed in fp32.  It chooses experts by the layer's rule: fp16 logits, probabilities rounded
+to fp16, equal ones by the lowest index.  Unlike the layer it rounds nothing between the logits and the result but the
+vector between an expert's two products, to fp16.
+"""
+import ctypes
+
+import torch
+
+from . import _lib
+from .moe import _check_fp16_cuda
+
+MAX_TOKENS = 32
+BLOCK = 128
+_SHARED = "shared_experts"
+
+
+class FewTokenMoE:
+    """One layer's handle: what its kernel needs of the weights, which have to stay where they are.
+
+    ``weights``: the layer's dict ('router.weight', 'experts.{i}.{0,1,2}.weight', 'shared_experts.{0,1,2}.weight', fp16), or the
+    dict of FP8 experts ('router.weight' fp16; 'experts.gate_up.weight' e4m3fn [E, 2f, d], gate rows first,
+    'experts.gate_up.scale' fp32 [E, 2f/128, d/128], 'experts.down.weight' [E, d, f], 'experts.down.scale' and the same under
+    'shared_experts' without the leading axis).  ``config``: d_hidden, d_expert, n_routed_experts (a power of two, at most 256),
+    n_experts_per_token (at most 8), n_shared_experts (0: no shared expert).  ``router_bias``: fp32 [E], added to the logits.
+
+    Calls on different streams may overlap: each stream has a workspace of its own, and so has each captured call.
+    """
+
+    def __init__(self, weights, config, router_bias=None):
+        d, f, e = (int(config[k]) for k in ("d_hidden", "d_expert", "n_routed_experts"))
+        n_shared = int(config["n_shared_experts"])
+        self._handle = None
+        self.fp8 = "experts.gate_up.weight" in weights
+        self.config = _lib.RfMoeFewConfig(d, f, e, int(config["n_experts_per_token"]), n_shared, int(self.fp8))
+        self.d_hidden, self._workspaces, self._sizes = d, {}, {}
+        router = weights["router.weight"]
+        _check_fp16_cuda("router.weight", router)
+        self.device = router.device
+        self._check_device("the weights")
+        if tuple(router.shape) != (e, d):
+            raise ValueError(f"moe: router.weight must be [{e}, {d}]")
+        if router_bias is not None and not (router_bias.dtype == torch.float32 and tuple(router_bias.shape) == (e,)
+                                            and router_bias.is_contiguous() and router_bias.device == self.device):
+            raise ValueError(f"moe: router_bias must be a contiguous float32 vector of {e} on the weights' device")
+        take = self._fp8_matrices if self.fp8 else self._fp16_matrices
+        matrices, scales = take(weights, d, f, e, n_shared)
+        self._keep = (router, router_bias, matrices, scales)
+        arrays = [(ctypes.c_void_p * len(m))(*m) for m in zip(*[[t.data_ptr() for t in row] for row in matrices])]
+        scale_arrays = [(ctypes.c_void_p * len(m))(*m) for m in zip(*[[t.data_ptr() for t in row] for row in scales])] or [None] * 3
+        handle = ctypes.c_void_p()
+        st = _lib.lib().rf_moe_few_create(ctypes.byref(self.config), router.data_ptr(),
+                                          None if router_bias is None else router_bias.data_ptr(), *arrays, *scale_arrays,
+                                          ctypes.byref(handle))
+        _lib.check(st, "rf_moe_few_create")
+        self._handle = handle
+
+    def _check_device(self, what):
+        if self.device.index != torch.cuda.current_device():
+            raise ValueError(f"moe: {what} must be on the current device")
+
+    def _fp16_matrices(self, weights, d, f, e, n_shared):
+        rows = []
+        for prefix, width in [(f"experts.{i}", f) for i in range(e)] + [(_SHARED, f * n_shared)] * (n_shared > 0):
+            row = [weights[f"{prefix}.{j}.weight"] for j in range(3)]
+            for j, (t, shape) in enumerate(zip(row, ((d, width), (d, width), (width, d)))):
+                _check_fp16_cuda(f"{prefix}.{j}.weight", t)
+                if tuple(t.shape) != shape or t.device != self.device:
+                    raise ValueError(f"moe: {prefix}.{j}.weight must be {list(shape)} on the router weight's device")
+            rows.append(row)
+        return rows, []
+
+    def _fp8_matrices(self, weights, d, f, e, n_shared):
+        def stack(prefix, name, *shape):
+            w, s = weights[f"{prefix}.{name}.weight"], weights[f"{prefix}.{name}.scale"]
+            blocks = (*shape[:-2], (shape[-2] + BLOCK - 1) // BLOCK, shape[-1] // BLOCK)
+            for t, dtype, want in ((w, torch.float8_e4m3fn, shape), (s, torch.float32, blocks)):
+                if not (t.is_cuda and t.dtype == dtype and t.is_contiguous() and tuple(t.shape) == want and t.device == self.device):
+                    raise ValueError(f"moe: {prefix}.{name} must be a contiguous {dtype} tensor {list(want)} on the router "
+                                     "weight's device")
+            return w, s
+
+        if d % BLOCK or f % BLOCK:
+            raise ValueError("moe: FP8 experts need d_hidden and d_expert in multiples of 128")
+        gu, gus = stack("experts", "gate_up", e, 2 * f, d)
+        dn, dns = stack("experts", "down", e, d, f)
+        rows = [[gu[i, :f], gu[i, f:], dn[i]] for i in range(e)]
+        scales = [[gus[i, :f // BLOCK], gus[i, f // BLOCK:], dns[i]] for i in range(e)]
+        if n_shared > 0:
+            fs = f * n_shared
+            gu, gus = stack(_SHARED, "gate_up", 2 * fs, d)
+            dn, dns = stack(_SHARED, "down", d, fs)
+            rows.append([gu[:fs], gu[fs:], dn])
+            scales.append([gus[:fs // BLOCK], gus[fs // BLOCK:], dns])
+        return rows, scales
+
+    def _workspace(self, n_tokens, stream):
+        size = self._sizes.get(n_tokens)
+        if size is None:
+            zeroed = ctypes.c_size_t()
+            n = _lib.lib().rf_moe_few_workspace_bytes(ctypes.byref(self.config), n_tokens, ctypes.byref(zeroed))
+            size = self._sizes[n_tokens] = (n, zeroed.value)
+        captured = torch.cuda.is_current_stream_capturing()
+        ws = None if captured else self._workspaces.get(stream)
+        if ws is None or ws.numel() < size[0]:
+            ws = torch.empty(size[0], dtype=torch.uint8, device=self.device)
+            ws[:size[1]].zero_()
+            if not captured:        # (a captured call's is the graph's: every replay zeroes it again)
+                self._workspaces[stream] = ws
+        return ws
+
+    def reset(self):
+        """Forgets the workspaces.  Needed after `gemm.device_status()` has told of a lost wait: until then every call with a
+        workspace that such a call left behind refuses to run and reports a lost wait again."""
+        self._workspaces.clear()
+
+    def forward(self, x, out=None):
+        """x fp16 [..., d_hidden], 1 to 32 tokens -> out, same shape.  Enqueues one kernel on the current stream."""
+        if not (x.is_cuda and x.dtype == torch.float16 and x.is_contiguous() and x.device == self.device):
+            raise ValueError("moe: input must be a contiguous CUDA fp16 tensor on the weights' device (there is no CPU path)")
+        self._check_device("the input")
+        if x.shape[-1] != self.d_hidden:
+            raise ValueError(f"moe: input must be [..., {self.d_hidden}]")
+        n_tokens = x.numel() // self.d_hidden
+        if n_tokens > MAX_TOKENS:
+            raise ValueError(f"moe: at most {MAX_TOKENS} tokens (moe_forward and Fp8MoE take more)")
+        if out is None:
+            out = torch.empty_like(x)
+        elif not (out.dtype == torch.float16 and out.shape == x.shape and out.is_contiguous() and out.device == x.device):
+            raise ValueError("moe: out must be a contiguous fp16 tensor like the input")
+        if n_tokens == 0:
+            return out
+        stream = _lib.current_stream()
+        ws = self._workspace(n_tokens, stream)
+        st = _lib.lib().rf_moe_few_forward(self._handle, x.data_ptr(), n_tokens, out.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+        _lib.check(st, "rf_moe_few_forward")
+        return out
+
+    def __del__(self):
+        if getattr(self, "_handle", None):
+            _lib.lib().rf_moe_few_destroy(self._handle)

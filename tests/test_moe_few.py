@@ -1,0 +1,91 @@
+"""Refusals of the layer for a few tokens, all before any device work, and the arithmetic of its workspace."""
+import ctypes
+
+import pytest
+import torch
+
+from radeonflow_kernels_b200 import _lib, moe_few
+
+A = 0x7000000                # aligned for everything; nothing stands behind it
+
+
+def config(d=256, f=128, e=8, k=2, ns=1, wt=0):
+    return _lib.RfMoeFewConfig(d, f, e, k, ns, wt)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(d=100), 1), (dict(d=0), 1), (dict(f=96), 1), (dict(f=192, wt=1), 1), (dict(d=192, wt=1), 1), (dict(ns=-1), 1), (dict(ns=65), 1),
+    (dict(d=2 ** 21), 1), (dict(e=6), 7), (dict(e=512), 7), (dict(e=0), 7), (dict(k=0), 7), (dict(k=9), 7), (dict(e=2, k=4), 7), (dict(wt=2), 7)])
+def test_config(rf_lib, kw, status):
+    c, h = config(**kw), ctypes.c_void_p()
+    assert rf_lib.rf_moe_few_create(ctypes.byref(c), A, None, A, A, A, A, A, A, ctypes.byref(h)) == status and not h
+    assert rf_lib.rf_moe_few_workspace_bytes(ctypes.byref(c), 4, None) == 0
+
+
+def test_pointers(rf_lib):
+    h = ctypes.c_void_p()
+    ptrs = lambda n, bad=None, at=0: (ctypes.c_void_p * n)(*[bad if i == at and bad is not None else A for i in range(n)])
+    null = (ctypes.c_void_p * 9)(*[A] * 8, None)
+
+    def create(router=A, bias=None, g=ptrs(9), u=ptrs(9), dn=ptrs(9), s=(None,) * 3, wt=0):
+        c = config(wt=wt)
+        return rf_lib.rf_moe_few_create(ctypes.byref(c), router, bias, g, u, dn, *s, ctypes.byref(h))
+
+    assert create(router=None) == 2 and create(g=None) == 2 and create(u=None) == 2 and create(dn=null) == 2
+    assert create(wt=1) == 2 and create(wt=1, s=(ptrs(9), ptrs(9), null)) == 2
+    assert create(router=A + 8) == 3 and create(bias=A + 2) == 3 and create(g=ptrs(9, A + 8, 8)) == 3 and create(dn=ptrs(9, A + 4)) == 3
+    assert create(wt=1, s=(ptrs(9), ptrs(9, A + 2, 3), ptrs(9))) == 3
+    assert rf_lib.rf_moe_few_create(None, A, None, A, A, A, None, None, None, ctypes.byref(h)) == 2
+    assert rf_lib.rf_moe_few_destroy(None) == 0
+    assert rf_lib.rf_moe_few_forward(None, A, 1, A, A, 1 << 30, None) == 2
+
+
+def test_workspace_bytes(rf_lib):
+    c = config(d=7168, f=2048, e=256, k=8)
+    z, zs, last = ctypes.c_size_t(), set(), 0
+    for t in range(1, 33):
+        n = rf_lib.rf_moe_few_workspace_bytes(ctypes.byref(c), t, ctypes.byref(z))
+        zs.add(z.value)
+        assert n % 256 == 0 and 0 < z.value < n
+        # partial sums of at least one K chunk each, and h
+        assert n >= t * 9 * (2 * 2048 * 4 + 2048 * 2 + 7168 * 4)
+    assert len(zs) == 1 and zs.pop() >= 4 * (8 + 257 + 257 * 32 + 56)
+    for t in (0, 33, -1):
+        assert rf_lib.rf_moe_few_workspace_bytes(ctypes.byref(c), t, ctypes.byref(z)) == 0 and z.value == 0
+
+
+class Meta(torch.Tensor):
+    """A tensor that says it lies on the GPU."""
+    is_cuda = True
+
+
+def test_python_weights(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: None)       # the index of the CPU's device
+    t = lambda *s, dtype=torch.float16: torch.zeros(*s, dtype=dtype).as_subclass(Meta)
+    cfg = {"d_hidden": 128, "d_expert": 64, "n_routed_experts": 2, "n_experts_per_token": 1, "n_shared_experts": 1}
+    good = {"router.weight": t(2, 128)}
+    for p in ("experts.0", "experts.1", "shared_experts"):
+        good.update({f"{p}.0.weight": t(128, 64), f"{p}.1.weight": t(128, 64), f"{p}.2.weight": t(64, 128)})
+    for name, bad, match in (("router.weight", t(3, 128), "router"), ("experts.1.2.weight", t(128, 64), "experts.1.2"),
+                             ("shared_experts.0.weight", t(128, 128), "shared_experts.0"),
+                             ("experts.0.1.weight", t(128, 64, dtype=torch.float32), "fp16"),
+                             ("experts.0.1.weight", t(64, 128).t(), "contiguous"),
+                             ("experts.0.0.weight", torch.zeros(128, 64, dtype=torch.float16), "CUDA")):
+        with pytest.raises(ValueError, match=match):
+            moe_few.FewTokenMoE({**good, name: bad}, cfg)
+    with pytest.raises(KeyError):
+        moe_few.FewTokenMoE({k: v for k, v in good.items() if k != "experts.1.0.weight"}, cfg)
+    with pytest.raises(ValueError, match="router_bias"):
+        moe_few.FewTokenMoE(good, cfg, router_bias=t(2))
+    f8 = torch.float8_e4m3fn
+    cfg["d_expert"] = 128
+    good8 = {"router.weight": t(2, 128), "experts.gate_up.weight": t(2, 256, 128, dtype=f8), "experts.gate_up.scale": t(2, 2, 1, dtype=torch.float32),
+             "experts.down.weight": t(2, 128, 128, dtype=f8), "experts.down.scale": t(2, 1, 1, dtype=torch.float32),
+             "shared_experts.gate_up.weight": t(256, 128, dtype=f8), "shared_experts.gate_up.scale": t(2, 1, dtype=torch.float32),
+             "shared_experts.down.weight": t(128, 128, dtype=f8), "shared_experts.down.scale": t(1, 1, dtype=torch.float32)}
+    for name, bad in (("experts.gate_up.scale", t(2, 1, 1, dtype=torch.float32)), ("experts.down.weight", t(2, 128, 128)),
+                      ("shared_experts.down.scale", t(1, 1, 1, dtype=torch.float32))):
+        with pytest.raises(ValueError, match=name.rsplit(".", 1)[0]):
+            moe_few.FewTokenMoE({**good8, name: bad}, cfg)
+    with pytest.raises(ValueError, match="multiples of 128"):
+        moe_few.FewTokenMoE(good8, {**cfg, "d_expert": 64})

@@ -1,0 +1,252 @@
+"""The layer for a few tokens against a plain computation in 64 bits.
+
+Routing is compared exactly: x and the router hold small multiples of powers of two, so that every sum of a logit is exact in
+fp32, and `oracle.moe.route` reproduces softmax, rounding and ties bit for bit.
+
+Tolerance of the result, with u = 2^-11 (fp16), s(K) = (K/16 + 40) 2^-23: an fp32 sum of K products, 16 to an MMA, cut off at
+every step, and 40 more additions of partial sums:
+    dg <= s(d) sum |x||Wg|, du likewise;  dh <= u |h| + 2^-24 + 1.1 dg |u| + |silu(g)| du + 2^-20 |h|     (1.1 >= |silu'|)
+    dy <= sum dh |Wd| + s(f) sum |h||Wd|;  dout <= u |out| + 2^-25 + (1 + 2^-20) sum_i p_i dy_i
+"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import moe as o
+from radeonflow_kernels_b200 import gemm, moe, moe_few, quant
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = 2.0 ** -11
+
+
+def make(t, d, f, e, k, ns, fp8, seed, router_scale=2.0 ** -5):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    ri = lambda lo, hi, *s: torch.randint(lo, hi, s, generator=g, device=DEV)
+    cfg = {"d_hidden": d, "d_expert": f, "n_routed_experts": e, "n_experts_per_token": k, "n_shared_experts": ns}
+    x = (ri(-8, 9, t, d) / 8).half()
+    router = (ri(-1, 2, e, d) * router_scale).half()
+    rn = lambda rows, cols, fan: torch.randn(rows, cols, generator=g, device=DEV).mul_(fan ** -0.5)
+    sets = [(f"experts.{i}", f) for i in range(e)] + [("shared_experts", f * ns)] * (ns > 0)
+    dense = {}         # prefix -> gate, up [d, width], down [width, d] in fp64, as the kernel's weights stand for
+    w = {"router.weight": router}
+    if not fp8:
+        for prefix, width in sets:
+            mats = [rn(d, width, d).half(), rn(d, width, d).half(), rn(width, d, max(width, 1)).half()]
+            for j, m in enumerate(mats):
+                w[f"{prefix}.{j}.weight"] = m
+            dense[prefix] = [m.double() for m in mats]
+        return x, w, cfg, dense
+
+    def pack(prefix, q, s, name, lead):
+        w[f"{prefix}.{name}.weight"], w[f"{prefix}.{name}.scale"] = (q, s) if lead else (q[0], s[0])
+        return (q.float().double().unflatten(-1, (-1, 128)) * s.double().repeat_interleave(128, -2)[..., None]).flatten(-2)
+
+    for prefix, n, width in (("experts", e, f),) + ((("shared_experts", 1, f * ns),) if ns else ()):
+        gu = torch.stack([rn(2 * width, d, d) for _ in range(n)])
+        dn = torch.stack([rn(d, width, width) for _ in range(n)])
+        gu = pack(prefix, *quant.fp8_quantize_blocks(gu), "gate_up", n == e and prefix == "experts")
+        dn = pack(prefix, *quant.fp8_quantize_blocks(dn), "down", n == e and prefix == "experts")
+        for i in range(n):
+            dense[f"experts.{i}" if prefix == "experts" else prefix] = [gu[i, :width].t(), gu[i, width:].t(), dn[i].t()]
+    return x, w, cfg, dense
+
+
+def reference(x, w, cfg, dense, bias=None):
+    """fp64 result, and how far the kernel may be from it."""
+    t, d = x.shape
+    k = cfg["n_experts_per_token"]
+    logits = x.double() @ w["router.weight"].double().t()
+    logits = logits.float()                 # exact
+    if bias is not None:
+        logits = logits + bias
+    idx, p, _ = o.route(logits.half().cpu().numpy(), k)
+    s = lambda n: (n / 16 + 40) * 2.0 ** -23
+    out, tol = torch.zeros(t, d, dtype=torch.float64, device=DEV), torch.zeros(t, d, dtype=torch.float64, device=DEV)
+
+    def add(rows, weight, mats):
+        gate, up, down = mats
+        xs = x[rows].double()
+        g, u = xs @ gate, xs @ up
+        sig = 1 / (1 + torch.exp(-g))
+        h = g * sig * u
+        dg, du = s(d) * (xs.abs() @ gate.abs()), s(d) * (xs.abs() @ up.abs())
+        dh = (U + 2.0 ** -20) * h.abs() + 2.0 ** -24 + 1.1 * dg * u.abs() + (g * sig).abs() * du
+        dy = dh @ down.abs() + s(gate.shape[1]) * (h.abs() @ down.abs())
+        out[rows] += weight[:, None] * (h @ down)
+        tol[rows] += weight[:, None] * dy * (1 + 2.0 ** -20)
+
+    for e in np.unique(idx):
+        tt, kk = np.nonzero(idx == e)
+        add(torch.from_numpy(tt).to(DEV), torch.from_numpy(p[tt, kk].astype(np.float64)).to(DEV), dense[f"experts.{e}"])
+    if cfg["n_shared_experts"]:
+        add(torch.arange(t, device=DEV), torch.ones(t, dtype=torch.float64, device=DEV), dense["shared_experts"])
+    return out, tol + U * out.abs() + 2.0 ** -25, idx
+
+
+def check(got, ref, tol):
+    err = (got.double() - ref).abs()
+    bad = ~(err <= tol)
+    assert not bad.any(), (int(bad.sum()), float((err / tol).max()))
+
+
+SHAPES = [
+    # t, d, f, e, k, shared
+    (1, 128, 128, 4, 1, 1), (1, 1024, 512, 8, 2, 1), (2, 256, 128, 256, 8, 0), (3, 384, 256, 32, 4, 2), (7, 640, 128, 16, 8, 1),
+    (8, 512, 384, 64, 8, 1), (9, 256, 256, 1, 1, 1), (16, 1152, 128, 128, 4, 1), (17, 128, 640, 8, 8, 0), (31, 256, 256, 32, 3, 3),
+    (32, 1024, 256, 256, 8, 1), (32, 2176, 1152, 4, 4, 1),
+]
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("t,d,f,e,k,ns", SHAPES)
+def test_against_64_bits(t, d, f, e, k, ns, fp8):
+    x, w, cfg, dense = make(t, d, f, e, k, ns, fp8, seed=t + d)
+    ref, tol, _ = reference(x, w, cfg, dense)
+    layer = moe_few.FewTokenMoE(w, cfg)
+    full = torch.full((t + 2, d), 77.0, device=DEV, dtype=torch.float16)
+    got = layer.forward(x, out=full[1:t + 1])
+    torch.cuda.synchronize()
+    assert gemm.device_status() == 0
+    check(got, ref, tol)
+    assert (full[0] == 77).all() and (full[-1] == 77).all()
+    again = layer.forward(x)                # the workspace as the first call left it
+    assert torch.equal(again, got)
+
+
+@pytest.mark.parametrize("t,d,f,e,k,ns", [(1, 64, 64, 4, 2, 1), (5, 192, 64, 8, 3, 1), (20, 320, 192, 16, 2, 2)])
+def test_widths_of_64(t, d, f, e, k, ns):
+    """fp16 widths that end inside a tile of 128 columns."""
+    x, w, cfg, dense = make(t, d, f, e, k, ns, False, seed=9)
+    ref, tol, _ = reference(x, w, cfg, dense)
+    check(moe_few.FewTokenMoE(w, cfg).forward(x), ref, tol)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_every_number_of_tokens_on_one_workspace(fp8):
+    x, w, cfg, dense = make(32, 256, 128, 16, 4, 1, fp8, seed=3)
+    layer = moe_few.FewTokenMoE(w, cfg)
+    ref, tol, _ = reference(x, w, cfg, dense)
+    for t in [32, 1, 31, 2, *range(3, 31, 3), 32, 1]:
+        check(layer.forward(x[:t]), ref[:t], tol[:t])
+    assert layer.forward(x[:0]).shape == (0, 256) and gemm.device_status() == 0
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_bias_sends_all_tokens_to_the_same_experts(fp8):
+    x, w, cfg, dense = make(32, 384, 256, 32, 4, 1, fp8, seed=4)
+    bias = torch.zeros(32, device=DEV)
+    bias[[3, 9, 30]] = 16.0
+    ref, tol, idx = reference(x, w, cfg, dense, bias)
+    assert (np.sort(idx, 1)[:, 1:] == [3, 9, 30]).sum() > 60
+    check(moe_few.FewTokenMoE(w, cfg, router_bias=bias).forward(x), ref, tol)
+
+
+def test_equal_logits_take_the_lowest_experts():
+    x, w, cfg, dense = make(6, 256, 128, 64, 8, 1, False, seed=5)
+    w["router.weight"].zero_()
+    ref, tol, idx = reference(x, w, cfg, dense)
+    assert (idx == np.arange(8)).all()
+    check(moe_few.FewTokenMoE(w, cfg).forward(x), ref, tol)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_nan_stays_in_its_token(fp8):
+    x, w, cfg, dense = make(11, 256, 128, 16, 4, 1, fp8, seed=6)
+    layer = moe_few.FewTokenMoE(w, cfg)
+    want = layer.forward(x)
+    for row, value in ((4, float("nan")), (10, float("inf"))):
+        y = x.clone()
+        y[row, 100] = value
+        got = layer.forward(y)
+        assert got[row].isnan().all()
+        keep = [i for i in range(11) if i != row]
+        assert torch.equal(got[keep], want[keep])
+    assert gemm.device_status() == 0
+
+
+def test_beside_the_layer():
+    """The same layer through moe_forward, whose intermediate roundings (fp16 gate, up, outputs of the experts) are more: the
+    layer's own tolerance, 1e-2 absolute and relative.  Both choose on the logits that they compute themselves."""
+    x, w, cfg = o.generate_input(1024, 512, 32, 1, 4, 24, 7)
+    tx, tw = torch.from_numpy(x).to(DEV), {n: torch.from_numpy(v).to(DEV) for n, v in w.items()}
+    want, _ = moe.moe_forward(tx, tw, cfg)
+    got = moe_few.FewTokenMoE(tw, cfg).forward(tx)
+    assert got.shape == tx.shape
+    ok, nbad, mx = o.check(got.cpu().numpy(), want.cpu().numpy())
+    assert ok, (nbad, mx)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_large_layer(fp8):
+    """The benchmark layer's widths; the weights of one shared and a few routed experts."""
+    for t in (1, 12):
+        x, w, cfg, dense = make(t, 7168, 2048, 8, 2, 1, fp8, seed=8, router_scale=2.0 ** -6)
+        ref, tol, _ = reference(x, w, cfg, dense)
+        check(moe_few.FewTokenMoE(w, cfg).forward(x), ref, tol)
+        assert gemm.device_status() == 0
+
+
+def test_streams_and_graphs_at_once():
+    """Calls on several streams, and graphs captured from one handle, each with a workspace of its own."""
+    x, w, cfg, _ = make(8, 1024, 512, 32, 4, 1, False, seed=10)
+    layer = moe_few.FewTokenMoE(w, cfg)
+    xs = [x, x.flip(0).contiguous(), (x * 0.5)]
+    want = [layer.forward(v).clone() for v in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = [[] for _ in xs]
+    for _ in range(5):
+        for i, (v, st) in enumerate(zip(xs, streams)):
+            with torch.cuda.stream(st):
+                got[i].append(layer.forward(v))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i in range(3) for g in got[i])
+    graphs, outs = [], []
+    for v in xs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            a = layer.forward(v)
+            outs.append((a, layer.forward(a.clamp(-1, 1))))
+        graphs.append(graph)
+    second = [layer.forward(v.clamp(-1, 1)).clone() for v in want]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for graph, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                graph.replay()
+        got_eager = layer.forward(x)
+    torch.cuda.synchronize()
+    assert torch.equal(got_eager, want[0]) and gemm.device_status() == 0
+    for i in range(3):
+        assert torch.equal(outs[i][0], want[i]) and torch.equal(outs[i][1], second[i])
+
+
+def test_a_marked_workspace_is_refused_until_reset():
+    """A workspace that a lost wait left behind holds counts that belong to nothing."""
+    x, w, cfg, dense = make(2, 128, 128, 4, 2, 1, False, seed=11)
+    layer = moe_few.FewTokenMoE(w, cfg)
+    want = layer.forward(x)
+    torch.cuda.synchronize()
+    assert gemm.device_status() == 0
+    for ws in layer._workspaces.values():
+        ws[12:16].view(torch.int32).fill_(1)             # the mark
+    out = torch.full_like(x, 5.0)
+    layer.forward(x, out=out)
+    assert gemm.device_status() == 5 and (out == 5).all()
+    layer.forward(x, out=out)
+    assert gemm.device_status() == 5 and (out == 5).all()
+    layer.reset()
+    assert torch.equal(layer.forward(x, out=out), want) and gemm.device_status() == 0
+
+
+def test_weights_are_read_at_every_call():
+    x, w, cfg, dense = make(3, 256, 128, 8, 2, 1, False, seed=12)
+    layer = moe_few.FewTokenMoE(w, cfg)
+    layer.forward(x)
+    for n in w:
+        if n.endswith(".2.weight"):
+            w[n].mul_(-2)
+    dense = {n: [m[0], m[1], -2 * m[2]] for n, m in dense.items()}
+    ref, tol, _ = reference(x, w, cfg, dense)
+    check(layer.forward(x), ref, tol)
