@@ -9,7 +9,8 @@ from .gemm import custom_kernel as gemm_custom_kernel, fp8_mm, fp8_mm_reference_
 from .grouped import fp8_grouped_mm  # noqa: F401
 from .moe import custom_kernel as moe_custom_kernel, moe_forward  # noqa: F401
 from .moe_few import FewTokenMoE  # noqa: F401
+from .moe_fp8 import Fp8MoE, quantize_experts  # noqa: F401
 from .quant import fp8_quantize, fp8_quantize_blocks, fp8_swiglu_quantize  # noqa: F401
 
-__all__ = ["FewTokenMoE", "fp8_grouped_mm", "fp8_mm", "fp8_mm_reference_layout", "fp8_quantize", "fp8_quantize_blocks", "fp8_swiglu_quantize",
-           "gemm_custom_kernel", "moe_custom_kernel", "moe_forward"]
+__all__ = ["FewTokenMoE", "Fp8MoE", "fp8_grouped_mm", "fp8_mm", "fp8_mm_reference_layout", "fp8_quantize", "fp8_quantize_blocks", "fp8_swiglu_quantize",
+           "gemm_custom_kernel", "moe_custom_kernel", "moe_forward", "quantize_experts"]
