@@ -553,10 +553,17 @@ int rf_moe_few_create(const RfMoeFewConfig *config, const void *router_weight, c
                       RfMoeFew **out);
 /* Synchronises the device (it frees the table).                                                     */
 int rf_moe_few_destroy(RfMoeFew *few);
-/* Workspace of a call with n_tokens tokens.  Its first *zeroed_bytes (the same for every n_tokens) have to be zero at the first
- * call; each call leaves them zero.  Calls that may overlap need a workspace each.  A call that loses a bounded wait
- * (rf_device_status) marks its workspace; until it is zeroed again, calls with it write no result and report a lost wait.  */
-size_t rf_moe_few_workspace_bytes(const RfMoeFewConfig *config, int n_tokens, size_t *zeroed_bytes);
+/* Workspace of a call with n_tokens tokens.  All of it has to be zero at its first call; after that it belongs to these calls, of
+ * any layer and number of tokens that it is large enough for, one after the other.  Calls that may overlap, captured ones
+ * among them, need a workspace each.  A call that loses a bounded wait (rf_device_status) marks its workspace; until that is zeroed
+ * again, calls with it write no result and report a lost wait.                                       */
+size_t rf_moe_few_workspace_bytes(const RfMoeFewConfig *config, int n_tokens);
+/* Zeroed device memory for that, on the current device; may be called while a stream is being captured (the zeroes are not part
+ * of the graph).                                                                                     */
+int rf_moe_few_workspace_alloc(size_t bytes, void **workspace);
+int rf_moe_few_workspace_free(void *workspace);
+/* *id = 0: the stream is not being captured; else a number of its own for each capture.              */
+int rf_stream_capture_id(rf_stream_t stream, unsigned long long *id);
 /* x fp16 [n_tokens, d_hidden] -> out fp16 [n_tokens, d_hidden], 16-byte aligned, workspace 256.  One kernel, asynchronous.  */
 int rf_moe_few_forward(RfMoeFew *few, const void *x, int n_tokens, void *out, void *workspace, size_t workspace_bytes,
                        rf_stream_t stream);

@@ -255,7 +255,13 @@ def _declare_fp8(L: ctypes.CDLL) -> None:
     L.rf_moe_few_destroy.restype = ci
     L.rf_moe_few_destroy.argtypes = [vp]
     L.rf_moe_few_workspace_bytes.restype = sz
-    L.rf_moe_few_workspace_bytes.argtypes = [config, ci, ctypes.POINTER(sz)]
+    L.rf_moe_few_workspace_bytes.argtypes = [config, ci]
+    L.rf_moe_few_workspace_alloc.restype = ci
+    L.rf_moe_few_workspace_alloc.argtypes = [sz, ctypes.POINTER(vp)]
+    L.rf_moe_few_workspace_free.restype = ci
+    L.rf_moe_few_workspace_free.argtypes = [vp]
+    L.rf_stream_capture_id.restype = ci
+    L.rf_stream_capture_id.argtypes = [vp, ctypes.POINTER(ctypes.c_ulonglong)]
     L.rf_moe_few_forward.restype = ci
     L.rf_moe_few_forward.argtypes = [vp, vp, ci, vp, vp, sz, vp]
 

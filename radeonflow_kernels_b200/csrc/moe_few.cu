@@ -7,20 +7,23 @@
 // What bounds it is the weight stream: each weight of every expert that a token chose is read once and used for a handful of
 // multiplications.  So one persistent CTA per SM keeps a ring of TMA loads full from the first microsecond to the last, and all
 // that depends on something else happens beside it.  The work is a list of items, dealt out by a ticket in this order:
-//   router units   16 experts x 512 columns of the logits, partial sums
+//   router units   16 experts x a chunk of K of the logits, partial sums
 //   first product  64 columns of gate and the same of up x a chunk of K, the shared expert's first (they need no routing)
 //   second product 128 columns of the result x a chunk of K
 // An item depends on items with smaller tickets only, and a CTA works its tickets off in order, so whatever share of the grid is
-// running makes progress, and the loads of an item never wait for its dependencies.  K chunks meet as fp32 partial sums in the
-// workspace; who finishes the last chunk of a column tile adds them up, in the order of the chunks, and likewise the last item of
-// a result tile adds the experts in rank order: results are the same bits whoever comes last.  Warps of a CTA:
+// running makes progress, and the loads of an item never wait for its dependencies.
+//
+// What one CTA computes for another travels as 64-bit words, 32 bits of data beside the number of the call, which the reader
+// polls for: no fence, no counter, one trip through L2.  (With partial sums behind fences and counters, each hand-over was four
+// or five trips of 1.2 us under load: one token through 9 experts of 1024 x 512 took 25 us, through 5 of 7168 x 2048 98.)  The
+// item with the last chunk of a column tile adds the chunks up in their order, and the last item of a result tile adds the
+// experts in rank order: results are the same bits whoever comes last.  Warps of a CTA:
 //   0      draws tickets, issues the weight loads (16 KB stages)
-//   1-3    the items' token rows (or, for the second product, h, once the expert's first is complete) into shared memory
+//   1-3    the items' token rows (or, for the second product, h) into shared memory
 //   4-11   mma.sync m16n8k16, weights as the 16-row operand, up to 8 tokens as the 8 columns: a warp owns 16 of the item's 128
 //          columns.  (The legacy tensor path on purpose: the stream feeds one such MMA per 21 cycles and SM, and its
 //          accumulators need no trip through TMEM.)  FP8 weights become fp16 on the way, their scale is applied per 128 of K.
-//   12-15  publish finished items, add up what is complete
-//   16-19  softmax, top-k and the experts' token lists, in every CTA for itself, once the logits are complete
+//   12-15  softmax, top-k and the experts' token lists, in every CTA for itself; then the sums of complete tiles
 // h is rounded to fp16, the type of the second product's operand; everything else is fp32.
 #include "moe_few.h"
 #include "launch.h"
@@ -31,12 +34,12 @@ namespace rf {
 
 namespace {
 
-constexpr int WARP_X = 1, WARP_MMA = 4, WARP_PUB = 12, WARP_ROUTE = 16, WARPS = 20;
-constexpr int X_WARPS = WARP_MMA - WARP_X, MMA_WARPS = WARP_PUB - WARP_MMA;
+constexpr int WARP_X = 1, WARP_MMA = 4, WARP_SUM = 12, WARPS = 16;
+constexpr int X_WARPS = WARP_MMA - WARP_X, MMA_WARPS = WARP_SUM - WARP_MMA, SUM_WARPS = WARPS - WARP_SUM;
 constexpr int THREADS = 32 * WARPS;
-constexpr int BAR_MMA = 1, BAR_PUB = 2, BAR_ROUTE = 3;
+constexpr int BAR_MMA = 1, BAR_SUM = 2;
 constexpr int STAGE_BYTES = 16384, BOX_BYTES = 8192;
-constexpr int ITEM_SLOTS = 8;
+constexpr int ITEM_SLOTS = 8, SUM_SLOTS = 8;
 constexpr int DRAW_AHEAD = 4;           // stages before an item's last load at which the next ticket is drawn
 constexpr int MAX_PAIRS = kFewMaxTokens * kFewMaxTopK;
 
@@ -52,8 +55,7 @@ struct Routing {
     int expert[MAX_PAIRS];              // [token][rank]
     int pos[MAX_PAIRS];                 // pair of [token][rank]
     float weight[MAX_PAIRS];            // [token][rank]
-    int sums[4];
-    int last;                           // publishers: whether the item was the last of its tile
+    int count[kFewMaxExperts];
 };
 
 template <bool FP8, int NG>
@@ -64,37 +66,57 @@ struct Cfg {
     // fp16 operands go through ldmatrix (rows 16 bytes apart modulo 128), those of FP8 through 8-byte loads (32 bytes)
     static constexpr int kPad = FP8 ? 32 : 16;
     static constexpr int kXStride = kMaxChunk * 2 + kPad;
-    static constexpr int kXBytes = kRows * kXStride;
+    // ... and behind the rows the scales of the item's two boxes, one per 128 of K
+    static constexpr int kXBytes = kRows * kXStride + (FP8 ? 64 : 0);
     static constexpr int kRedBytes = MMA_WARPS * 16 * kRows * 4;
     static constexpr int kStages = NG == 1 ? 11 : 8;
-    static constexpr int kBars = 2 * kStages + 4 + 3 * ITEM_SLOTS + 1;
-    static constexpr int kSmemBytes = kStages * STAGE_BYTES + 2 * kXBytes + kRedBytes + ITEM_SLOTS * 16 + kBars * 8 +
+    static constexpr int kBars = 2 * kStages + 4 + 2 * ITEM_SLOTS + 2 * SUM_SLOTS + 1;
+    static constexpr int kSmemBytes = kStages * STAGE_BYTES + 2 * kXBytes + kRedBytes + (ITEM_SLOTS + SUM_SLOTS) * 16 + kBars * 8 +
                                       (int)sizeof(Routing) + 1024;
     static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
 };
 
-__device__ __forceinline__ int ld_acquire_gpu_s32(const int* p) {
-    int v;
-    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+// A word that travels between CTAs: data below, the number of the call above.  One 64-bit access each, so that data and number
+// arrive together; two words at a time where they lie side by side.
+__device__ __forceinline__ unsigned long long word_of(uint32_t data, uint32_t call) {
+    return (unsigned long long)data | ((unsigned long long)call << 32);
+}
+__device__ __forceinline__ void st_word(unsigned long long* p, uint32_t data, uint32_t call) {
+    asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(word_of(data, call)) : "memory");
+}
+__device__ __forceinline__ unsigned long long ld_word(const unsigned long long* p) {
+    unsigned long long v;
+    asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
     return v;
 }
-// Bounded wait for *p >= want (limit, status word and unwinding as in mbar_wait).
-__device__ __forceinline__ bool counter_wait(const int* p, int want, int* status, int code, int tag) {
-    unsigned long long t0 = 0;
-    for (uint32_t it = 1;; ++it) {
-        if (ld_acquire_gpu_s32(p) >= want) return true;
-        if ((it & 0x3fu) == 0) {
-            const int seen = *reinterpret_cast<volatile int*>(status);
-            if (seen != 0 && (seen >> kStatusTagShift) == tag) return false;
-            const unsigned long long now = globaltimer_ns();
-            if (t0 == 0) t0 = now;
-            else if (now - t0 > wait_limit_ns(status)) {
-                atomicCAS(status, 0, code | (tag << kStatusTagShift));
-                return false;
-            }
-        }
-    }
+__device__ __forceinline__ ulonglong2 ld_words(const unsigned long long* p) {
+    ulonglong2 v;
+    asm volatile("ld.relaxed.gpu.global.v2.u64 {%0, %1}, [%2];" : "=l"(v.x), "=l"(v.y) : "l"(p) : "memory");
+    return v;
 }
+__device__ __forceinline__ uint32_t call_of(unsigned long long w) { return (uint32_t)(w >> 32); }
+__device__ __forceinline__ float float_of(unsigned long long w) { return __uint_as_float((uint32_t)w); }
+
+// The limit of a polling loop (status word and unwinding as in mbar_wait): false = give up.
+struct Patience {
+    int* status;
+    int tag;
+    uint32_t polls = 0;
+    unsigned long long t0 = 0;
+    __device__ __forceinline__ Patience(int* s, int t) : status(s), tag(t) {}
+    __device__ __forceinline__ bool more() {
+        if ((++polls & 0x3fu) != 0) return true;
+        const int seen = *reinterpret_cast<volatile int*>(status);
+        if (seen != 0 && (seen >> kStatusTagShift) == tag) return false;
+        const unsigned long long now = globaltimer_ns();
+        if (t0 == 0) t0 = now;
+        else if (now - t0 > wait_limit_ns(status)) {
+            atomicCAS(status, 0, kErrSchedWait | (tag << kStatusTagShift));
+            return false;
+        }
+        return true;
+    }
+};
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -109,25 +131,49 @@ __device__ __forceinline__ uint2 ld_shared_v2(uint32_t addr) {
     asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
     return v;
 }
+// (no "volatile": a function of its operands alone)
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t f16x2_of_e4m3x2(uint16_t v) {
     uint32_t r;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
     return r;
 }
-__device__ __forceinline__ float2 ld_cg_f2(const float* p) {
-    float2 v;
-    asm volatile("ld.global.cg.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p) : "memory");
-    return v;
-}
-__device__ __forceinline__ float ld_cg_f(const float* p) {
-    float v;
-    asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
-    return v;
+
+// A warp's sums of n partial sums, `step` words apart, in their order: two neighbouring words at `a` and two at `b`.  Eight chunks are
+// in flight together.
+__device__ __forceinline__ bool sum_chunks(const unsigned long long* a, const unsigned long long* b, size_t step, int n,
+                                           uint32_t call, Patience& patience, float2* sa, float2* sb) {
+    float2 x = make_float2(0.f, 0.f), y = x;
+    for (int c0 = 0; c0 < n; c0 += 8) {
+        ulonglong2 u[8], v[8];
+        for (;;) {
+            bool here = true;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const size_t at = (size_t)min(c0 + i, n - 1) * step;
+                u[i] = ld_words(a + at);
+                v[i] = ld_words(b + at);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                here = here && call_of(u[i].x) == call && call_of(u[i].y) == call && call_of(v[i].x) == call && call_of(v[i].y) == call;
+            if (__all_sync(0xffffffffu, here)) break;
+            if (!__all_sync(0xffffffffu, patience.more())) return false;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c0 + i < n) {
+                x.x += float_of(u[i].x); x.y += float_of(u[i].y);
+                y.x += float_of(v[i].x); y.y += float_of(v[i].y);
+            }
+    }
+    *sa = x;
+    *sb = y;
+    return true;
 }
 
 // How the work divides: known once the routing is.
@@ -162,6 +208,141 @@ __device__ __forceinline__ Item decode_routed(int r, const Shape& s, int n_activ
     return make_int4(kEnd, 0, 0, 0);
 }
 
+// One warp: a token's logits from their partial sums, softmax and top-k as topk_kernel (moe_route.cu) does them, on the same fp16
+// roundings.  Lane l owns experts l * VPT ..; a key is an fp16 probability, then the complement of the expert's number.
+template <int VPT>
+__device__ __forceinline__ bool route_token(const MoeFewParams& p, Routing& rt, int t, uint32_t call, Patience& patience) {
+    constexpr int BATCH = 16 / VPT < 8 ? 16 / VPT : 8;          // chunks whose loads are in flight together
+    const int lane = threadIdx.x & 31, e0 = lane * VPT;
+    const bool active = e0 < p.experts;
+    const unsigned long long* src = p.logits + (size_t)t * p.experts + (active ? e0 : 0);
+    const size_t step = (size_t)p.t * p.experts;
+    float l[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) l[i] = 0.f;
+    for (int c0 = 0; c0 < p.router_chunks; c0 += BATCH) {
+        unsigned long long v[BATCH][VPT];
+        for (;;) {
+            bool here = true;
+#pragma unroll
+            for (int c = 0; c < BATCH; ++c) {
+                const unsigned long long* at = src + (size_t)min(c0 + c, p.router_chunks - 1) * step;
+                if (VPT == 1) {
+                    v[c][0] = ld_word(at);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < VPT / 2; ++i) {
+                        const ulonglong2 w = ld_words(at + 2 * i);
+                        v[c][2 * i] = w.x;
+                        v[c][VPT == 1 ? 0 : 2 * i + 1] = w.y;
+                    }
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < BATCH; ++c)
+#pragma unroll
+                for (int i = 0; i < VPT; ++i) here = here && call_of(v[c][i]) == call;
+            if (__all_sync(0xffffffffu, here)) break;
+            if (!__all_sync(0xffffffffu, patience.more())) return false;
+        }
+#pragma unroll
+        for (int c = 0; c < BATCH; ++c)
+            if (c0 + c < p.router_chunks)
+#pragma unroll
+                for (int i = 0; i < VPT; ++i) l[i] += float_of(v[c][i]);
+    }
+    float mx = -65504.0f;
+    if (active)
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            if (p.router_bias != nullptr) l[i] += ld_global_f32(p.router_bias + e0 + i);
+            l[i] = __half2float(__float2half_rn(l[i]));
+            mx = fmaxf(mx, l[i]);
+        }
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
+    float part = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        l[i] = active ? det_exp(__fsub_rn(l[i], mx)) : 0.f;
+        part = i == 0 ? l[0] : __fadd_rn(part, l[i]);
+    }
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) part = __fadd_rn(part, __shfl_xor_sync(0xffffffffu, part, s));
+    const float recip = __fdiv_rn(1.0f, part);
+    uint32_t key[VPT], mine = 0;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+        key[i] = active ? ((uint32_t)__half_as_ushort(__float2half_rn(__fmul_rn(l[i], recip))) << 16) | (0xFFFFu - (uint32_t)(e0 + i))
+                        : 0u;
+    for (int k = 0; k < p.top_k; ++k) {
+        uint32_t best = key[0];
+#pragma unroll
+        for (int i = 1; i < VPT; ++i) best = max(best, key[i]);
+        best = __reduce_max_sync(0xffffffffu, best);
+        if (lane == k) mine = best;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+            if (key[i] == best) key[i] = 0u;
+    }
+    if (lane < p.top_k) {
+        rt.expert[t * p.top_k + lane] = (int)(0xFFFFu - (mine & 0xFFFFu));
+        rt.weight[t * p.top_k + lane] = __half2float(__ushort_as_half((unsigned short)(mine >> 16)));
+    }
+    return true;
+}
+
+// One warp: the experts' token lists, in an order that every CTA finds alike.  Ranks inside 32 pairs by match_any, pairs in order;
+// then the experts' offsets, eight experts a lane.
+__device__ __forceinline__ void build_lists(const MoeFewParams& p, Routing& rt) {
+    const int lane = threadIdx.x & 31, pairs = p.t * p.top_k;
+    for (int e = lane; e < kFewMaxExperts; e += 32) rt.count[e] = 0;
+    __syncwarp();
+    for (int i0 = 0; i0 < pairs; i0 += 32) {
+        const int i = i0 + lane, e = i < pairs ? rt.expert[i] : -1;
+        const unsigned peers = __match_any_sync(0xffffffffu, e);
+        const int before = __popc(peers & ((1u << lane) - 1));
+        if (e >= 0) rt.pos[i] = rt.count[e] + before;
+        __syncwarp();
+        if (e >= 0 && before == 0) rt.count[e] += __popc(peers);
+        __syncwarp();
+    }
+    // pairs (low half) and active experts (high half) in front of this lane's eight experts
+    int n[8], mine = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        n[i] = rt.count[8 * lane + i];
+        mine += n[i] + ((n[i] > 0) << 16);
+    }
+    int incl = mine;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, incl, s);
+        if (lane >= s) incl += o;
+    }
+    int run = incl - mine;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (n[i] > 0) {
+            rt.active[run >> 16] = 8 * lane + i;
+            rt.base[run >> 16] = run & 0xFFFF;
+        }
+        rt.count[8 * lane + i] = run & 0xFFFF;          // now the expert's first pair
+        run += n[i] + ((n[i] > 0) << 16);
+    }
+    if (lane == 31) {
+        rt.n_active = run >> 16;
+        rt.base[run >> 16] = pairs;
+    }
+    __syncwarp();
+    for (int i = lane; i < pairs; i += 32) {
+        const int at = rt.count[rt.expert[i]] + rt.pos[i];
+        rt.pos[i] = at;
+        rt.token[at] = i / p.top_k;
+    }
+    __syncwarp();
+}
+
 template <bool FP8, int NG>
 __global__ void __launch_bounds__(THREADS, 1)
 moe_few_kernel(const MoeFewParams p) {
@@ -173,17 +354,19 @@ moe_few_kernel(const MoeFewParams p) {
     const uint32_t x_base = smem_base + STAGES * STAGE_BYTES;
     const uint32_t red_base = x_base + 2 * C::kXBytes;
     const uint32_t item_base = red_base + C::kRedBytes;
-    const uint32_t bar_base = item_base + ITEM_SLOTS * 16;
+    const uint32_t sum_base = item_base + ITEM_SLOTS * 16;
+    const uint32_t bar_base = sum_base + SUM_SLOTS * 16;
     auto full_bar = [&](uint32_t s) { return bar_base + 8u * s; };
     auto empty_bar = [&](uint32_t s) { return bar_base + 8u * (STAGES + s); };
     auto x_full_bar = [&](uint32_t b) { return bar_base + 8u * (2 * STAGES + b); };
     auto x_empty_bar = [&](uint32_t b) { return bar_base + 8u * (2 * STAGES + 2 + b); };
+    // rings of items: for the rows and MMA warps, and of those that end with a sum
     auto item_bar = [&](uint32_t j) { return bar_base + 8u * (2 * STAGES + 4 + j % ITEM_SLOTS); };
-    auto done_bar = [&](uint32_t j) { return bar_base + 8u * (2 * STAGES + 4 + ITEM_SLOTS + j % ITEM_SLOTS); };
-    auto free_bar = [&](uint32_t j) { return bar_base + 8u * (2 * STAGES + 4 + 2 * ITEM_SLOTS + j % ITEM_SLOTS); };
-    const uint32_t routed_bar = bar_base + 8u * (2 * STAGES + 4 + 3 * ITEM_SLOTS);
-    auto at = [&](uint32_t addr) { return smem_raw + (addr - smem_u32(smem_raw)); };
-    Routing& rt = *reinterpret_cast<Routing*>(at(bar_base + 8u * C::kBars));
+    auto free_bar = [&](uint32_t j) { return bar_base + 8u * (2 * STAGES + 4 + ITEM_SLOTS + j % ITEM_SLOTS); };
+    auto sum_bar = [&](uint32_t j) { return bar_base + 8u * (2 * STAGES + 4 + 2 * ITEM_SLOTS + j % SUM_SLOTS); };
+    auto sum_free_bar = [&](uint32_t j) { return bar_base + 8u * (2 * STAGES + 4 + 2 * ITEM_SLOTS + SUM_SLOTS + j % SUM_SLOTS); };
+    const uint32_t routed_bar = bar_base + 8u * (2 * STAGES + 4 + 2 * ITEM_SLOTS + 2 * SUM_SLOTS);
+    Routing& rt = *reinterpret_cast<Routing*>(smem_raw + (bar_base + 8u * C::kBars - smem_u32(smem_raw)));
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -199,14 +382,22 @@ moe_few_kernel(const MoeFewParams p) {
         }
         for (int j = 0; j < ITEM_SLOTS; ++j) {
             mbar_init(item_bar(j), 1);
-            mbar_init(done_bar(j), MMA_WARPS);
-            mbar_init(free_bar(j), X_WARPS + MMA_WARPS + 1);
+            mbar_init(free_bar(j), X_WARPS + MMA_WARPS);
+        }
+        for (int j = 0; j < SUM_SLOTS; ++j) {
+            mbar_init(sum_bar(j), 1);
+            mbar_init(sum_free_bar(j), SUM_WARPS);
         }
         mbar_init(routed_bar, 1);
         mbar_fence_init();
     }
     griddep_wait();
-    // A workspace in which an earlier call lost a wait holds counts that belong to nothing: no result then, and a code.
+    // The number of this call: zero, which fresh words hold, is left out.  (A word that no call has written for the 2^32 - 1 calls
+    // before this one could pass for this call's.)
+    uint32_t call = (uint32_t)ld_global_s32(p.head + kFewCalls) + 1;
+    if (call == 0) call = 1;
+    // A workspace in which an earlier call lost a wait holds a ticket that belongs to nothing: no result then, and a code.
+    int ticket = threadIdx.x == 0 ? atomicAdd(p.head + kFewTicket, 1) : 0;
     const int bad = __syncthreads_or(ld_global_s32(p.head + kFewBad) != 0);
     if (bad) {
         if (threadIdx.x == 0) atomicCAS(p.status, 0, kErrSchedWait | (p.launch_tag << kStatusTagShift));
@@ -217,15 +408,16 @@ moe_few_kernel(const MoeFewParams p) {
     const int shared_first = shape.tiles1s * shape.chunks1;
     const int before_routed = p.router_units + shared_first;
     const int pairs = p.t * p.top_k;            // the shared expert's pairs come behind them, one per token
-    int* const done1 = p.head + kFewHeadWords;
+    const size_t rows = pairs + p.t;            // of h and the partial sums
     auto wait_routed = [&](int code) { return mbar_wait(routed_bar, 0, p.status, code, p.launch_tag); };
     auto wait_item = [&](uint32_t j, int code) {
         return mbar_wait(item_bar(j), (j / ITEM_SLOTS) & 1, p.status, code, p.launch_tag);
     };
-    auto get_item = [&](uint32_t j) {
-        const uint4 v = ld_shared_v4(item_base + 16u * (j % ITEM_SLOTS));
+    auto read_item = [&](uint32_t addr) {
+        const uint4 v = ld_shared_v4(addr);
         return make_int4((int)v.x, (int)v.y, (int)v.z, (int)v.w);
     };
+    auto get_item = [&](uint32_t j) { return read_item(item_base + 16u * (j % ITEM_SLOTS)); };
     // K range of an item
     auto k_range = [&](const Item& it, int* k0, int* len) {
         const int kc = it.x == kFirst ? p.kc1 : p.kc2;
@@ -243,7 +435,7 @@ moe_few_kernel(const MoeFewParams p) {
         if (lane == 0) {
             uint32_t st = 0, s = 0, ph = 1;
             bool ok = true, routed = false;
-            int ticket = atomicAdd(p.head + kFewTicket, 1);
+            uint32_t sums = 0;
             for (uint32_t j = 0; ok; ++j) {
                 Item it;
                 if (ticket < p.router_units) {
@@ -263,6 +455,14 @@ moe_few_kernel(const MoeFewParams p) {
                 if (!ok) break;
                 st_shared_v4(item_base + 16u * (j % ITEM_SLOTS), it.x, it.y, it.z, it.w);
                 mbar_arrive(item_bar(j));
+                // the last chunk of a column tile, the last item of a result tile
+                if (it.x == kEnd || (it.x == kFirst && it.w == shape.chunks1 - 1) ||
+                    (it.x == kSecond && it.y == rt.n_active - 1 && it.w == shape.chunks2 - 1)) {
+                    ok = mbar_wait(sum_free_bar(sums), ((sums / SUM_SLOTS) & 1) ^ 1, p.status, kErrProducerWait, p.launch_tag);
+                    if (!ok) break;
+                    st_shared_v4(sum_base + 16u * (sums % SUM_SLOTS), it.x, it.y, it.z, it.w);
+                    mbar_arrive(sum_bar(sums++));
+                }
                 if (it.x == kEnd) break;
                 if (it.x == kRouter) {
                     ticket = atomicAdd(p.head + kFewTicket, 1);
@@ -315,46 +515,67 @@ moe_few_kernel(const MoeFewParams p) {
             ok = __all_sync(0xffffffffu, mbar_wait(x_empty_bar(b), ((n >> 1) & 1) ^ 1, p.status, kErrMmaWaitFull, p.launch_tag));
             if (!ok) break;
             const int n_rows = pair_count(it), first = first_pair(it);
-            const __half* src;
-            size_t stride;
-            if (it.x == kFirst) {
-                src = static_cast<const __half*>(p.x) + k0;
-                stride = p.d;
-            } else {
-                const int e = expert_of(it);
-                if (lane == 0)
-                    ok = counter_wait(done1 + e, it.y < 0 ? shape.tiles1s : shape.tiles1, p.status, kErrSchedWait, p.launch_tag);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                src = static_cast<const __half*>(p.h) + (size_t)first * p.width + k0;
-                stride = p.width;
-            }
-            const int vecs = len >> 3;
             const uint32_t dst = x_base + b * C::kXBytes;
-            const bool gather = it.x == kFirst && it.y >= 0;
-#pragma unroll 4
-            for (int i = tid; i < n_rows * vecs; i += 32 * X_WARPS) {
-                const int r = i / vecs, v = i - r * vecs;
-                const int row = gather ? rt.token[first + r] : r;
-                const uint4 q = ld_global_cg_v4(src + (size_t)row * stride + 8 * v);
-                st_shared_v4(dst + r * C::kXStride + 16 * v, q.x, q.y, q.z, q.w);
+            float scale = 0.f;
+            if (FP8 && warp == WARP_X && lane < 16 && (lane & 7) < len / 128) {
+                const int m = it.x == kFirst ? lane >> 3 : 2, k = it.x == kFirst ? p.d : it.y < 0 ? p.fs : p.f;
+                scale = ld_global_f32(p.scales[3 * expert_of(it) + m] +
+                                      (size_t)(it.x == kFirst ? it.z >> 1 : it.z) * (k / 128) + k0 / 128 + (lane & 7));
             }
+            if (it.x == kFirst) {
+                // one bulk copy per row, all by the first of the warps
+                if (warp == WARP_X) {
+                    if (lane == 0) mbar_expect_tx_only(x_full_bar(b), (uint32_t)(n_rows * len * 2));
+                    __syncwarp();
+                    if (lane < n_rows) {
+                        const int row = it.y >= 0 ? rt.token[first + lane] : lane;
+                        bulk_load(dst + lane * C::kXStride, static_cast<const __half*>(p.x) + (size_t)row * p.d + k0, (uint32_t)len * 2,
+                                  x_full_bar(b));
+                    }
+                }
+            } else {
+                // h comes as words of two values: two of them make 8 bytes of a row
+                const int vecs = len >> 2, total = n_rows * vecs;
+                const unsigned long long* src = p.h + (size_t)first * (p.width / 2) + k0 / 2;
+                Patience patience(p.status, p.launch_tag);
+                constexpr int BATCH = 8;
+                for (int i0 = 0; i0 < total && ok; i0 += BATCH * 32 * X_WARPS) {
+                    ulonglong2 v[BATCH];
+                    for (;;) {
+                        bool here = true;
+#pragma unroll
+                        for (int i = 0; i < BATCH; ++i) {
+                            const int at = min(i0 + i * 32 * X_WARPS + tid, total - 1), r = at / vecs;
+                            v[i] = ld_words(src + (size_t)r * (p.width / 2) + 2 * (at - r * vecs));
+                        }
+#pragma unroll
+                        for (int i = 0; i < BATCH; ++i) here = here && call_of(v[i].x) == call && call_of(v[i].y) == call;
+                        if (__all_sync(0xffffffffu, here)) break;
+                        ok = __all_sync(0xffffffffu, patience.more());
+                        if (!ok) break;
+                    }
+                    if (!ok) break;
+#pragma unroll
+                    for (int i = 0; i < BATCH; ++i) {
+                        const int at = i0 + i * 32 * X_WARPS + tid, r = at / vecs;
+                        if (at < total) st_shared_v2(dst + r * C::kXStride + 8 * (at - r * vecs), (uint32_t)v[i].x, (uint32_t)v[i].y);
+                    }
+                }
+                if (!ok) break;
+            }
+            if (FP8 && warp == WARP_X && lane < 16) st_shared_f32(dst + C::kRows * C::kXStride + lane * 4, scale);
             __syncwarp();
             if (lane == 0) mbar_arrive(x_full_bar(b));
             ++n;
         }
         lost = !ok;
-        // This CTA draws no ticket, and this warp waits for no counter any more: the last warp to come here clears them for the
-        // next call.  (Where a wait was lost the workspace is marked below, and its next call refuses to run.)
-        if (ok) {
-            int last = 0;
-            if (lane == 0) last = atomicAdd(p.head + kFewExits, 1) == (int)gridDim.x * X_WARPS - 1;
-            if (__shfl_sync(0xffffffffu, last, 0)) {
-                if (lane < 3) p.head[lane] = 0;             // ticket, router units done, exits
-                for (int e = lane; e <= p.experts; e += 32) done1[e] = 0;
-            }
+        // This CTA draws no ticket any more: the last warp to come here gives the next call its ticket and its number.  (Where a wait
+        // was lost the workspace is marked below, and its next call refuses to run.)
+        if (ok && lane == 0 && atomicAdd(p.head + kFewExits, 1) == (int)gridDim.x * X_WARPS - 1) {
+            p.head[kFewTicket] = p.head[kFewExits] = 0;
+            p.head[kFewCalls] = (int)call;
         }
-    } else if (warp < WARP_PUB) {
+    } else if (warp < WARP_SUM) {
         // ------------------------------------------------------------------------------ MMA
         const int w = warp - WARP_MMA;
         const int g = lane >> 2, q = lane & 3;      // row (column) of the fragments, pair inside
@@ -373,12 +594,12 @@ moe_few_kernel(const MoeFewParams p) {
             if (lane == 0) mbar_arrive(free_bar(j));
             if (it.x == kEnd) break;
             if (it.x == kRouter) {
-                // 16 experts x 512 columns, 64 of them per warp.  A lane holds 16 consecutive k of its row (and token): the
+                // 16 experts x a chunk of K, 64 columns per warp and round.  A lane holds 16 consecutive k of its row (and token): the
                 // order of k inside a fragment is free as long as both operands share it.
                 const int e0 = it.z / p.router_chunks * 16, c = it.z % p.router_chunks;
-                const int k = c * kFewRouterChunk + w * 64;
                 float acc[NG][4] = {};
-                if (k < p.d) {
+#pragma unroll 1
+                for (int k = c * p.router_kc + w * 64; k < min((c + 1) * p.router_kc, p.d); k += MMA_WARPS * 64) {
                     uint4 a[2][2], b[NG][2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
@@ -417,293 +638,213 @@ moe_few_kernel(const MoeFewParams p) {
 #pragma unroll
                     for (int o = 0; o < MMA_WARPS; ++o)
                         v += __uint_as_float(ld_shared_u32(red_base + (o * 16 * C::kRows + i) * 4));
-                    if (e < p.experts && t < p.t) p.logits[((size_t)c * p.t + t) * p.experts + e] = v;
+                    if (e < p.experts && t < p.t) st_word(p.logits + ((size_t)c * p.t + t) * p.experts + e, __float_as_uint(v), call);
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(done_bar(j));
                 continue;
             }
             int k0, len;
             k_range(it, &k0, &len);
             const int n_rows = pair_count(it), first = first_pair(it);
             const uint32_t b = n & 1;
-            float scale = 0.f;
-            if (FP8) {
-                // lane i holds the scale of the chunk's i-th 128 of K
-                const int m = it.x == kFirst ? (w >> 2) : 2, k = it.x == kFirst ? p.d : it.y < 0 ? p.fs : p.f;
-                const int block = it.x == kFirst ? it.z >> 1 : it.z;
-                if (lane < len / 128)
-                    scale = ld_global_f32(p.scales[3 * expert_of(it) + m] + (size_t)block * (k / 128) + k0 / 128 + lane);
-            }
             ok = __all_sync(0xffffffffu, mbar_wait(x_full_bar(b), (n >> 1) & 1, p.status, kErrMmaWaitFull, p.launch_tag));
             const uint32_t xb = x_base + b * C::kXBytes;
             const int groups = (n_rows + 7) >> 3;
             float acc[NG][4] = {};
             const int n_stages = len / C::kStageK;
-            for (int i = 0; i < n_stages && ok; ++i) {
-                ok = __all_sync(0xffffffffu, mbar_wait(full_bar(s), ph, p.status, kErrMmaWaitFull, p.launch_tag));
-                if (!ok) break;
-                const uint32_t wb = smem_base + s * STAGE_BYTES + box;
-                if (FP8) {
-                    // rows are output columns; a lane takes 4 consecutive k of its two rows per MMA
-                    float part[NG][4] = {};
-                    const int r0 = (w & 3) * 16 + g;
-                    const uint32_t row = wb + r0 * 128 + 4 * q;
+            auto next_stage = [&] {
+                const bool here = __all_sync(0xffffffffu, mbar_wait(full_bar(s), ph, p.status, kErrMmaWaitFull, p.launch_tag));
+                return here;
+            };
+            auto give_back = [&] {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(empty_bar(s));
+                if (++s == STAGES) { s = 0; ph ^= 1; }
+            };
+            if (FP8) {
+                // Rows are output columns; a lane takes 4 consecutive k of its two rows per MMA.  A stage's words are in registers
+                // before the stage in front of it is multiplied, so that barrier and load latency lie under the conversions; two
+                // chains of MMAs alternate.
+                const int r0 = (w & 3) * 16 + g;
+                const uint32_t scales = xb + C::kRows * C::kXStride + (w >> 2) * 32;
+                uint32_t lo[2][8], hi[2][8];
+                auto load = [&](uint32_t (&l)[8], uint32_t (&h)[8]) {
+                    const uint32_t row = smem_base + s * STAGE_BYTES + box + r0 * 128 + 4 * q;
 #pragma unroll
                     for (int kk = 0; kk < 8; ++kk) {
                         const uint32_t off = (uint32_t)((kk ^ (r0 & 7)) << 4);
-                        const uint32_t lo = ld_shared_u32(row + off), hi = ld_shared_u32(row + 8 * 128 + off);
-                        const uint32_t a[4] = {f16x2_of_e4m3x2((uint16_t)lo), f16x2_of_e4m3x2((uint16_t)hi),
-                                               f16x2_of_e4m3x2((uint16_t)(lo >> 16)), f16x2_of_e4m3x2((uint16_t)(hi >> 16))};
-#pragma unroll
-                        for (int u = 0; u < NG; ++u) {
-                            if (u >= groups) break;
-                            const uint2 x = ld_shared_v2(xb + (8 * u + g) * C::kXStride + 2 * (i * 128 + kk * 16 + 4 * q));
-                            mma_f16(part[u], a, x.x, x.y);
-                        }
+                        l[kk] = ld_shared_u32(row + off);
+                        h[kk] = ld_shared_u32(row + 8 * 128 + off);
                     }
-                    const float sc = __shfl_sync(0xffffffffu, scale, i);
+                };
+                auto multiply = [&](int i, const uint32_t (&l)[8], const uint32_t (&h)[8]) {
+                    const float sc = __uint_as_float(ld_shared_u32(scales + i * 4));
 #pragma unroll
-                    for (int u = 0; u < NG; ++u)
+                    for (int u = 0; u < NG; ++u) {
+                        if (u >= groups) break;
+                        float part[4] = {}, odd[4] = {};
+                        uint2 x[8];
 #pragma unroll
-                        for (int v = 0; v < 4; ++v) acc[u][v] = fmaf(sc, part[u][v], acc[u][v]);
-                } else {
-                    // rows are k; transposed 8 x 8 pieces give the weights as [column][k] fragments
-                    const int kr = (lane & 7) + 8 * (lane >> 4), chunk = 2 * (w & 3) + ((lane >> 3) & 1);
-                    const uint32_t wa = wb + kr * 128 + ((chunk ^ (kr & 7)) << 4);
+                        for (int kk = 0; kk < 8; ++kk)
+                            x[kk] = ld_shared_v2(xb + (8 * u + g) * C::kXStride + 2 * (i * 128 + kk * 16 + 4 * q));
+#pragma unroll
+                        for (int kk = 0; kk < 8; ++kk) {
+                            const uint32_t a[4] = {f16x2_of_e4m3x2((uint16_t)l[kk]), f16x2_of_e4m3x2((uint16_t)h[kk]),
+                                                   f16x2_of_e4m3x2((uint16_t)(l[kk] >> 16)), f16x2_of_e4m3x2((uint16_t)(h[kk] >> 16))};
+                            mma_f16(kk & 1 ? odd : part, a, x[kk].x, x[kk].y);
+                        }
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) acc[u][v] = fmaf(sc, part[v] + odd[v], acc[u][v]);
+                    }
+                };
+                ok = ok && next_stage();
+                if (ok) {
+                    load(lo[0], hi[0]);
+                    give_back();
+                }
+                for (int i = 0; i < n_stages && ok; i += 2) {
+                    if (i + 1 < n_stages) {
+                        ok = next_stage();
+                        if (!ok) break;
+                        load(lo[1], hi[1]);
+                        give_back();
+                    }
+                    multiply(i, lo[0], hi[0]);
+                    if (i + 1 >= n_stages) break;
+                    if (i + 2 < n_stages) {
+                        ok = next_stage();
+                        if (!ok) break;
+                        load(lo[0], hi[0]);
+                        give_back();
+                    }
+                    multiply(i + 1, lo[1], hi[1]);
+                }
+            } else {
+                // rows are k; transposed 8 x 8 pieces give the weights as [column][k] fragments
+                const int kr = (lane & 7) + 8 * (lane >> 4), chunk = 2 * (w & 3) + ((lane >> 3) & 1);
+                const uint32_t w_off = box + kr * 128 + ((chunk ^ (kr & 7)) << 4);
+                for (int i = 0; i < n_stages && ok; ++i) {
+                    ok = next_stage();
+                    if (!ok) break;
+                    const uint32_t wa = smem_base + s * STAGE_BYTES + w_off;
                     const uint32_t xa = xb + (lane & 7) * C::kXStride + 2 * (i * 64 + 8 * (lane >> 3));
-                    uint32_t x[2][NG][4];
+                    uint32_t a[4][4], x[2][NG][4];
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) ldmatrix_x4_trans(wa + kk * 16 * 128, a[kk]);
 #pragma unroll
                     for (int v = 0; v < 2; ++v)
 #pragma unroll
                         for (int u = 0; u < NG; ++u)
                             if (u < groups) ldmatrix_x4(xa + u * 8 * C::kXStride + v * 64, x[v][u]);
+                    give_back();
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk) {
-                        uint32_t a[4];
-                        ldmatrix_x4_trans(wa + kk * 16 * 128, a);
+                    for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
                         for (int u = 0; u < NG; ++u)
-                            if (u < groups) mma_f16(acc[u], a, x[kk >> 1][u][2 * (kk & 1)], x[kk >> 1][u][2 * (kk & 1) + 1]);
-                    }
+                            if (u < groups) mma_f16(acc[u], a[kk], x[kk >> 1][u][2 * (kk & 1)], x[kk >> 1][u][2 * (kk & 1) + 1]);
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(empty_bar(s));
-                if (++s == STAGES) { s = 0; ph ^= 1; }
             }
             if (ok) {
-                float* dst;
-                size_t stride;
-                if (it.x == kFirst) {
-                    stride = 2 * (size_t)p.width;
-                    dst = p.part1 + ((size_t)it.w * (pairs + p.t) + first) * stride + it.z * 128 + w * 16;
-                } else {
-                    stride = p.d;
-                    dst = p.part2 + ((size_t)it.w * (pairs + p.t) + first) * stride + it.z * 128 + w * 16;
-                }
+                const size_t stride = it.x == kFirst ? 2 * (size_t)p.width : (size_t)p.d;
+                unsigned long long* dst = (it.x == kFirst ? p.part1 : p.part2) + ((size_t)it.w * rows + first) * stride + it.z * 128 + w * 16;
                 const bool inside = it.x == kFirst || it.z * 128 + w * 16 < p.d;
 #pragma unroll
                 for (int u = 0; u < NG; ++u)
 #pragma unroll
                     for (int v = 0; v < 4; ++v) {
                         const int r = 8 * u + 2 * q + (v & 1);
-                        if (r < n_rows && inside) dst[r * stride + g + 8 * (v >> 1)] = acc[u][v];
+                        if (r < n_rows && inside) st_word(dst + r * stride + g + 8 * (v >> 1), __float_as_uint(acc[u][v]), call);
                     }
             }
             __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(x_empty_bar(b));
-                mbar_arrive(done_bar(j));
-            }
+            if (lane == 0) mbar_arrive(x_empty_bar(b));
             ++n;
-        }
-        lost = !ok;
-    } else if (warp < WARP_ROUTE) {
-        // ------------------------------------------------------------------------------ finished items
-        const int w = warp - WARP_PUB;
-        bool ok = true;
-        for (uint32_t j = 0;; ++j) {
-            ok = ok && wait_item(j, kErrEpilogueWait);
-            const Item it = get_item(j);
-            if (ok && it.x != kEnd)
-                ok = mbar_wait(done_bar(j), (j / ITEM_SLOTS) & 1, p.status, kErrEpilogueWait, p.launch_tag);
-            if (ok && it.x == kSecond) ok = wait_routed(kErrEpilogueWait);
-            ok = named_barrier_all(BAR_PUB, 128, ok);
-            if (!ok || it.x == kEnd) break;
-            if (it.x == kRouter) {
-                if (w == 0 && lane == 0) {
-                    __threadfence();
-                    atomicAdd(p.head + kFewRouterDone, 1);
-                }
-            } else {
-                const int e = it.x == kFirst ? expert_of(it) : 0;
-                int* const count = it.x == kFirst ? p.count1 + e * p.tiles1_max + it.z : p.count2 + it.z;
-                const int want = it.x == kFirst ? shape.chunks1 : rt.n_active * shape.chunks2 + shape.chunks2s;
-                if (w == 0 && lane == 0) {
-                    __threadfence();
-                    const bool last = atomicAdd(count, 1) == want - 1;
-                    if (last) *count = 0;       // for the next call; nobody else comes here in this one
-                    __threadfence();
-                    rt.last = last;
-                }
-                named_barrier(BAR_PUB, 128);
-                if (rt.last) {
-                    const size_t rows = pairs + p.t;
-                    if (it.x == kFirst) {
-                        const int n_rows = pair_count(it), first = first_pair(it);
-                        for (int r = w; r < n_rows; r += 4) {
-                            const float* src = p.part1 + (size_t)(first + r) * 2 * p.width + it.z * 128 + 2 * lane;
-                            float2 gate = make_float2(0.f, 0.f), up = gate;
-#pragma unroll 8
-                            for (int c = 0; c < shape.chunks1; ++c) {
-                                const float2 a = ld_cg_f2(src + c * rows * 2 * p.width), b = ld_cg_f2(src + c * rows * 2 * p.width + 64);
-                                gate.x += a.x; gate.y += a.y;
-                                up.x += b.x; up.y += b.y;
-                            }
-                            const float hx = gate.x / (1.0f + expf(-gate.x)) * up.x, hy = gate.y / (1.0f + expf(-gate.y)) * up.y;
-                            *reinterpret_cast<uint32_t*>(static_cast<__half*>(p.h) + (size_t)(first + r) * p.width + it.z * 64 + 2 * lane) =
-                                pack_f16x2(hx, hy);
-                        }
-                        named_barrier(BAR_PUB, 128);
-                        if (w == 0 && lane == 0) {
-                            __threadfence();
-                            atomicAdd(done1 + e, 1);
-                        }
-                    } else {
-                        const int col = it.z * 128 + 4 * lane;
-                        for (int t = w; t < p.t && col < p.d; t += 4) {
-                            float4 y[kFewMaxTopK];
-#pragma unroll
-                            for (int i = 0; i < kFewMaxTopK; ++i) y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                            for (int c = 0; c < shape.chunks2; ++c)
-#pragma unroll
-                                for (int i = 0; i < kFewMaxTopK; ++i)
-                                    if (i < p.top_k) {
-                                        const float4 v = ld_global_cg_v4_f32(p.part2 + (c * rows + rt.pos[t * p.top_k + i]) * p.d + col);
-                                        y[i].x += v.x; y[i].y += v.y; y[i].z += v.z; y[i].w += v.w;
-                                    }
-                            float4 o = make_float4(0.f, 0.f, 0.f, 0.f), sh = o;
-#pragma unroll
-                            for (int i = 0; i < kFewMaxTopK; ++i)
-                                if (i < p.top_k) {
-                                    const float wt = rt.weight[t * p.top_k + i];
-                                    o.x = fmaf(wt, y[i].x, o.x); o.y = fmaf(wt, y[i].y, o.y);
-                                    o.z = fmaf(wt, y[i].z, o.z); o.w = fmaf(wt, y[i].w, o.w);
-                                }
-                            for (int c = 0; c < shape.chunks2s; ++c) {
-                                const float4 v = ld_global_cg_v4_f32(p.part2 + (c * rows + pairs + t) * p.d + col);
-                                sh.x += v.x; sh.y += v.y; sh.z += v.z; sh.w += v.w;
-                            }
-                            *reinterpret_cast<uint2*>(static_cast<__half*>(p.out) + (size_t)t * p.d + col) =
-                                make_uint2(pack_f16x2(o.x + sh.x, o.y + sh.y), pack_f16x2(o.z + sh.z, o.w + sh.w));
-                        }
-                    }
-                }
-            }
-            named_barrier(BAR_PUB, 128);        // rt.last has been read
-            if (w == 0 && lane == 0) mbar_arrive(free_bar(j));
         }
         lost = !ok;
     } else {
         // ------------------------------------------------------------------------------ routing
-        const int w = warp - WARP_ROUTE, tid = w * 32 + lane;
+        const int w = warp - WARP_SUM;
+        Patience patience(p.status, p.launch_tag);
         bool ok = true;
-        if (lane == 0) ok = counter_wait(p.head + kFewRouterDone, p.router_units, p.status, kErrSchedWait, p.launch_tag);
-        ok = named_barrier_all(BAR_ROUTE, 128, ok);
-        if (ok) {
-            // softmax and top-k as topk_kernel (moe_route.cu) does them, on the same fp16 roundings: lane l owns experts
-            // l * vpt ..; a key is an fp16 probability, then the complement of the expert's number
-            const int vpt = p.experts <= 32 ? 1 : p.experts / 32, e0 = lane * vpt;
-            const bool active = e0 < p.experts;
-            for (int t = w; t < p.t; t += 4) {
-                float l[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) l[i] = 0.f;
-                for (int c = 0; c < p.router_chunks; ++c)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (active && i < vpt) l[i] += ld_cg_f(p.logits + ((size_t)c * p.t + t) * p.experts + e0 + i);
-                float mx = -65504.0f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (active && i < vpt) {
-                        if (p.router_bias != nullptr) l[i] += ld_global_f32(p.router_bias + e0 + i);
-                        l[i] = __half2float(__float2half_rn(l[i]));
-                        mx = fmaxf(mx, l[i]);
-                    }
-#pragma unroll
-                for (int s = 16; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
-                float part = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (i < vpt) {
-                        l[i] = active ? det_exp(__fsub_rn(l[i], mx)) : 0.f;
-                        part = i == 0 ? l[0] : __fadd_rn(part, l[i]);
-                    }
-#pragma unroll
-                for (int s = 16; s > 0; s >>= 1) part = __fadd_rn(part, __shfl_xor_sync(0xffffffffu, part, s));
-                const float recip = __fdiv_rn(1.0f, part);
-                uint32_t key[8], mine = 0;
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    key[i] = active && i < vpt ? ((uint32_t)__half_as_ushort(__float2half_rn(__fmul_rn(l[i], recip))) << 16) |
-                                                     (0xFFFFu - (uint32_t)(e0 + i))
-                                               : 0u;
-                for (int k = 0; k < p.top_k; ++k) {
-                    uint32_t best = key[0];
-#pragma unroll
-                    for (int i = 1; i < 8; ++i) best = max(best, key[i]);
-                    best = __reduce_max_sync(0xffffffffu, best);
-                    if (lane == k) mine = best;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (key[i] == best) key[i] = 0u;
+        for (int t = w; t < p.t && ok; t += SUM_WARPS) {
+            if (p.experts <= 32) ok = route_token<1>(p, rt, t, call, patience);
+            else if (p.experts == 64) ok = route_token<2>(p, rt, t, call, patience);
+            else if (p.experts == 128) ok = route_token<4>(p, rt, t, call, patience);
+            else ok = route_token<8>(p, rt, t, call, patience);
+        }
+        ok = named_barrier_all(BAR_SUM, 32 * SUM_WARPS, ok);
+        if (ok && w == 0) build_lists(p, rt);
+        named_barrier(BAR_SUM, 32 * SUM_WARPS);
+        if (ok && w == 0 && lane == 0) mbar_arrive(routed_bar);
+        // ------------------------------------------------------------------------------ sums of complete tiles
+        for (uint32_t j = 0; ok; ++j) {
+            ok = __all_sync(0xffffffffu, mbar_wait(sum_bar(j), (j / SUM_SLOTS) & 1, p.status, kErrEpilogueWait, p.launch_tag));
+            if (!ok) break;
+            const Item it = read_item(sum_base + 16u * (j % SUM_SLOTS));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sum_free_bar(j));
+            if (it.x == kEnd) break;
+            Patience wait(p.status, p.launch_tag);
+            if (it.x == kFirst) {
+                // a warp per row, two columns a lane
+                const int n_rows = pair_count(it), first = first_pair(it);
+                for (int r = w; r < n_rows && ok; r += SUM_WARPS) {
+                    const unsigned long long* src = p.part1 + (size_t)(first + r) * 2 * p.width + it.z * 128 + 2 * lane;
+                    float2 gate, up;
+                    ok = sum_chunks(src, src + 64, rows * 2 * p.width, shape.chunks1, call, wait, &gate, &up);
+                    if (!ok) break;
+                    const float hx = gate.x / (1.0f + expf(-gate.x)) * up.x, hy = gate.y / (1.0f + expf(-gate.y)) * up.y;
+                    st_word(p.h + (size_t)(first + r) * (p.width / 2) + it.z * 32 + lane, pack_f16x2(hx, hy), call);
                 }
-                if (lane < p.top_k) {
-                    rt.expert[t * p.top_k + lane] = (int)(0xFFFFu - (mine & 0xFFFFu));
-                    rt.weight[t * p.top_k + lane] = __half2float(__ushort_as_half((unsigned short)(mine >> 16)));
+            } else {
+                // two warps per token, two columns a lane; the words of two chunks of every expert and of the shared one are in flight
+                const int col = it.z * 128 + (w & 1) * 64 + 2 * lane;
+                const size_t step = rows * p.d;
+                for (int t = w >> 1; t < p.t && it.z * 128 + (w & 1) * 64 < p.d && ok; t += SUM_WARPS / 2) {
+                    float2 y[kFewMaxTopK + 1];
+#pragma unroll
+                    for (int i = 0; i <= kFewMaxTopK; ++i) y[i] = make_float2(0.f, 0.f);
+                    for (int c0 = 0; c0 < max(shape.chunks2, shape.chunks2s) && ok; c0 += 2) {
+                        ulonglong2 v[kFewMaxTopK + 1][2];
+                        for (;;) {
+                            bool here = true;
+#pragma unroll
+                            for (int i = 0; i <= kFewMaxTopK; ++i)
+#pragma unroll
+                                for (int c = 0; c < 2; ++c) {
+                                    v[i][c] = make_ulonglong2(word_of(0, call), word_of(0, call));
+                                    const bool wanted = i < kFewMaxTopK ? i < p.top_k && c0 + c < shape.chunks2 : c0 + c < shape.chunks2s;
+                                    const int pair = i < kFewMaxTopK ? rt.pos[t * p.top_k + min(i, p.top_k - 1)] : pairs + t;
+                                    if (wanted) v[i][c] = ld_words(p.part2 + (size_t)(c0 + c) * step + (size_t)pair * p.d + col);
+                                }
+#pragma unroll
+                            for (int i = 0; i <= kFewMaxTopK; ++i)
+#pragma unroll
+                                for (int c = 0; c < 2; ++c) here = here && call_of(v[i][c].x) == call && call_of(v[i][c].y) == call;
+                            if (__all_sync(0xffffffffu, here)) break;
+                            ok = __all_sync(0xffffffffu, wait.more());
+                            if (!ok) break;
+                        }
+#pragma unroll
+                        for (int i = 0; i <= kFewMaxTopK; ++i)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) {
+                                y[i].x += float_of(v[i][c].x);
+                                y[i].y += float_of(v[i][c].y);
+                            }
+                    }
+                    float2 o = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int i = 0; i < kFewMaxTopK; ++i)
+                        if (i < p.top_k) {
+                            const float wt = rt.weight[t * p.top_k + i];
+                            o.x = fmaf(wt, y[i].x, o.x);
+                            o.y = fmaf(wt, y[i].y, o.y);
+                        }
+                    if (ok)
+                        *reinterpret_cast<uint32_t*>(static_cast<__half*>(p.out) + (size_t)t * p.d + col) =
+                            pack_f16x2(o.x + y[kFewMaxTopK].x, o.y + y[kFewMaxTopK].y);
                 }
             }
-            named_barrier(BAR_ROUTE, 128);
-            // the experts' token lists: a thread counts for two experts
-            int n[2] = {0, 0};
-            for (int i = 0; i < pairs; ++i) {
-                const int e = rt.expert[i];
-                n[0] += e == 2 * tid;
-                n[1] += e == 2 * tid + 1;
-            }
-            // pairs before (low half) and active experts before (high half)
-            const int mine = n[0] + n[1] + ((n[0] > 0) << 16) + ((n[1] > 0) << 16);
-            int incl = mine;
-#pragma unroll
-            for (int s = 1; s < 32; s <<= 1) {
-                const int o = __shfl_up_sync(0xffffffffu, incl, s);
-                if (lane >= s) incl += o;
-            }
-            if (lane == 31) rt.sums[w] = incl;
-            named_barrier(BAR_ROUTE, 128);
-            int before = incl - mine;
-            for (int i = 0; i < w; ++i) before += rt.sums[i];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (n[i] == 0) continue;
-                const int slot = before >> 16;
-                int pair = before & 0xFFFF;
-                rt.active[slot] = 2 * tid + i;
-                rt.base[slot] = pair;
-                for (int o = 0; o < pairs; ++o)
-                    if (rt.expert[o] == 2 * tid + i) {
-                        rt.token[pair] = o / p.top_k;
-                        rt.pos[o] = pair++;
-                    }
-                before += n[i] + (1 << 16);
-            }
-            if (tid == 127) {
-                rt.n_active = before >> 16;
-                rt.base[before >> 16] = pairs;
-            }
-            named_barrier(BAR_ROUTE, 128);
-            if (tid == 0) mbar_arrive(routed_bar);
         }
         lost = !ok;
     }

@@ -10,8 +10,8 @@ constexpr int kFewMaxTokens = 32;
 constexpr int kFewMaxExperts = 256;
 constexpr int kFewMaxTopK = 8;
 
-// Words in front of the workspace's counters
-enum { kFewTicket = 0, kFewRouterDone = 1, kFewExits = 2, kFewBad = 3, kFewHeadWords = 8 };
+// Words in front of the workspace (128 bytes apart: the ticket is drawn while the others are read)
+enum { kFewTicket = 0, kFewExits = 32, kFewBad = 64, kFewCalls = 96, kFewHeadWords = 128 };
 
 struct MoeFewParams {
     const void* x;                  // fp16 [t, d]
@@ -20,20 +20,17 @@ struct MoeFewParams {
     const CUtensorMap* maps;        // device: gate, up, down of every expert, then of the shared one
     const float* const* scales;     // device: the same order (FP8 weights)
     void* out;                      // fp16 [t, d]
-    // workspace
-    int* head;                      // kFewHeadWords, then done [experts + 1]: finished column tiles of an expert's first product
-    int* count1;                    // [experts + 1][tiles1_max] finished K chunks of a column tile, first product
-    int* count2;                    // [tiles2] finished items of a column tile of the result
-    float* logits;                  // [router_chunks][t][experts] partial sums
-    float* part1;                   // [chunks1][pairs][2 * width] partial sums of gate | up, 64 + 64 columns per tile
-    void* h;                        // fp16 [pairs][width]
-    float* part2;                   // [chunks2][pairs][d]
+    // workspace: words of 32 bits of data and the call's number
+    int* head;                      // kFewHeadWords
+    unsigned long long* logits;     // [router_chunks][t][experts] partial sums
+    unsigned long long* part1;      // [chunks1][pairs][2 * width] partial sums of gate | up, 64 + 64 columns per tile
+    unsigned long long* h;          // [pairs][width / 2] two fp16 values each
+    unsigned long long* part2;      // [chunks2][pairs][d] partial sums
     int t, d, f, fs;                // fs: the shared expert's width, 0 = none
     int experts, top_k;
     int width;                      // max(f, fs)
-    int tiles1_max;                 // width / 64
     int kc1, kc2;                   // K of an item of the first and the second product
-    int router_chunks, router_units;
+    int router_kc, router_chunks, router_units;
     int* status;
     int launch_tag;
 };
@@ -42,7 +39,8 @@ struct MoeFewParams {
 inline int moe_few_groups(int t) { return t <= 8 ? 1 : t <= 16 ? 2 : 4; }
 // Largest K chunk whose two operand buffers leave room for the weight stages.
 inline int moe_few_max_chunk(int t) { return t <= 16 ? 1024 : 512; }
-constexpr int kFewRouterChunk = 512;
+// K of a router unit: whole rounds of the eight MMA warps; longer for many experts, whose sums every CTA has to gather.
+inline int moe_few_router_chunk(int experts) { return experts <= 64 ? 512 : 1024; }
 
 cudaError_t moe_few_launch(const MoeFewParams& p, bool fp8, int num_sms, cudaStream_t stream);
 

@@ -23,8 +23,8 @@ size_t align_up(size_t v) { return (v + 255) / 256 * 256; }
 
 // What a call of t tokens needs: K chunks, and where the parts of the workspace lie.
 struct Plan {
-    int kc1, kc2, router_chunks;
-    size_t zeroed, count1, count2, logits, part1, h, part2, bytes;
+    int kc1, kc2, router_kc, router_chunks;
+    size_t logits, part1, h, part2, bytes;
 };
 
 // The longest K chunk that still gives `tiles` column tiles enough items for an even load on every SM; chunks below 256 would
@@ -44,18 +44,15 @@ Plan make_plan(const RfMoeFewConfig& c, int t) {
     Plan p;
     p.kc1 = choose_chunk((hit * c.d_expert + fs) / 64, c.d_hidden, most, num_sms);
     p.kc2 = choose_chunk((hit + (fs > 0)) * ((c.d_hidden + 127) / 128), c.d_expert, most, num_sms);
-    p.router_chunks = (c.d_hidden + rf::kFewRouterChunk - 1) / rf::kFewRouterChunk;
+    p.router_kc = rf::moe_few_router_chunk(c.n_routed_experts);
+    p.router_chunks = (c.d_hidden + p.router_kc - 1) / p.router_kc;
     const size_t chunks1 = (d + p.kc1 - 1) / p.kc1, chunks2 = ((size_t)width + p.kc2 - 1) / p.kc2;
-    // counters first: their place does not depend on t
-    size_t b = align_up((rf::kFewHeadWords + c.n_routed_experts + 1) * sizeof(int));
-    auto take = [&](size_t n) { const size_t at = b; b += align_up(n); return at; };
-    p.count1 = take((size_t)(c.n_routed_experts + 1) * (width / 64) * sizeof(int));
-    p.count2 = take((d + 127) / 128 * sizeof(int));
-    p.zeroed = b;
-    p.logits = take((size_t)p.router_chunks * t * c.n_routed_experts * sizeof(float));
-    p.part1 = take(chunks1 * pairs * 2 * width * sizeof(float));
-    p.h = take(pairs * width * 2);
-    p.part2 = take(chunks2 * pairs * d * sizeof(float));
+    size_t b = rf::kFewHeadWords * sizeof(int);
+    auto take = [&](size_t words) { const size_t at = b; b += align_up(words * 8); return at; };
+    p.logits = take((size_t)p.router_chunks * t * c.n_routed_experts);
+    p.part1 = take(chunks1 * pairs * 2 * width);
+    p.h = take(pairs * width / 2);
+    p.part2 = take(chunks2 * pairs * d);
     p.bytes = b;
     return p;
 }
@@ -153,12 +150,51 @@ int rf_moe_few_destroy(RfMoeFew* few) {
     return e == cudaSuccess ? RF_OK : RF_ERR_CUDA;
 }
 
-size_t rf_moe_few_workspace_bytes(const RfMoeFewConfig* config, int n_tokens, size_t* zeroed_bytes) {
-    if (zeroed_bytes) *zeroed_bytes = 0;
+size_t rf_moe_few_workspace_bytes(const RfMoeFewConfig* config, int n_tokens) {
     if (!config || check_config(*config) != RF_OK || n_tokens < 1 || n_tokens > rf::kFewMaxTokens) return 0;
-    const Plan p = make_plan(*config, n_tokens);
-    if (zeroed_bytes) *zeroed_bytes = p.zeroed;
-    return p.bytes;
+    return make_plan(*config, n_tokens).bytes;
+}
+
+int rf_moe_few_workspace_alloc(size_t bytes, void** out) {
+    if (!out) return RF_ERR_NULL_POINTER;
+    *out = nullptr;
+    if (!rf::device_state()) return RF_ERR_CUDA;
+    // Allowed while a stream of this thread is being captured: nothing here touches that stream.
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return RF_ERR_CUDA;
+    void* p = nullptr;
+    cudaStream_t s = nullptr;
+    cudaError_t e = cudaMalloc(&p, bytes);
+    if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, bytes, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    if (s) cudaStreamDestroy(s);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        if (p) cudaFree(p);
+        p = nullptr;
+    }
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    *out = p;
+    return e == cudaSuccess ? RF_OK : RF_ERR_CUDA;
+}
+
+int rf_moe_few_workspace_free(void* workspace) {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return RF_ERR_CUDA;
+    const cudaError_t e = cudaFree(workspace);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    return e == cudaSuccess ? RF_OK : RF_ERR_CUDA;
+}
+
+int rf_stream_capture_id(rf_stream_t stream, unsigned long long* id) {
+    if (!id) return RF_ERR_NULL_POINTER;
+    *id = 0;
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long n = 0;
+    if (cudaStreamGetCaptureInfo(reinterpret_cast<cudaStream_t>(stream), &status, &n) != cudaSuccess) return RF_ERR_CUDA;
+    if (status != cudaStreamCaptureStatusNone) *id = n + 1;
+    return RF_OK;
 }
 
 int rf_moe_few_forward(RfMoeFew* few, const void* x, int n_tokens, void* out, void* workspace, size_t workspace_bytes,
@@ -184,12 +220,10 @@ int rf_moe_few_forward(RfMoeFew* few, const void* x, int n_tokens, void* out, vo
     p.scales = few->scales;
     p.out = out;
     p.head = reinterpret_cast<int*>(ws);
-    p.count1 = reinterpret_cast<int*>(ws + plan.count1);
-    p.count2 = reinterpret_cast<int*>(ws + plan.count2);
-    p.logits = reinterpret_cast<float*>(ws + plan.logits);
-    p.part1 = reinterpret_cast<float*>(ws + plan.part1);
-    p.h = ws + plan.h;
-    p.part2 = reinterpret_cast<float*>(ws + plan.part2);
+    p.logits = reinterpret_cast<unsigned long long*>(ws + plan.logits);
+    p.part1 = reinterpret_cast<unsigned long long*>(ws + plan.part1);
+    p.h = reinterpret_cast<unsigned long long*>(ws + plan.h);
+    p.part2 = reinterpret_cast<unsigned long long*>(ws + plan.part2);
     p.t = n_tokens;
     p.d = c.d_hidden;
     p.f = c.d_expert;
@@ -197,9 +231,9 @@ int rf_moe_few_forward(RfMoeFew* few, const void* x, int n_tokens, void* out, vo
     p.experts = c.n_routed_experts;
     p.top_k = c.n_experts_per_token;
     p.width = p.fs > p.f ? p.fs : p.f;
-    p.tiles1_max = p.width / 64;
     p.kc1 = plan.kc1;
     p.kc2 = plan.kc2;
+    p.router_kc = plan.router_kc;
     p.router_chunks = plan.router_chunks;
     p.router_units = (p.experts + 15) / 16 * p.router_chunks;
     p.status = st->status;

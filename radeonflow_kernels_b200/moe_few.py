@@ -7,6 +7,7 @@ to fp16, equal ones by the lowest index.  Unlike the layer it rounds nothing bet
 vector between an expert's two products, to fp16.
 """
 import ctypes
+import weakref
 
 import torch
 
@@ -18,6 +19,23 @@ BLOCK = 128
 _SHARED = "shared_experts"
 
 
+class _Workspace:
+    """Zeroed device memory, freed with the last layer that uses it."""
+
+    def __init__(self, size):
+        self.size, ptr = size, ctypes.c_void_p()
+        _lib.check(_lib.lib().rf_moe_few_workspace_alloc(size, ctypes.byref(ptr)), "rf_moe_few_workspace_alloc")
+        self.ptr, self._free = ptr.value, _lib.lib().rf_moe_few_workspace_free
+
+    def __del__(self):
+        if getattr(self, "ptr", None):
+            self._free(self.ptr)
+
+
+# (device, stream, capture) -> workspace.  The layers of a model run one after the other on a stream, so they share them.
+_workspaces = weakref.WeakValueDictionary()
+
+
 class FewTokenMoE:
     """One layer's handle: what its kernel needs of the weights, which have to stay where they are.
 
@@ -27,16 +45,19 @@ class FewTokenMoE:
     'shared_experts' without the leading axis).  ``config``: d_hidden, d_expert, n_routed_experts (a power of two, at most 256),
     n_experts_per_token (at most 8), n_shared_experts (0: no shared expert).  ``router_bias``: fp32 [E], added to the logits.
 
-    Calls on different streams may overlap: each stream has a workspace of its own, and so has each captured call.
+    Calls on different streams may overlap: each stream has a workspace of its own, which the layers called on it share, and so
+    has each capture.  A captured graph uses the handle's tables and workspace: the handle has to outlive it.
     """
 
     def __init__(self, weights, config, router_bias=None):
         d, f, e = (int(config[k]) for k in ("d_hidden", "d_expert", "n_routed_experts"))
         n_shared = int(config["n_shared_experts"])
         self._handle = None
+        self._capture = ctypes.c_ulonglong()
+        self._capture_ref = ctypes.byref(self._capture)
         self.fp8 = "experts.gate_up.weight" in weights
         self.config = _lib.RfMoeFewConfig(d, f, e, int(config["n_experts_per_token"]), n_shared, int(self.fp8))
-        self.d_hidden, self._workspaces, self._sizes = d, {}, {}
+        self.d_hidden, self._held, self._sizes = d, {}, {}
         router = weights["router.weight"]
         _check_fp16_cuda("router.weight", router)
         self.device = router.device
@@ -56,7 +77,7 @@ class FewTokenMoE:
                                           None if router_bias is None else router_bias.data_ptr(), *arrays, *scale_arrays,
                                           ctypes.byref(handle))
         _lib.check(st, "rf_moe_few_create")
-        self._handle = handle
+        self._handle, self._destroy = handle, _lib.lib().rf_moe_few_destroy
 
     def _check_device(self, what):
         if self.device.index != torch.cuda.current_device():
@@ -98,24 +119,28 @@ class FewTokenMoE:
         return rows, scales
 
     def _workspace(self, n_tokens, stream):
+        L = _lib.lib()
         size = self._sizes.get(n_tokens)
         if size is None:
-            zeroed = ctypes.c_size_t()
-            n = _lib.lib().rf_moe_few_workspace_bytes(ctypes.byref(self.config), n_tokens, ctypes.byref(zeroed))
-            size = self._sizes[n_tokens] = (n, zeroed.value)
-        captured = torch.cuda.is_current_stream_capturing()
-        ws = None if captured else self._workspaces.get(stream)
-        if ws is None or ws.numel() < size[0]:
-            ws = torch.empty(size[0], dtype=torch.uint8, device=self.device)
-            ws[:size[1]].zero_()
-            if not captured:        # (a captured call's is the graph's: every replay zeroes it again)
-                self._workspaces[stream] = ws
-        return ws
+            size = self._sizes[n_tokens] = L.rf_moe_few_workspace_bytes(ctypes.byref(self.config), n_tokens)
+        _lib.check(L.rf_stream_capture_id(stream, self._capture_ref), "rf_stream_capture_id")
+        key = (self.device.index, stream, self._capture.value)
+        ws = self._held.get(key)
+        if ws is None or ws[-1].size < size:
+            shared = _workspaces.get(key)
+            if shared is None or shared.size < size:
+                # (one that has become too small stays: earlier calls, or a graph, may still use it)
+                shared = _workspaces[key] = _Workspace(1 << (size - 1).bit_length())
+            ws = self._held.setdefault(key, [])
+            ws.append(shared)
+        return ws[-1]
 
     def reset(self):
-        """Forgets the workspaces.  Needed after `gemm.device_status()` has told of a lost wait: until then every call with a
-        workspace that such a call left behind refuses to run and reports a lost wait again."""
-        self._workspaces.clear()
+        """Forgets the workspaces of this process's layers.  Needed after `gemm.device_status()` has told of a lost wait: until then
+        every call with a workspace that such a call left behind refuses to run and reports a lost wait again.  The other layers
+        have to be reset too.  Graphs captured before it must not be replayed after it."""
+        _workspaces.clear()
+        self._held.clear()
 
     def forward(self, x, out=None):
         """x fp16 [..., d_hidden], 1 to 32 tokens -> out, same shape.  Enqueues one kernel on the current stream."""
@@ -135,10 +160,10 @@ class FewTokenMoE:
             return out
         stream = _lib.current_stream()
         ws = self._workspace(n_tokens, stream)
-        st = _lib.lib().rf_moe_few_forward(self._handle, x.data_ptr(), n_tokens, out.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+        st = _lib.lib().rf_moe_few_forward(self._handle, x.data_ptr(), n_tokens, out.data_ptr(), ws.ptr, ws.size, stream)
         _lib.check(st, "rf_moe_few_forward")
         return out
 
     def __del__(self):
         if getattr(self, "_handle", None):
-            _lib.lib().rf_moe_few_destroy(self._handle)
+            self._destroy(self._handle)

@@ -8,6 +8,8 @@ every step, and 40 more additions of partial sums:
     dg <= s(d) sum |x||Wg|, du likewise;  dh <= u |h| + 2^-24 + 1.1 dg |u| + |silu(g)| du + 2^-20 |h|     (1.1 >= |silu'|)
     dy <= sum dh |Wd| + s(f) sum |h||Wd|;  dout <= u |out| + 2^-25 + (1 + 2^-20) sum_i p_i dy_i
 """
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -229,8 +231,10 @@ def test_a_marked_workspace_is_refused_until_reset():
     want = layer.forward(x)
     torch.cuda.synchronize()
     assert gemm.device_status() == 0
-    for ws in layer._workspaces.values():
-        ws[12:16].view(torch.int32).fill_(1)             # the mark
+    one, mark = ctypes.c_int(1), [held[-1].ptr + 256 for held in layer._held.values()]
+    cudart = ctypes.CDLL("libcudart.so.12")
+    for at in mark:
+        assert cudart.cudaMemcpy(ctypes.c_void_p(at), ctypes.byref(one), ctypes.c_size_t(4), 1) == 0
     out = torch.full_like(x, 5.0)
     layer.forward(x, out=out)
     assert gemm.device_status() == 5 and (out == 5).all()
