@@ -37,7 +37,7 @@ namespace {
 constexpr int WARP_X = 1, WARP_MMA = 4, WARP_SUM = 12, WARPS = 16;
 constexpr int X_WARPS = WARP_MMA - WARP_X, MMA_WARPS = WARP_SUM - WARP_MMA, SUM_WARPS = WARPS - WARP_SUM;
 constexpr int THREADS = 32 * WARPS;
-constexpr int BAR_MMA = 1, BAR_SUM = 2;
+constexpr int BAR_SUM = 1;
 constexpr int STAGE_BYTES = 16384, BOX_BYTES = 8192;
 constexpr int ITEM_SLOTS = 8, SUM_SLOTS = 8;
 constexpr int DRAW_AHEAD = 4;           // stages before an item's last load at which the next ticket is drawn
@@ -56,6 +56,7 @@ struct Routing {
     int pos[MAX_PAIRS];                 // pair of [token][rank]
     float weight[MAX_PAIRS];            // [token][rank]
     int count[kFewMaxExperts];
+    float logits[SUM_WARPS][kFewMaxExperts];
 };
 
 template <bool FP8, int NG>
@@ -63,14 +64,16 @@ struct Cfg {
     static constexpr int kStageK = FP8 ? 128 : 64;
     static constexpr int kRows = 8 * NG;
     static constexpr int kMaxChunk = NG == 4 ? 512 : 1024;
-    // fp16 operands go through ldmatrix (rows 16 bytes apart modulo 128), those of FP8 through 8-byte loads (32 bytes)
-    static constexpr int kPad = FP8 ? 32 : 16;
+    // beside fp16 weights x goes through ldmatrix (rows 16 bytes apart modulo 128), beside FP8 through 16-byte loads (64 bytes)
+    static constexpr int kPad = FP8 ? 64 : 16;
     static constexpr int kXStride = kMaxChunk * 2 + kPad;
     // ... and behind the rows the scales of the item's two boxes, one per 128 of K
     static constexpr int kXBytes = kRows * kXStride + (FP8 ? 64 : 0);
+    // a router unit's partial sums of every MMA warp; later the sums that one group of them hands to the other
     static constexpr int kRedBytes = MMA_WARPS * 16 * kRows * 4;
+    static_assert(kRedBytes == MMA_WARPS / 2 * 2 * NG * 4 * 128, "both uses");
     static constexpr int kStages = NG == 1 ? 11 : 8;
-    static constexpr int kBars = 2 * kStages + 4 + 2 * ITEM_SLOTS + 2 * SUM_SLOTS + 1;
+    static constexpr int kBars = 2 * kStages + 4 + 2 * ITEM_SLOTS + 2 * SUM_SLOTS + 2 + MMA_WARPS;
     static constexpr int kSmemBytes = kStages * STAGE_BYTES + 2 * kXBytes + kRedBytes + (ITEM_SLOTS + SUM_SLOTS) * 16 + kBars * 8 +
                                       (int)sizeof(Routing) + 1024;
     static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
@@ -83,6 +86,9 @@ __device__ __forceinline__ unsigned long long word_of(uint32_t data, uint32_t ca
 }
 __device__ __forceinline__ void st_word(unsigned long long* p, uint32_t data, uint32_t call) {
     asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(word_of(data, call)) : "memory");
+}
+__device__ __forceinline__ void st_words(unsigned long long* p, uint32_t a, uint32_t b, uint32_t call) {
+    asm volatile("st.relaxed.gpu.global.v2.u64 [%0], {%1, %2};" ::"l"(p), "l"(word_of(a, call)), "l"(word_of(b, call)) : "memory");
 }
 __device__ __forceinline__ unsigned long long ld_word(const unsigned long long* p) {
     unsigned long long v;
@@ -176,6 +182,20 @@ __device__ __forceinline__ bool sum_chunks(const unsigned long long* a, const un
     return true;
 }
 
+// mbar_wait for the roles that mostly wait: they sleep between polls, which would take issue slots and shared memory cycles from the
+// MMA warps.
+__device__ __forceinline__ bool idle_wait(uint32_t bar, uint32_t parity, int* status, int code, int tag) {
+    for (int i = 0; i < 4; ++i)
+        if (mbar_try_wait(bar, parity)) return true;
+    Patience patience(status, tag);
+    while (!mbar_try_wait(bar, parity)) {
+        __nanosleep(64);
+        if (!patience.more()) return false;
+    }
+    (void)code;
+    return true;
+}
+
 // How the work divides: known once the routing is.
 struct Shape {
     int tiles1, tiles1s;        // column tiles of the first product: of an expert, of the shared one
@@ -212,11 +232,13 @@ __device__ __forceinline__ Item decode_routed(int r, const Shape& s, int n_activ
 // roundings.  Lane l owns experts l * VPT ..; a key is an fp16 probability, then the complement of the expert's number.
 template <int VPT>
 __device__ __forceinline__ bool route_token(const MoeFewParams& p, Routing& rt, int t, uint32_t call, Patience& patience) {
-    constexpr int BATCH = 16 / VPT < 8 ? 16 / VPT : 8;          // chunks whose loads are in flight together
+    constexpr int BATCH = 32 / VPT < 8 ? 32 / VPT : 8;          // chunks whose loads are in flight together
     const int lane = threadIdx.x & 31, e0 = lane * VPT;
     const bool active = e0 < p.experts;
-    const unsigned long long* src = p.logits + (size_t)t * p.experts + (active ? e0 : 0);
+    const unsigned long long* src = p.logits + (size_t)t * p.experts;
     const size_t step = (size_t)p.t * p.experts;
+    // The words are read side by side (two experts a lane, 512 bytes a load) ...
+    float* row = rt.logits[(threadIdx.x >> 5) % SUM_WARPS];
     float l[VPT];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) l[i] = 0.f;
@@ -228,11 +250,11 @@ __device__ __forceinline__ bool route_token(const MoeFewParams& p, Routing& rt, 
             for (int c = 0; c < BATCH; ++c) {
                 const unsigned long long* at = src + (size_t)min(c0 + c, p.router_chunks - 1) * step;
                 if (VPT == 1) {
-                    v[c][0] = ld_word(at);
+                    v[c][0] = ld_word(at + min(lane, p.experts - 1));
                 } else {
 #pragma unroll
                     for (int i = 0; i < VPT / 2; ++i) {
-                        const ulonglong2 w = ld_words(at + 2 * i);
+                        const ulonglong2 w = ld_words(at + 64 * i + 2 * lane);
                         v[c][2 * i] = w.x;
                         v[c][VPT == 1 ? 0 : 2 * i + 1] = w.y;
                     }
@@ -250,6 +272,15 @@ __device__ __forceinline__ bool route_token(const MoeFewParams& p, Routing& rt, 
             if (c0 + c < p.router_chunks)
 #pragma unroll
                 for (int i = 0; i < VPT; ++i) l[i] += float_of(v[c][i]);
+    }
+    // ... and change places for the softmax
+    if (VPT > 1) {
+#pragma unroll
+        for (int i = 0; i < VPT / 2; ++i) *reinterpret_cast<float2*>(row + 64 * i + 2 * lane) = make_float2(l[2 * i], l[VPT == 1 ? 0 : 2 * i + 1]);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) l[i] = row[e0 + i];
+        __syncwarp();
     }
     float mx = -65504.0f;
     if (active)
@@ -366,6 +397,9 @@ moe_few_kernel(const MoeFewParams p) {
     auto sum_bar = [&](uint32_t j) { return bar_base + 8u * (2 * STAGES + 4 + 2 * ITEM_SLOTS + j % SUM_SLOTS); };
     auto sum_free_bar = [&](uint32_t j) { return bar_base + 8u * (2 * STAGES + 4 + 2 * ITEM_SLOTS + SUM_SLOTS + j % SUM_SLOTS); };
     const uint32_t routed_bar = bar_base + 8u * (2 * STAGES + 4 + 2 * ITEM_SLOTS + 2 * SUM_SLOTS);
+    const uint32_t meet_bar = routed_bar + 8;
+    auto merge_bar = [&](uint32_t i) { return meet_bar + 8u * (1 + i); };
+    auto merge_free_bar = [&](uint32_t i) { return meet_bar + 8u * (1 + MMA_WARPS / 2 + i); };
     Routing& rt = *reinterpret_cast<Routing*>(smem_raw + (bar_base + 8u * C::kBars - smem_u32(smem_raw)));
 
     const int warp = threadIdx.x >> 5;
@@ -374,7 +408,11 @@ moe_few_kernel(const MoeFewParams p) {
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(full_bar(s), 1);
-            mbar_init(empty_bar(s), MMA_WARPS);
+            mbar_init(empty_bar(s), FP8 ? MMA_WARPS / 2 : MMA_WARPS);
+        }
+        for (int i = 0; i < MMA_WARPS / 2; ++i) {
+            mbar_init(merge_bar(i), 1);
+            mbar_init(merge_free_bar(i), 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(x_full_bar(b), X_WARPS);
@@ -389,8 +427,10 @@ moe_few_kernel(const MoeFewParams p) {
             mbar_init(sum_free_bar(j), SUM_WARPS);
         }
         mbar_init(routed_bar, 1);
+        mbar_init(meet_bar, MMA_WARPS);
         mbar_fence_init();
     }
+    if (warp == WARP_SUM && lane < 3 && p.fs > 0) tma_prefetch_desc(p.maps + 3 * p.experts + lane);
     griddep_wait();
     // The number of this call: zero, which fresh words hold, is left out.  (A word that no call has written for the 2^32 - 1 calls
     // before this one could pass for this call's.)
@@ -409,7 +449,7 @@ moe_few_kernel(const MoeFewParams p) {
     const int before_routed = p.router_units + shared_first;
     const int pairs = p.t * p.top_k;            // the shared expert's pairs come behind them, one per token
     const size_t rows = pairs + p.t;            // of h and the partial sums
-    auto wait_routed = [&](int code) { return mbar_wait(routed_bar, 0, p.status, code, p.launch_tag); };
+    auto wait_routed = [&](int code) { return idle_wait(routed_bar, 0, p.status, code, p.launch_tag); };
     auto wait_item = [&](uint32_t j, int code) {
         return mbar_wait(item_bar(j), (j / ITEM_SLOTS) & 1, p.status, code, p.launch_tag);
     };
@@ -451,14 +491,14 @@ moe_few_kernel(const MoeFewParams p) {
                     }
                     it = decode_routed(ticket - before_routed, shape, rt.n_active);
                 }
-                ok = mbar_wait(free_bar(j), ((j / ITEM_SLOTS) & 1) ^ 1, p.status, kErrProducerWait, p.launch_tag);
+                ok = idle_wait(free_bar(j), ((j / ITEM_SLOTS) & 1) ^ 1, p.status, kErrProducerWait, p.launch_tag);
                 if (!ok) break;
                 st_shared_v4(item_base + 16u * (j % ITEM_SLOTS), it.x, it.y, it.z, it.w);
                 mbar_arrive(item_bar(j));
                 // the last chunk of a column tile, the last item of a result tile
                 if (it.x == kEnd || (it.x == kFirst && it.w == shape.chunks1 - 1) ||
                     (it.x == kSecond && it.y == rt.n_active - 1 && it.w == shape.chunks2 - 1)) {
-                    ok = mbar_wait(sum_free_bar(sums), ((sums / SUM_SLOTS) & 1) ^ 1, p.status, kErrProducerWait, p.launch_tag);
+                    ok = idle_wait(sum_free_bar(sums), ((sums / SUM_SLOTS) & 1) ^ 1, p.status, kErrProducerWait, p.launch_tag);
                     if (!ok) break;
                     st_shared_v4(sum_base + 16u * (sums % SUM_SLOTS), it.x, it.y, it.z, it.w);
                     mbar_arrive(sum_bar(sums++));
@@ -477,7 +517,7 @@ moe_few_kernel(const MoeFewParams p) {
                 const int n_stages = len / C::kStageK;
                 for (int i = 0; i < n_stages; ++i, ++st) {
                     if (i == max(n_stages - DRAW_AHEAD, 0)) ticket = atomicAdd(p.head + kFewTicket, 1);
-                    ok = mbar_wait(empty_bar(s), ph, p.status, kErrProducerWait, p.launch_tag);
+                    ok = idle_wait(empty_bar(s), ph, p.status, kErrProducerWait, p.launch_tag);
                     if (!ok) break;
                     const uint32_t dst = smem_base + s * STAGE_BYTES;
                     const int k = k0 + i * C::kStageK;
@@ -497,7 +537,7 @@ moe_few_kernel(const MoeFewParams p) {
         bool ok = true, routed = false;
         uint32_t n = 0;         // items with rows so far
         for (uint32_t j = 0; ok; ++j) {
-            ok = __all_sync(0xffffffffu, wait_item(j, kErrMmaWaitFull));
+            ok = __all_sync(0xffffffffu, idle_wait(item_bar(j), (j / ITEM_SLOTS) & 1, p.status, kErrMmaWaitFull, p.launch_tag));
             if (!ok) break;
             const Item it = get_item(j);
             __syncwarp();
@@ -512,7 +552,7 @@ moe_few_kernel(const MoeFewParams p) {
             int k0, len;
             k_range(it, &k0, &len);
             const uint32_t b = n & 1;
-            ok = __all_sync(0xffffffffu, mbar_wait(x_empty_bar(b), ((n >> 1) & 1) ^ 1, p.status, kErrMmaWaitFull, p.launch_tag));
+            ok = __all_sync(0xffffffffu, idle_wait(x_empty_bar(b), ((n >> 1) & 1) ^ 1, p.status, kErrMmaWaitFull, p.launch_tag));
             if (!ok) break;
             const int n_rows = pair_count(it), first = first_pair(it);
             const uint32_t dst = x_base + b * C::kXBytes;
@@ -579,20 +619,27 @@ moe_few_kernel(const MoeFewParams p) {
         // ------------------------------------------------------------------------------ MMA
         const int w = warp - WARP_MMA;
         const int g = lane >> 2, q = lane & 3;      // row (column) of the fragments, pair inside
-        const uint32_t box = (w >> 2) * BOX_BYTES;
+        const uint32_t box = (w >> 2) * BOX_BYTES;      // (fp16: 16 columns a warp)
         bool ok = true, routed = false;
-        uint32_t n = 0, s = 0, ph = 0;
+        uint32_t n = 0, s = 0, ph = 0, met = 0;
+        // A barrier of the MMA warps with a limit: a warp that gave a wait up does not come.
+        auto meet = [&] {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(meet_bar);
+            return __all_sync(0xffffffffu, mbar_wait(meet_bar, met++ & 1, p.status, kErrMmaWaitFull, p.launch_tag)) != 0;
+        };
         for (uint32_t j = 0;; ++j) {
-            ok = ok && wait_item(j, kErrMmaWaitFull);
-            Item it = get_item(j);
-            if (ok && it.x != kRouter && it.x != kEnd && it.y >= 0 && !routed) {
-                ok = wait_routed(kErrMmaWaitFull);
-                routed = true;
-            }
-            ok = named_barrier_all(BAR_MMA, 32 * MMA_WARPS, ok);       // all of the group go on, or none: they meet at barriers below
+            ok = ok && __all_sync(0xffffffffu, wait_item(j, kErrMmaWaitFull));
             if (!ok) break;
+            const Item it = get_item(j);
+            __syncwarp();
             if (lane == 0) mbar_arrive(free_bar(j));
             if (it.x == kEnd) break;
+            if (it.x != kRouter && it.y >= 0 && !routed) {
+                ok = __all_sync(0xffffffffu, wait_routed(kErrMmaWaitFull));
+                if (!ok) break;
+                routed = true;
+            }
             if (it.x == kRouter) {
                 // 16 experts x a chunk of K, 64 columns per warp and round.  A lane holds 16 consecutive k of its row (and token): the
                 // order of k inside a fragment is free as long as both operands share it.
@@ -631,7 +678,9 @@ moe_few_kernel(const MoeFewParams p) {
 #pragma unroll
                     for (int v = 0; v < 4; ++v)
                         st_shared_f32(mine + ((g + 8 * (v >> 1)) * C::kRows + 8 * i + 2 * q + (v & 1)) * 4, acc[i][v]);
-                named_barrier(BAR_MMA, 32 * MMA_WARPS);
+                // (met: all have written; met again: all have read, and the next unit may write)
+                ok = meet();
+                if (!ok) break;
                 for (int i = w * 32 + lane; i < 16 * C::kRows; i += 32 * MMA_WARPS) {
                     const int e = e0 + i / C::kRows, t = i % C::kRows;
                     float v = 0.f;
@@ -640,6 +689,7 @@ moe_few_kernel(const MoeFewParams p) {
                         v += __uint_as_float(ld_shared_u32(red_base + (o * 16 * C::kRows + i) * 4));
                     if (e < p.experts && t < p.t) st_word(p.logits + ((size_t)c * p.t + t) * p.experts + e, __float_as_uint(v), call);
                 }
+                ok = meet();
                 continue;
             }
             int k0, len;
@@ -649,7 +699,7 @@ moe_few_kernel(const MoeFewParams p) {
             ok = __all_sync(0xffffffffu, mbar_wait(x_full_bar(b), (n >> 1) & 1, p.status, kErrMmaWaitFull, p.launch_tag));
             const uint32_t xb = x_base + b * C::kXBytes;
             const int groups = (n_rows + 7) >> 3;
-            float acc[NG][4] = {};
+            float acc[FP8 ? 2 * NG : NG][4] = {};       // FP8: two tiles of 16 columns for each 8 tokens
             const int n_stages = len / C::kStageK;
             auto next_stage = [&] {
                 const bool here = __all_sync(0xffffffffu, mbar_wait(full_bar(s), ph, p.status, kErrMmaWaitFull, p.launch_tag));
@@ -661,62 +711,96 @@ moe_few_kernel(const MoeFewParams p) {
                 if (++s == STAGES) { s = 0; ph ^= 1; }
             };
             if (FP8) {
-                // Rows are output columns; a lane takes 4 consecutive k of its two rows per MMA.  A stage's words are in registers
-                // before the stage in front of it is multiplied, so that barrier and load latency lie under the conversions; two
-                // chains of MMAs alternate.
-                const int r0 = (w & 3) * 16 + g;
-                const uint32_t scales = xb + C::kRows * C::kXStride + (w >> 2) * 32;
-                uint32_t lo[2][8], hi[2][8];
-                auto load = [&](uint32_t (&l)[8], uint32_t (&h)[8]) {
-                    const uint32_t row = smem_base + s * STAGE_BYTES + box + r0 * 128 + 4 * q;
+                // Two groups of four warps take the item's stages in turn, 32 columns a warp: while one group waits and loads, the
+                // other multiplies, and a row of x is read by half as many warps.  (All eight on every stage, 16 columns each:
+                // barrier, loads, conversions and MMAs of a stage come one after the other, 540 cycles; so 360.)  Which of the
+                // MMA's 16 rows is which column, and the order of k inside it, are free as long as both operands and the result
+                // agree: rows g and g + 8 are columns 2g and 2g + 1 (their 8-byte pieces lie in banks of their own), a lane
+                // takes 8 consecutive k for two MMAs.  Rows of x that hold no token are not read.
+                const int group = w >> 2, c0 = (w & 3) * 32 + 2 * g;
+                const uint32_t scales = xb + C::kRows * C::kXStride + ((w >> 1) & 1) * 32;
+                for (int i = group; i < n_stages; i += 2) {
+                    const bool wrap = s + i >= (uint32_t)STAGES;
+                    const uint32_t si = s + i - (wrap ? STAGES : 0);
+                    ok = __all_sync(0xffffffffu, mbar_wait(full_bar(si), ph ^ (wrap ? 1u : 0u), p.status, kErrMmaWaitFull, p.launch_tag));
+                    if (!ok) break;
+                    uint2 l[2][4], h[2][4];
 #pragma unroll
-                    for (int kk = 0; kk < 8; ++kk) {
-                        const uint32_t off = (uint32_t)((kk ^ (r0 & 7)) << 4);
-                        l[kk] = ld_shared_u32(row + off);
-                        h[kk] = ld_shared_u32(row + 8 * 128 + off);
+                    for (int t = 0; t < 2; ++t) {
+                        const int col = c0 + 16 * t;            // (64 columns to a box of 8 KB)
+                        const uint32_t row = smem_base + si * STAGE_BYTES + col * 128 + 8 * (q & 1);
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) {
+                            l[t][b] = ld_shared_v2(row + (((2 * b + (q >> 1)) ^ (col & 7)) << 4));
+                            h[t][b] = ld_shared_v2(row + 128 + (((2 * b + (q >> 1)) ^ ((col + 1) & 7)) << 4));
+                        }
                     }
-                };
-                auto multiply = [&](int i, const uint32_t (&l)[8], const uint32_t (&h)[8]) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(empty_bar(si));
                     const float sc = __uint_as_float(ld_shared_u32(scales + i * 4));
 #pragma unroll
                     for (int u = 0; u < NG; ++u) {
                         if (u >= groups) break;
-                        float part[4] = {}, odd[4] = {};
-                        uint2 x[8];
+                        float part[2][4] = {};
+                        uint4 x[4];
 #pragma unroll
-                        for (int kk = 0; kk < 8; ++kk)
-                            x[kk] = ld_shared_v2(xb + (8 * u + g) * C::kXStride + 2 * (i * 128 + kk * 16 + 4 * q));
+                        for (int b = 0; b < 4; ++b) {
+                            x[b] = make_uint4(0, 0, 0, 0);
+                            if (8 * u + g < n_rows) x[b] = ld_shared_v4(xb + (8 * u + g) * C::kXStride + 2 * (i * 128 + b * 32 + 8 * q));
+                        }
+                        auto convert = [](uint32_t lo, uint32_t hi, uint32_t (&a)[4]) {
+                            a[0] = f16x2_of_e4m3x2((uint16_t)lo);
+                            a[1] = f16x2_of_e4m3x2((uint16_t)hi);
+                            a[2] = f16x2_of_e4m3x2((uint16_t)(lo >> 16));
+                            a[3] = f16x2_of_e4m3x2((uint16_t)(hi >> 16));
+                        };
 #pragma unroll
-                        for (int kk = 0; kk < 8; ++kk) {
-                            const uint32_t a[4] = {f16x2_of_e4m3x2((uint16_t)l[kk]), f16x2_of_e4m3x2((uint16_t)h[kk]),
-                                                   f16x2_of_e4m3x2((uint16_t)(l[kk] >> 16)), f16x2_of_e4m3x2((uint16_t)(h[kk] >> 16))};
-                            mma_f16(kk & 1 ? odd : part, a, x[kk].x, x[kk].y);
+                        for (int b = 0; b < 4; ++b) {
+                            uint32_t a[4];
+#pragma unroll
+                            for (int t = 0; t < 2; ++t) {
+                                convert(l[t][b].x, h[t][b].x, a);
+                                mma_f16(part[t], a, x[b].x, x[b].y);
+                            }
+#pragma unroll
+                            for (int t = 0; t < 2; ++t) {
+                                convert(l[t][b].y, h[t][b].y, a);
+                                mma_f16(part[t], a, x[b].z, x[b].w);
+                            }
                         }
 #pragma unroll
-                        for (int v = 0; v < 4; ++v) acc[u][v] = fmaf(sc, part[v] + odd[v], acc[u][v]);
+                        for (int t = 0; t < 2; ++t)
+#pragma unroll
+                            for (int v = 0; v < 4; ++v) acc[2 * u + t][v] = fmaf(sc, part[t][v], acc[2 * u + t][v]);
                     }
-                };
-                ok = ok && next_stage();
-                if (ok) {
-                    load(lo[0], hi[0]);
-                    give_back();
                 }
-                for (int i = 0; i < n_stages && ok; i += 2) {
-                    if (i + 1 < n_stages) {
-                        ok = next_stage();
-                        if (!ok) break;
-                        load(lo[1], hi[1]);
-                        give_back();
+                s += n_stages;
+                if (s >= (uint32_t)STAGES) {
+                    s -= STAGES;
+                    ph ^= 1;
+                }
+                // the second group's sums join the first's
+                const uint32_t mine = red_base + (w & 3) * (2 * NG * 4 * 128) + lane * 4;
+                if (group == 1) {
+                    ok = ok && __all_sync(0xffffffffu, mbar_wait(merge_free_bar(w & 3), (n & 1) ^ 1, p.status, kErrMmaWaitFull, p.launch_tag));
+                    if (ok) {
+#pragma unroll
+                        for (int i = 0; i < 2 * NG; ++i)
+#pragma unroll
+                            for (int v = 0; v < 4; ++v) st_shared_f32(mine + (4 * i + v) * 128, acc[i][v]);
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(merge_bar(w & 3));
                     }
-                    multiply(i, lo[0], hi[0]);
-                    if (i + 1 >= n_stages) break;
-                    if (i + 2 < n_stages) {
-                        ok = next_stage();
-                        if (!ok) break;
-                        load(lo[0], hi[0]);
-                        give_back();
+                } else {
+                    ok = ok && __all_sync(0xffffffffu, mbar_wait(merge_bar(w & 3), n & 1, p.status, kErrMmaWaitFull, p.launch_tag));
+                    if (ok) {
+#pragma unroll
+                        for (int i = 0; i < 2 * NG; ++i)
+#pragma unroll
+                            for (int v = 0; v < 4; ++v) acc[i][v] += __uint_as_float(ld_shared_u32(mine + (4 * i + v) * 128));
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(merge_free_bar(w & 3));
                     }
-                    multiply(i + 1, lo[1], hi[1]);
                 }
             } else {
                 // rows are k; transposed 8 x 8 pieces give the weights as [column][k] fragments
@@ -743,16 +827,26 @@ moe_few_kernel(const MoeFewParams p) {
                             if (u < groups) mma_f16(acc[u], a[kk], x[kk >> 1][u][2 * (kk & 1)], x[kk >> 1][u][2 * (kk & 1) + 1]);
                 }
             }
-            if (ok) {
+            if (ok && (!FP8 || w < 4)) {
                 const size_t stride = it.x == kFirst ? 2 * (size_t)p.width : (size_t)p.d;
-                unsigned long long* dst = (it.x == kFirst ? p.part1 : p.part2) + ((size_t)it.w * rows + first) * stride + it.z * 128 + w * 16;
-                const bool inside = it.x == kFirst || it.z * 128 + w * 16 < p.d;
+                const int col0 = it.z * 128 + (FP8 ? (w & 3) * 32 : w * 16);
+                unsigned long long* dst = (it.x == kFirst ? p.part1 : p.part2) + ((size_t)it.w * rows + first) * stride + col0;
+                const bool inside = it.x == kFirst || col0 < p.d;
 #pragma unroll
                 for (int u = 0; u < NG; ++u)
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) {
-                        const int r = 8 * u + 2 * q + (v & 1);
-                        if (r < n_rows && inside) st_word(dst + r * stride + g + 8 * (v >> 1), __float_as_uint(acc[u][v]), call);
+                    for (int v = 0; v < 2; ++v) {
+                        const int r = 8 * u + 2 * q + v;
+                        if (r >= n_rows || !inside) continue;
+                        if (FP8) {
+#pragma unroll
+                            for (int t = 0; t < 2; ++t)
+                                st_words(dst + r * stride + 16 * t + 2 * g, __float_as_uint(acc[FP8 ? 2 * u + t : 0][v]),
+                                         __float_as_uint(acc[FP8 ? 2 * u + t : 0][v + 2]), call);
+                        } else {
+                            st_word(dst + r * stride + g, __float_as_uint(acc[u][v]), call);
+                            st_word(dst + r * stride + g + 8, __float_as_uint(acc[u][v + 2]), call);
+                        }
                     }
             }
             __syncwarp();
@@ -777,7 +871,7 @@ moe_few_kernel(const MoeFewParams p) {
         if (ok && w == 0 && lane == 0) mbar_arrive(routed_bar);
         // ------------------------------------------------------------------------------ sums of complete tiles
         for (uint32_t j = 0; ok; ++j) {
-            ok = __all_sync(0xffffffffu, mbar_wait(sum_bar(j), (j / SUM_SLOTS) & 1, p.status, kErrEpilogueWait, p.launch_tag));
+            ok = __all_sync(0xffffffffu, idle_wait(sum_bar(j), (j / SUM_SLOTS) & 1, p.status, kErrEpilogueWait, p.launch_tag));
             if (!ok) break;
             const Item it = read_item(sum_base + 16u * (j % SUM_SLOTS));
             __syncwarp();

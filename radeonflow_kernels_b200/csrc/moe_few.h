@@ -40,7 +40,7 @@ inline int moe_few_groups(int t) { return t <= 8 ? 1 : t <= 16 ? 2 : 4; }
 // Largest K chunk whose two operand buffers leave room for the weight stages.
 inline int moe_few_max_chunk(int t) { return t <= 16 ? 1024 : 512; }
 // K of a router unit: whole rounds of the eight MMA warps; longer for many experts, whose sums every CTA has to gather.
-inline int moe_few_router_chunk(int experts) { return experts <= 64 ? 512 : 1024; }
+inline int moe_few_router_chunk(int experts) { return experts <= 64 ? 512 : experts == 128 ? 1024 : 2048; }
 
 cudaError_t moe_few_launch(const MoeFewParams& p, bool fp8, int num_sms, cudaStream_t stream);
 
