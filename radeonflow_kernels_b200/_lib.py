@@ -115,6 +115,12 @@ class _NoHost:
     def fp16_addresses(*args):
         return None
 
+    @staticmethod
+    def grouped(*args):
+        return False
+
+    quantize = swiglu_quantize = quantize_blocks = fp16_addresses
+
 
 def host():
     """The `_host` extension, set up, or its stand-in (with a warning) where it cannot be loaded."""
@@ -128,6 +134,9 @@ def host():
             spec.loader.exec_module(module)
             module.setup(run, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, torch.float8_e4m3fn,
                          torch.float32, torch.bfloat16, torch.float16)
+            L = lib()
+            module.setup_fp8(*[ctypes.cast(fn, ctypes.c_void_p).value for fn in (
+                L.rf_fp8_quantize, L.rf_fp8_swiglu_quantize, L.rf_fp8_quantize_blocks, L.rf_fp8_grouped_gemm)], torch.int32)
         except (ImportError, AttributeError) as e:      # not built for this interpreter; a torch without CUDA
             warnings.warn(f"{HOST_PATH} cannot be used ({e}): calls take longer on the host; `python -m "
                           "radeonflow_kernels_b200.build` builds it", RuntimeWarning, stacklevel=2)

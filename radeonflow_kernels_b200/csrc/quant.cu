@@ -6,7 +6,9 @@
 // 448 is e4m3's largest value; the floor keeps 448 / a finite for blocks of zeros.  A NaN makes its whole block NaN, scale
 // included, and an infinity makes the scale infinite: an overflow stays visible behind the product.
 //
-// All three are one pass over the data, held in registers between the block's maximum and its conversion; HBM bounds them.
+// All three are one pass over the data, held in registers between the block's maximum and its conversion.  HBM bounds them as long as
+// the instructions per element stay few: with two IEEE divisions a lane, 64-bit index arithmetic and a modulo per block,
+// 32768 x 7168 gathered bf16 rows took 146 us and SwiGLU of 32768 x 2048 fp16 81.
 #include "ptx.cuh"
 #include "host_util.h"
 #include "launch.h"
@@ -73,43 +75,73 @@ __device__ __forceinline__ float half_warp_max(float a) {
     return a;
 }
 
+// 448 / a for 2^-100 <= a, within two units in the last place, zero for an infinity: the reciprocal of a scaled value, so that
+// neither it nor the reciprocal leaves the range of normal numbers.
+__device__ __forceinline__ float steps_per_unit(float a) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a * 0x1p-20f));
+    return r * (kE4m3Max * 0x1p-20f);
+}
+// a / 448 rounded to nearest: a quotient corrected by its exact remainder (Markstein), for a divisor whose reciprocal is rounded to
+// nearest.  An infinity stays one.
+__device__ __forceinline__ float over_448(float a) {
+    constexpr float inv = 1.0f / kE4m3Max;
+    const float q = a * inv;
+    return isinf(a) ? a : fmaf(fmaf(-q, kE4m3Max, a), inv, q);
+}
+// g / (1 + exp(-g)).  exp(-g) = 2^t (1 + d ln 2) with t = fl(-g log2 e) and d what its rounding left out.
+__device__ __forceinline__ float silu(float g) {
+    constexpr float log2e = 1.44269504f, ln2 = 0.693147181f;
+    const float t = -g * log2e, d = fmaf(-g, log2e, -t);
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+    // (where t is infinite, or 2^t, d says nothing)
+    if (fabsf(t) < 126.0f) e = fmaf(e, d * ln2, e);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return g * r;
+}
+
 // This lane's eight of a block's 128 values -> its eight bytes, and the block's scale.
 __device__ __forceinline__ uint2 quantize_eight(const float (&x)[8], float* scale) {
     float a = fabsf(x[0]);
 #pragma unroll
     for (int i = 1; i < 8; ++i) a = max_nan(a, fabsf(x[i]));
     a = max_nan(half_warp_max(a), kAmaxFloor);
-    *scale = __fdiv_rn(a, kE4m3Max);
-    const float r = __fdiv_rn(kE4m3Max, a);
+    *scale = over_448(a);
+    const float r = steps_per_unit(a);
     return make_uint2(to_e4m3x4(x[0] * r, x[1] * r, x[2] * r, x[3] * r), to_e4m3x4(x[4] * r, x[5] * r, x[6] * r, x[7] * r));
 }
 
 // ------------------------------------------------------------------------------------------------- rows --
-// 16 lanes per block of 128 columns, kPerHalf blocks in a row per half warp: all their loads are in flight before the first
-// is used.  Row i of the result is row i of x, or row rows[i] mod n_src (as an unsigned number, so that no index leaves x).
+// 16 lanes per block of 128 columns, PER blocks in a row per half warp: all their loads are in flight before the first is used.
+// PER is 4, or 1 where that fills the chip no more than twice over.  Row i of the result is row i of x, or row rows[i] mod n_src
+// (as an unsigned number, so that no index leaves x).
 constexpr int kRowThreads = 256;
-constexpr int kPerHalf = 4;
-constexpr int kBlocksPerCta = kRowThreads / 16 * kPerHalf;
 
-// SWIGLU: x is [gate | up], 2 k columns, and what is quantised is SiLU(gate) * up = gate / (1 + exp(-gate)) * up in fp32.
-template <class T, bool VEC, bool SWIGLU>
+// SWIGLU: x is [gate | up], 2 k columns, and what is quantised is SiLU(gate) * up in fp32.
+template <class T, bool VEC, bool SWIGLU, int PER>
 __global__ void __launch_bounds__(kRowThreads)
-quantize_rows_kernel(const T* x, long long row_stride, const int* rows, int n_src, int m, int kb, uint8_t* q, float* scale) {
+quantize_rows_kernel(const T* x, long long row_stride, const int* rows, uint32_t n_src, uint32_t total, uint32_t kb, uint8_t* q,
+                     float* scale) {
     griddep_launch_dependents();
     griddep_wait();
     const int lane = threadIdx.x & 15;
-    const long long total = (long long)m * kb;
-    const long long first = ((long long)blockIdx.x * (kRowThreads / 16) + (threadIdx.x >> 4)) * kPerHalf;
-    if (first - (threadIdx.x & 16 ? kPerHalf : 0) >= total) return;       // whole warps leave: the shuffles need all lanes
-    int row = (int)(first / kb), col = (int)(first - (long long)row * kb);
-    Eight<T> g[kPerHalf], u[SWIGLU ? kPerHalf : 1];
+    // (total < 2^31, and the last CTA reaches less than 64 beyond it)
+    const uint32_t first = (blockIdx.x * (kRowThreads / 16) + (threadIdx.x >> 4)) * PER;
+    if (first - (threadIdx.x & 16 ? PER : 0) >= total) return;       // whole warps leave: the shuffles need all lanes
+    uint32_t row = first / kb, col = first - row * kb;
+    Eight<T> g[PER], u[SWIGLU ? PER : 1];
 #pragma unroll
-    for (int i = 0; i < kPerHalf; ++i) {
+    for (int i = 0; i < PER; ++i) {
         if (first + i < total) {
-            const long long src = rows != nullptr ? (long long)((uint32_t)ld_global_s32(rows + row) % (uint32_t)n_src) : row;
-            const T* p = x + src * row_stride + col * kBlock + lane * 8;
+            uint32_t src = row;
+            if (rows != nullptr) {
+                src = (uint32_t)ld_global_s32(rows + row);
+                if (src >= n_src) src %= n_src;
+            }
+            const T* p = x + (long long)src * row_stride + col * kBlock + lane * 8;
             g[i].template load<VEC>(p);
-            if (SWIGLU) u[i].template load<VEC>(p + (long long)kb * kBlock);
+            if (SWIGLU) u[i].template load<VEC>(p + (size_t)kb * kBlock);
         }
         if (++col == kb) {
             col = 0;
@@ -117,18 +149,18 @@ quantize_rows_kernel(const T* x, long long row_stride, const int* rows, int n_sr
         }
     }
 #pragma unroll
-    for (int i = 0; i < kPerHalf; ++i) {
+    for (int i = 0; i < PER; ++i) {
         const bool valid = first + i < total;
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             v[j] = valid ? g[i].f(j) : 0.f;
-            if (SWIGLU && valid) v[j] = __fdividef(v[j], 1.0f + expf(-v[j])) * u[i].f(j);
+            if (SWIGLU) v[j] = silu(v[j]) * (valid ? u[i].f(j) : 0.f);
         }
         float s;
         const uint2 o = quantize_eight(v, &s);
         if (valid) {
-            *reinterpret_cast<uint2*>(q + (first + i) * kBlock + lane * 8) = o;
+            *reinterpret_cast<uint2*>(q + (size_t)(first + i) * kBlock + lane * 8) = o;
             if (lane == 0) scale[first + i] = s;
         }
     }
@@ -177,8 +209,8 @@ quantize_blocks_kernel(const T* w, long long stride_e, long long stride_n, long 
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kBlockThreads / 32; ++i) a = max_nan(a, warp_max[i]);
-    const float r = __fdiv_rn(kE4m3Max, a);
-    if (tid == 0) scale[((long long)e * gridDim.y + nb) * kb + blockIdx.x] = __fdiv_rn(a, kE4m3Max);
+    const float r = steps_per_unit(a);
+    if (tid == 0) scale[((long long)e * gridDim.y + nb) * kb + blockIdx.x] = over_448(a);
     if (KMAJOR) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -206,14 +238,14 @@ quantize_blocks_kernel(const T* w, long long stride_e, long long stride_n, long 
     }
 }
 
-template <class T>
+template <class T, int PER>
 cudaError_t launch_rows(bool vec, bool swiglu, const void* x, long long row_stride, const int* rows, int n_src, int m, int k,
                         void* q, float* scale, cudaStream_t stream) {
-    auto kernel = swiglu ? (vec ? quantize_rows_kernel<T, true, true> : quantize_rows_kernel<T, false, true>)
-                         : (vec ? quantize_rows_kernel<T, true, false> : quantize_rows_kernel<T, false, false>);
-    const long long blocks = (long long)m * (k / kBlock);
-    return launch_kernel(kernel, dim3((unsigned)((blocks + kBlocksPerCta - 1) / kBlocksPerCta)), kRowThreads, 0, stream, true,
-                         static_cast<const T*>(x), row_stride, rows, n_src, m, k / kBlock, static_cast<uint8_t*>(q), scale);
+    auto kernel = swiglu ? (vec ? quantize_rows_kernel<T, true, true, PER> : quantize_rows_kernel<T, false, true, PER>)
+                         : (vec ? quantize_rows_kernel<T, true, false, PER> : quantize_rows_kernel<T, false, false, PER>);
+    const uint32_t kb = (uint32_t)(k / kBlock), total = (uint32_t)m * kb, per_cta = kRowThreads / 16 * PER;
+    return launch_kernel(kernel, dim3((total + per_cta - 1) / per_cta), kRowThreads, 0, stream, true, static_cast<const T*>(x),
+                         row_stride, rows, (uint32_t)n_src, total, kb, static_cast<uint8_t*>(q), scale);
 }
 
 template <class T>
@@ -242,9 +274,14 @@ int quantize_rows(bool swiglu, const void* x, int dtype, long long row_stride, c
     if (m == 0) return RF_OK;
     if (!x || !q || !scale) return RF_ERR_NULL_POINTER;
     if (misaligned({q}, 16) || misaligned({scale, rows}, 4) || misaligned({x}, (unsigned)bytes)) return RF_ERR_MISALIGNED;
-    if (!device_state()) return RF_ERR_CUDA;
+    DeviceState* st = device_state();
+    if (!st) return RF_ERR_CUDA;
     const bool vec = rows_aligned(x, row_stride, bytes);
-    auto run = dtype == RF_F16 ? launch_rows<__half> : dtype == RF_BF16 ? launch_rows<__nv_bfloat16> : launch_rows<float>;
+    // 24 x 7168: 1344 blocks on 84 CTAs instead of 21
+    const bool few = (long long)m * (k / kBlock) <= 2LL * st->num_sms * (kRowThreads / 16);
+    auto run = dtype == RF_F16    ? (few ? launch_rows<__half, 1> : launch_rows<__half, 4>)
+               : dtype == RF_BF16 ? (few ? launch_rows<__nv_bfloat16, 1> : launch_rows<__nv_bfloat16, 4>)
+                                  : (few ? launch_rows<float, 1> : launch_rows<float, 4>);
     return run(vec, swiglu, x, row_stride, rows, n_src, m, k, q, scale, reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess
                ? RF_OK : RF_ERR_CUDA;
 }

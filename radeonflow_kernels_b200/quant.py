@@ -43,6 +43,10 @@ def fp8_quantize(x, rows=None, out=None):
     unsigned numbers) row i of the result is x[rows[i]]: the gather of `MoE` token rows costs no pass of its own.
     ``out``: (q, scale) to write to, not overlapping x.
     """
+    if out is None:
+        hot = (_lib._host or _lib.host()).quantize(x, rows)         # (the same checks and call in native code, where nothing is amiss)
+        if hot is not None:
+            return hot
     _check_input("fp8_quantize", "x", x)
     if x.dim() != 2 or x.shape[1] % BLOCK != 0 or x.shape[1] == 0:
         raise ValueError("fp8_quantize: x must be [m, k] with k a multiple of 128")
@@ -68,6 +72,10 @@ def fp8_swiglu_quantize(gate_up, out=None):
 
     Columns are contiguous, rows may lie any distance apart; f % 128 == 0.
     """
+    if out is None:
+        hot = (_lib._host or _lib.host()).swiglu_quantize(gate_up)
+        if hot is not None:
+            return hot
     _check_input("fp8_swiglu_quantize", "gate_up", gate_up)
     if gate_up.dim() != 2 or gate_up.shape[1] % (2 * BLOCK) != 0 or gate_up.shape[1] == 0:
         raise ValueError("fp8_swiglu_quantize: gate_up must be [m, 2f] with f a multiple of 128")
@@ -87,6 +95,10 @@ def fp8_quantize_blocks(w, out=None):
     One of the last two axes is contiguous: a weight held as [k, n] goes in as its transposed view and is turned round on the
     way.  k % 128 == 0; the last block of n may be shorter than 128.
     """
+    if out is None:
+        hot = (_lib._host or _lib.host()).quantize_blocks(w)
+        if hot is not None:
+            return hot
     _check_input("fp8_quantize_blocks", "w", w)
     if w.dim() not in (2, 3) or w.shape[-1] % BLOCK != 0 or w.shape[-1] == 0:
         raise ValueError("fp8_quantize_blocks: w must be [n, k] or [e, n, k] with k a multiple of 128")

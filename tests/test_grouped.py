@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from radeonflow_kernels_b200 import grouped
+from radeonflow_kernels_b200 import _lib, grouped
 
 A = 0x7000000                # aligned for everything; nothing stands behind it
 
@@ -27,6 +27,7 @@ class Meta(torch.Tensor):
 
 
 def test_python(monkeypatch):
+    monkeypatch.setattr(_lib, "_host", _lib._NoHost)                      # the Python code's checks
     monkeypatch.setattr(torch.cuda, "current_device", lambda: None)       # the index of the CPU's device
     t = lambda *s, dtype=torch.float32: torch.zeros(*s, dtype=dtype).as_subclass(Meta)
     f8 = torch.float8_e4m3fn

@@ -4,7 +4,7 @@ import ctypes
 import pytest
 import torch
 
-from radeonflow_kernels_b200 import quant
+from radeonflow_kernels_b200 import _lib, quant
 
 A = 0x7000000                # aligned for everything; nothing stands behind it
 
@@ -46,6 +46,7 @@ class Meta(torch.Tensor):
 
 
 def test_python_shapes(monkeypatch):
+    monkeypatch.setattr(_lib, "_host", _lib._NoHost)                      # the Python code's checks
     monkeypatch.setattr(torch.cuda, "current_device", lambda: None)       # the index of the CPU's device
     cuda = lambda *shape, dtype=torch.float16: torch.zeros(*shape, dtype=dtype).as_subclass(Meta)
     for x, match in ((cuda(4, 100), "multiple of 128"), (cuda(128), "multiple of 128"), (cuda(4, 0), "multiple of 128"),
