@@ -119,8 +119,6 @@ class _NoHost:
     def grouped(*args):
         return False
 
-    quantize = swiglu_quantize = quantize_blocks = fp16_addresses
-
 
 def host():
     """The `_host` extension, set up, or its stand-in (with a warning) where it cannot be loaded."""
@@ -134,15 +132,48 @@ def host():
             spec.loader.exec_module(module)
             module.setup(run, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, torch.float8_e4m3fn,
                          torch.float32, torch.bfloat16, torch.float16)
-            L = lib()
-            module.setup_fp8(*[ctypes.cast(fn, ctypes.c_void_p).value for fn in (
-                L.rf_fp8_quantize, L.rf_fp8_swiglu_quantize, L.rf_fp8_quantize_blocks, L.rf_fp8_grouped_gemm)], torch.int32)
+            module.setup_grouped(ctypes.cast(lib().rf_fp8_grouped_gemm, ctypes.c_void_p).value, torch.int32)
         except (ImportError, AttributeError) as e:      # not built for this interpreter; a torch without CUDA
             warnings.warn(f"{HOST_PATH} cannot be used ({e}): calls take longer on the host; `python -m "
                           "radeonflow_kernels_b200.build` builds it", RuntimeWarning, stacklevel=2)
             module = _NoHost
         _host = module
     return _host
+
+
+# the extension that makes tensors is bound to the installed torch as well
+TENSORS_PATH = os.path.join(PKG_DIR, "_tensors" + sysconfig.get_config_var("EXT_SUFFIX"))
+_tensors = None
+
+
+class _NoTensors:
+    """Stands in where there is no such extension: every call is left to the Python code, which takes 7 us longer."""
+
+    @staticmethod
+    def quantize(*args):
+        return None
+
+    swiglu_quantize = quantize_blocks = quantize
+
+
+def tensors():
+    """The `_tensors` extension, set up, or its stand-in (with a warning) where it cannot be loaded."""
+    global _tensors
+    if _tensors is None:
+        L = lib()
+        try:
+            import torch  # noqa: F401  (its libraries are loaded before the extension asks for them)
+            spec = importlib.util.spec_from_file_location(__name__.rpartition(".")[0] + "._tensors", TENSORS_PATH)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            module.setup(*[ctypes.cast(fn, ctypes.c_void_p).value for fn in (
+                L.rf_fp8_quantize, L.rf_fp8_swiglu_quantize, L.rf_fp8_quantize_blocks)])
+        except ImportError as e:        # not built, or for another interpreter or torch
+            warnings.warn(f"{TENSORS_PATH} cannot be used ({e}): calls take longer on the host; `python -m "
+                          "radeonflow_kernels_b200.build` builds it", RuntimeWarning, stacklevel=2)
+            module = _NoTensors
+        _tensors = module
+    return _tensors
 
 
 def _declare(L: ctypes.CDLL) -> None:

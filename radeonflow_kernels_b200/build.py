@@ -1,4 +1,4 @@
-"""In-tree build of librf_b200.so (sm_100a only) with nvcc, and of the CPython extension _host with the host compiler.
+"""In-tree build of librf_b200.so (sm_100a only) with nvcc, and of the CPython extensions _host and _tensors with the host compiler.
 
     python -m radeonflow_kernels_b200.build [--force] [--verbose]
 
@@ -17,6 +17,8 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "librf_b200.so")
 HOST_SRC = os.path.join(CSRC, "host_path.cpp")
 HOST_PATH = os.path.join(PKG_DIR, "_host" + sysconfig.get_config_var("EXT_SUFFIX"))
+TENSORS_SRC = os.path.join(CSRC, "host_tensors.cpp")
+TENSORS_PATH = os.path.join(PKG_DIR, "_tensors" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -72,17 +74,35 @@ def build_host(force: bool = False) -> str:
     return HOST_PATH
 
 
+def build_tensors(force: bool = False) -> str:
+    """As build_host; it is bound to the torch that is installed, too."""
+    import torch
+    root = os.path.dirname(torch.__file__)
+    built = os.path.getmtime(TENSORS_PATH) if os.path.exists(TENSORS_PATH) else 0.0
+    if not force and built >= max(os.path.getmtime(TENSORS_SRC), os.path.getmtime(os.path.join(root, "version.py"))):
+        return TENSORS_PATH
+    cuda = os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I" + sysconfig.get_paths()["include"],
+           "-isystem", os.path.join(root, "include"), "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           "-isystem", cuda, "-L" + os.path.join(root, "lib"), "-o", TENSORS_PATH, TENSORS_SRC,
+           "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+    _compile(cmd, TENSORS_PATH)
+    return TENSORS_PATH
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Path of the library.  The extension is built too where that is possible; without it the Python code does its work."""
+    """Path of the library.  The extensions are built too where that is possible; without them the Python code does their work."""
     if force or _stale():
         cmd = [_nvcc()] + NVCC_FLAGS
         if verbose:
             cmd += ["-Xptxas", "-v"]
         _compile(cmd + ["-o", LIB_PATH] + sources() + ["-lcudart"], LIB_PATH, verbose)
-    try:
-        build_host(force)
-    except (RuntimeError, OSError) as e:        # no host compiler, or no Python headers
-        sys.stderr.write(f"{e}: the Python boundary runs without its extension\n")
+    for extension in (build_host, build_tensors):
+        try:
+            extension(force)
+        except (RuntimeError, OSError, ImportError) as e:       # no host compiler, no Python headers, no torch or one without CUDA
+            sys.stderr.write(f"{e}: the Python boundary runs without its extension\n")
     return LIB_PATH
 
 

@@ -6,8 +6,8 @@
 // hot path wants it, calls the library: 4.2 to 5.4 us, of which the launch is 2.  Where anything is not, it answers "not
 // here", and the Python code that it stands in front of runs as ever, with its errors.  (It includes no torch header: it
 // reads tensors through their Python attributes.)  The addresses of a MoE layer's expert weights are gathered the same way:
-// 64 experts, 96 us of host time for a layer, now 70.  So are the FP8 quantisations, whose kernels take 2 to 3 us for a decode
-// batch, their two results included (24 x 7168: 12.3 us of host time in Python), and the grouped product.
+// 64 experts, 96 us of host time for a layer, now 70.  So is the call of the grouped product.  (The quantisations, which make
+// tensors, have host_tensors.cpp.)
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -18,20 +18,14 @@ namespace {
 
 using RunFn = void (*)(void*, void*, void*, void*, void*, int, int, int, void*, void*);
 
-using RowsFn = int (*)(const void*, int, long long, const int*, int, int, int, void*, float*, void*);
-using SwigluFn = int (*)(const void*, int, long long, int, int, void*, float*, void*);
-using BlocksFn = int (*)(const void*, int, int, int, int, long long, long long, long long, void*, float*, void*);
 using GroupedFn = int (*)(const void*, const void*, const float*, const float*, const int*, void*, int, int, int, int, int, void*);
 
 RunFn g_run = nullptr;
-RowsFn g_rows = nullptr;
-SwigluFn g_swiglu = nullptr;
-BlocksFn g_blocks = nullptr;
 GroupedFn g_grouped = nullptr;
 PyObject *g_get_device = nullptr, *g_get_stream = nullptr;
 PyObject *g_fp8 = nullptr, *g_f32 = nullptr, *g_bf16 = nullptr, *g_f16 = nullptr;
 PyObject* g_i32 = nullptr;
-PyObject *s_is_cuda, *s_is_contiguous, *s_dtype, *s_shape, *s_data_ptr, *s_stride, *s_get_device, *s_new_empty, *s_kw_dtype;
+PyObject *s_is_cuda, *s_is_contiguous, *s_dtype, *s_shape, *s_data_ptr, *s_get_device;
 
 // 1 / 0 = the attribute is (is not) `want`; -1 = an exception is set
 int attr_is(PyObject* o, PyObject* name, PyObject* want) {
@@ -153,21 +147,17 @@ PyObject* fp16_addresses(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(out.data()), count * (Py_ssize_t)sizeof(uint64_t));
 }
 
-// setup_fp8(addresses of rf_fp8_quantize, rf_fp8_swiglu_quantize, rf_fp8_quantize_blocks, rf_fp8_grouped_gemm; int32)
-PyObject* setup_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
-    if (n != 5) {
-        PyErr_SetString(PyExc_TypeError, "setup_fp8: five arguments");
+// setup_grouped(address of rf_fp8_grouped_gemm, int32)
+PyObject* setup_grouped(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != 2) {
+        PyErr_SetString(PyExc_TypeError, "setup_grouped: two arguments");
         return nullptr;
     }
-    uintptr_t fn[4];
-    for (int i = 0; i < 4; ++i) fn[i] = static_cast<uintptr_t>(PyLong_AsUnsignedLongLong(args[i]));
+    const unsigned long long fn = PyLong_AsUnsignedLongLong(args[0]);
     if (PyErr_Occurred()) return nullptr;
-    g_rows = reinterpret_cast<RowsFn>(fn[0]);
-    g_swiglu = reinterpret_cast<SwigluFn>(fn[1]);
-    g_blocks = reinterpret_cast<BlocksFn>(fn[2]);
-    g_grouped = reinterpret_cast<GroupedFn>(fn[3]);
-    Py_INCREF(args[4]);
-    Py_XSETREF(g_i32, args[4]);
+    g_grouped = reinterpret_cast<GroupedFn>(static_cast<uintptr_t>(fn));
+    Py_INCREF(args[1]);
+    Py_XSETREF(g_i32, args[1]);
     Py_RETURN_NONE;
 }
 
@@ -205,136 +195,7 @@ int on_device(PyObject* o, long long device) {
     return PyErr_Occurred() ? -1 : d == device;
 }
 
-// A matrix to quantise: a CUDA tensor in one of the three types (source), on the current device (here).
-struct Source {
-    int dtype;          // as the library numbers them
-    int dims;
-    long long shape[3], stride[3];
-    long long device;
-    void* stream;
-    uint64_t ptr;
-};
-int source(PyObject* o, Source* s) {
-    int r = attr_is(o, s_is_cuda, Py_True);
-    if (r != 1) return r;
-    PyObject* t = PyObject_GetAttr(o, s_dtype);
-    if (!t) return -1;
-    s->dtype = t == g_f16 ? 0 : t == g_bf16 ? 1 : t == g_f32 ? 2 : -1;
-    Py_DECREF(t);
-    if (s->dtype < 0) return 0;
-    s->dims = numbers(PyObject_GetAttr(o, s_shape), s->shape, 3);
-    if (s->dims <= 0) return s->dims;
-    const int n = numbers(PyObject_CallMethodNoArgs(o, s_stride), s->stride, 3);
-    if (n != s->dims) return n < 0 ? -1 : 0;
-    for (int i = 0; i < n; ++i)
-        if (s->shape[i] > INT32_MAX) return 0;
-    return data_ptr(o, &s->ptr) ? 1 : -1;
-}
-int here(PyObject* o, Source* s) { return device_and_stream(&s->device, &s->stream) ? on_device(o, s->device) : -1; }
-
-// A new tensor on o's device and its address; null: an exception is set
-PyObject* new_tensor(PyObject* o, const long long* shape, int dims, PyObject* dtype, uint64_t* ptr) {
-    PyObject* sizes = PyTuple_New(dims);
-    if (!sizes) return nullptr;
-    for (int i = 0; i < dims; ++i) {
-        PyObject* v = PyLong_FromLongLong(shape[i]);
-        if (!v) {
-            Py_DECREF(sizes);
-            return nullptr;
-        }
-        PyTuple_SET_ITEM(sizes, i, v);
-    }
-    PyObject* call[3] = {o, sizes, dtype};
-    PyObject* t = PyObject_VectorcallMethod(s_new_empty, call, 2, s_kw_dtype);
-    Py_DECREF(sizes);
-    if (t && !data_ptr(t, ptr)) Py_CLEAR(t);
-    return t;
-}
-
 inline void* at(uint64_t v) { return reinterpret_cast<void*>(static_cast<uintptr_t>(v)); }
-
-// Both results of a quantisation, `launch(q, scale)` between their making and their return; None: the library refused.
-template <class Launch>
-PyObject* results(PyObject* o, const long long* q_shape, const long long* s_shape, int dims, Launch launch) {
-    uint64_t q, s;
-    PyObject* tq = new_tensor(o, q_shape, dims, g_fp8, &q);
-    PyObject* ts = tq ? new_tensor(o, s_shape, dims, g_f32, &s) : nullptr;
-    PyObject* out = nullptr;
-    if (ts) {
-        int st;
-        Py_BEGIN_ALLOW_THREADS
-        st = launch(at(q), static_cast<float*>(at(s)));
-        Py_END_ALLOW_THREADS
-        out = st == 0 ? PyTuple_Pack(2, tq, ts) : Py_NewRef(Py_None);
-    }
-    Py_XDECREF(tq);
-    Py_XDECREF(ts);
-    return out;
-}
-
-// quantize(x, rows or None) -> (q, scale); None: not the hot form, nothing done
-PyObject* quantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
-    if (n != 2 || !g_rows) Py_RETURN_NONE;
-    Source x;
-    int r = source(args[0], &x);
-    if (r < 0) return nullptr;
-    if (r == 0 || x.dims != 2 || x.shape[1] % 128 != 0 || x.shape[1] == 0 || x.stride[1] != 1) Py_RETURN_NONE;
-    if ((r = here(args[0], &x)) < 0) return nullptr;
-    if (r == 0) Py_RETURN_NONE;
-    long long m = x.shape[0];
-    uint64_t rows = 0;
-    if (args[1] != Py_None) {
-        long long len[3];
-        r = hot_tensor(args[1], g_i32);
-        if (r == 1) r = numbers(PyObject_GetAttr(args[1], s_shape), len, 3) == 1 ? 1 : PyErr_Occurred() ? -1 : 0;
-        if (r == 1) r = on_device(args[1], x.device);
-        if (r == 1 && !data_ptr(args[1], &rows)) r = -1;
-        if (r < 0) return nullptr;
-        m = len[0];
-        if (r == 0 || x.shape[0] == 0 || m > INT32_MAX) Py_RETURN_NONE;
-    }
-    const long long q[2] = {m, x.shape[1]}, s[2] = {m, x.shape[1] / 128};
-    return results(args[0], q, s, 2, [&](void* tq, float* ts) {
-        return g_rows(at(x.ptr), x.dtype, x.stride[0], static_cast<const int*>(at(rows)), (int)x.shape[0], (int)m, (int)x.shape[1], tq, ts,
-                      x.stream);
-    });
-}
-
-// swiglu_quantize(gate_up) -> (q, scale) or None
-PyObject* swiglu_quantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
-    if (n != 1 || !g_swiglu) Py_RETURN_NONE;
-    Source x;
-    int r = source(args[0], &x);
-    if (r < 0) return nullptr;
-    if (r == 0 || x.dims != 2 || x.shape[1] % 256 != 0 || x.shape[1] == 0 || x.stride[1] != 1) Py_RETURN_NONE;
-    if ((r = here(args[0], &x)) < 0) return nullptr;
-    if (r == 0) Py_RETURN_NONE;
-    const long long f = x.shape[1] / 2, q[2] = {x.shape[0], f}, s[2] = {x.shape[0], f / 128};
-    return results(args[0], q, s, 2, [&](void* tq, float* ts) {
-        return g_swiglu(at(x.ptr), x.dtype, x.stride[0], (int)x.shape[0], (int)f, tq, ts, x.stream);
-    });
-}
-
-// quantize_blocks(w) -> (q, scale) or None
-PyObject* quantize_blocks(PyObject*, PyObject* const* args, Py_ssize_t n) {
-    if (n != 1 || !g_blocks) Py_RETURN_NONE;
-    Source w;
-    int r = source(args[0], &w);
-    if (r < 0) return nullptr;
-    if (r == 0 || w.dims < 2) Py_RETURN_NONE;
-    const int d = w.dims;
-    const long long rows = w.shape[d - 2], k = w.shape[d - 1];
-    if (k % 128 != 0 || k == 0 || (w.stride[d - 1] != 1 && w.stride[d - 2] != 1)) Py_RETURN_NONE;
-    if ((r = here(args[0], &w)) < 0) return nullptr;
-    if (r == 0) Py_RETURN_NONE;
-    long long s[3] = {w.shape[0], 0, 0};
-    s[d - 2] = (rows + 127) / 128;
-    s[d - 1] = k / 128;
-    return results(args[0], w.shape, s, d, [&](void* tq, float* ts) {
-        return g_blocks(at(w.ptr), w.dtype, d == 3 ? (int)w.shape[0] : 1, (int)rows, (int)k, d == 3 ? w.stride[0] : 0, w.stride[d - 2],
-                        w.stride[d - 1], tq, ts, w.stream);
-    });
-}
 
 // grouped(a, b, a_scale, b_scale, offsets, c) -> True: launched; False: not the hot form, or refused
 PyObject* grouped(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -383,10 +244,7 @@ PyCFunction fast(F f) { return reinterpret_cast<PyCFunction>(reinterpret_cast<vo
 PyMethodDef methods[] = {{"setup", fast(setup), METH_FASTCALL, nullptr},
                          {"gemm", fast(gemm), METH_FASTCALL, nullptr},
                          {"fp16_addresses", fast(fp16_addresses), METH_FASTCALL, nullptr},
-                         {"setup_fp8", fast(setup_fp8), METH_FASTCALL, nullptr},
-                         {"quantize", fast(quantize), METH_FASTCALL, nullptr},
-                         {"swiglu_quantize", fast(swiglu_quantize), METH_FASTCALL, nullptr},
-                         {"quantize_blocks", fast(quantize_blocks), METH_FASTCALL, nullptr},
+                         {"setup_grouped", fast(setup_grouped), METH_FASTCALL, nullptr},
                          {"grouped", fast(grouped), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
@@ -399,11 +257,7 @@ PyMODINIT_FUNC PyInit__host(void) {
     s_dtype = PyUnicode_InternFromString("dtype");
     s_shape = PyUnicode_InternFromString("shape");
     s_data_ptr = PyUnicode_InternFromString("data_ptr");
-    s_stride = PyUnicode_InternFromString("stride");
     s_get_device = PyUnicode_InternFromString("get_device");
-    s_new_empty = PyUnicode_InternFromString("new_empty");
-    s_kw_dtype = s_dtype ? PyTuple_Pack(1, s_dtype) : nullptr;
-    if (!s_is_cuda || !s_is_contiguous || !s_dtype || !s_shape || !s_data_ptr || !s_stride || !s_get_device || !s_new_empty || !s_kw_dtype)
-        return nullptr;
+    if (!s_is_cuda || !s_is_contiguous || !s_dtype || !s_shape || !s_data_ptr || !s_get_device) return nullptr;
     return PyModule_Create(&module);
 }

@@ -44,7 +44,7 @@ def fp8_quantize(x, rows=None, out=None):
     ``out``: (q, scale) to write to, not overlapping x.
     """
     if out is None:
-        hot = (_lib._host or _lib.host()).quantize(x, rows)         # (the same checks and call in native code, where nothing is amiss)
+        hot = (_lib._tensors or _lib.tensors()).quantize(x, rows)         # (the same checks and call in native code, where nothing is amiss)
         if hot is not None:
             return hot
     _check_input("fp8_quantize", "x", x)
@@ -73,7 +73,7 @@ def fp8_swiglu_quantize(gate_up, out=None):
     Columns are contiguous, rows may lie any distance apart; f % 128 == 0.
     """
     if out is None:
-        hot = (_lib._host or _lib.host()).swiglu_quantize(gate_up)
+        hot = (_lib._tensors or _lib.tensors()).swiglu_quantize(gate_up)
         if hot is not None:
             return hot
     _check_input("fp8_swiglu_quantize", "gate_up", gate_up)
@@ -96,7 +96,7 @@ def fp8_quantize_blocks(w, out=None):
     way.  k % 128 == 0; the last block of n may be shorter than 128.
     """
     if out is None:
-        hot = (_lib._host or _lib.host()).quantize_blocks(w)
+        hot = (_lib._tensors or _lib.tensors()).quantize_blocks(w)
         if hot is not None:
             return hot
     _check_input("fp8_quantize_blocks", "w", w)

@@ -4,7 +4,7 @@ import ctypes
 import pytest
 import torch
 
-from radeonflow_kernels_b200 import _lib, quant
+from radeonflow_kernels_b200 import _lib, build, quant
 
 A = 0x7000000                # aligned for everything; nothing stands behind it
 
@@ -46,7 +46,7 @@ class Meta(torch.Tensor):
 
 
 def test_python_shapes(monkeypatch):
-    monkeypatch.setattr(_lib, "_host", _lib._NoHost)                      # the Python code's checks
+    monkeypatch.setattr(_lib, "_tensors", _lib._NoTensors)                    # the Python code's checks
     monkeypatch.setattr(torch.cuda, "current_device", lambda: None)       # the index of the CPU's device
     cuda = lambda *shape, dtype=torch.float16: torch.zeros(*shape, dtype=dtype).as_subclass(Meta)
     for x, match in ((cuda(4, 100), "multiple of 128"), (cuda(128), "multiple of 128"), (cuda(4, 0), "multiple of 128"),
@@ -64,3 +64,33 @@ def test_python_shapes(monkeypatch):
         quant.fp8_quantize(cuda(0, 128), rows=torch.zeros(3, dtype=torch.int32))
     with pytest.raises(ValueError, match="out's q"):
         quant.fp8_quantize(cuda(4, 128), out=(torch.zeros(4, 128), torch.zeros(4, 1)))
+
+
+def test_the_extension_leaves_what_is_amiss_to_the_python_code(rf_lib):
+    t = _lib.tensors()
+    assert t is not _lib._NoTensors and t.__file__ == _lib.TENSORS_PATH
+    for x in (1, None, torch.zeros(4, 128), torch.zeros(4, 128, dtype=torch.float64), cls_like()):
+        assert t.quantize(x, None) is None and t.swiglu_quantize(x) is None and t.quantize_blocks(x) is None
+    assert t.quantize(torch.zeros(4, 128)) is None and t.swiglu_quantize() is None
+    with pytest.raises(TypeError):
+        t.setup(1)
+
+
+def cls_like():
+    return torch.zeros(4, 128).as_subclass(Meta)
+
+
+def test_without_the_extension(rf_lib, monkeypatch, tmp_path):
+    monkeypatch.setattr(_lib, "_tensors", None)
+    monkeypatch.setattr(_lib, "TENSORS_PATH", str(tmp_path / "_tensors.so"))
+    with pytest.warns(RuntimeWarning, match="cannot be used"):
+        assert _lib.tensors() is _lib._NoTensors
+    with pytest.raises(ValueError, match="CUDA"):
+        quant.fp8_quantize(torch.zeros(4, 128))
+
+
+def test_the_library_is_built_where_the_extension_cannot_be(rf_lib, monkeypatch, capsys):
+    assert build.TENSORS_PATH == _lib.TENSORS_PATH and build.build_tensors() == build.TENSORS_PATH
+    monkeypatch.setenv("CXX", "false")
+    monkeypatch.setattr(build, "TENSORS_PATH", build.TENSORS_PATH + ".other")
+    assert build.build() == build.LIB_PATH and "without its extension" in capsys.readouterr().err

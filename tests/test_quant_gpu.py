@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 import torch
 
-from radeonflow_kernels_b200 import gemm, quant
+from radeonflow_kernels_b200 import _lib, gemm, quant
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -188,3 +188,38 @@ def test_operands_of_the_gemm():
     ref = da @ db.T
     # bf16 rounding 2^-8 of the value; the fp32 sum over k blocks and the tensor cores' sums inside one: 2^-12 of the terms
     assert (np.abs(c.double().cpu().numpy() - ref) <= 2.0 ** -8 * np.abs(ref) + 2.0 ** -12 * (np.abs(da) @ np.abs(db).T)).all()
+
+
+def test_without_the_extension_the_same_bits(monkeypatch):
+    x = torch.randn(33, 640, device=DEV).bfloat16()
+    rows = torch.tensor([3, 3, 32, 0], device=DEV, dtype=torch.int32)
+    w = torch.randn(3, 256, 200, device=DEV).half().transpose(1, 2)
+    calls = (lambda: quant.fp8_quantize(x), lambda: quant.fp8_quantize(x[:, 128:384], rows=rows), lambda: quant.fp8_quantize_blocks(w),
+             lambda: quant.fp8_quantize_blocks(w[1]), lambda: quant.fp8_swiglu_quantize(x[:, :512]), lambda: quant.fp8_quantize(x[:0]))
+    assert _lib.tensors() is not _lib._NoTensors
+    native = [f() for f in calls]
+    monkeypatch.setattr(_lib, "_tensors", _lib._NoTensors)
+    for f, (q, s) in zip(calls, native):
+        q1, s1 = f()
+        assert q.dtype == q1.dtype and q.shape == q1.shape and s.shape == s1.shape and q.is_contiguous()
+        assert torch.equal(q.view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s, s1)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_refusals_on_the_gpu(native, monkeypatch):
+    if not native:
+        monkeypatch.setattr(_lib, "_tensors", _lib._NoTensors)
+    x = torch.zeros(4, 256, device=DEV)
+    for bad, match in ((x[:, :100], "multiple of 128"), (x[0], "multiple of 128"), (x.t(), "multiple of 128"), (x.double(), "float16"),
+                       (x.cpu(), "CUDA"), (torch.zeros(256, 256, device=DEV)[:, ::2], "contiguous")):
+        with pytest.raises(ValueError, match=match):
+            quant.fp8_quantize(bad)
+    for rows in (torch.zeros(3, device=DEV), torch.zeros(3, dtype=torch.int32), torch.zeros(6, device=DEV, dtype=torch.int32)[::2]):
+        with pytest.raises(ValueError, match="rows"):
+            quant.fp8_quantize(x, rows=rows)
+    with pytest.raises(ValueError, match="no rows"):
+        quant.fp8_quantize(x[:0], rows=torch.zeros(3, device=DEV, dtype=torch.int32))
+    with pytest.raises(ValueError, match="multiple of 128"):
+        quant.fp8_swiglu_quantize(x[:, :128])
+    with pytest.raises(ValueError, match="contiguous"):
+        quant.fp8_quantize_blocks(torch.zeros(2, 256, 512, device=DEV)[:, ::2, ::2])
