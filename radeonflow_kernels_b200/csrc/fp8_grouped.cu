@@ -1,10 +1,15 @@
-// Grouped FP8 block-scaled product for groups of many rows, on CTA pairs, sm_100a; and the C-ABI entry.
+// Grouped FP8 block-scaled product for groups of many rows, sm_100a; and the C-ABI entry.
 //
-// The formula is that of fp8_grouped_few.cu.  Here a tile is 256 rows of a group x 256 columns, shared out over a 2-CTA cluster
-// as in fp8_gemm_pair.cu: each CTA loads its 128 rows of a and half of the weight rows; the columns are two halves of 128 =
-// one scale block, whose MMAs alternate, each with accumulator buffers and four epilogue warps per CTA of its own; two
-// warps multiply the scales ahead.  What differs is where a tile lies and how it leaves: row ranges come from the device, and a
-// warp's 32 rows x 64 columns go out by TMA where they are all of the group, else row by row up to the group's end.
+// The formula is that of fp8_grouped_few.cu.  Here a tile is 128 rows of a group x 256 columns.  As in fp8_gemm_pair.cu the columns are
+// two halves of 128 = one scale block, whose MMAs alternate, each with accumulator buffers and four epilogue warps of its own:
+// one half's epilogue works while the other's waits for its next K block; two warps multiply the scales ahead.  What differs is
+// where a tile lies and how it leaves: row ranges come from the device, and a warp's 32 rows x 64 columns go out by TMA where they
+// are all of the group, else row by row up to the group's end.
+//
+// What bounds it: as the plain product the power cap and the epilogue's K block, and here the rows that tiles hold beyond their
+// groups' ends, half a tile a group.  32768 rows, n 4096, k 7168: one group 0.89 ms (the plain product's CTA pairs 0.81 to 0.90 on
+// that box), 32 uneven groups, which need a ninth tile every other time, 0.96 to 1.15 between runs.  The same on CTA pairs with
+// 256 x 256 tiles: 1.01 to 1.19; 8192 rows in 32 groups 368 us, here 331; they win in one group only, 870 / 887.
 #include "fp8_grouped.cuh"
 #include "host_util.h"
 #include "launch.h"
@@ -25,17 +30,20 @@ constexpr int NB = 512 / BN;     // accumulator buffers of each half
 constexpr int NUM_NON_EPI_WARPS = 4;
 constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 32 * (NUM_NON_EPI_WARPS + EPI_WARPS);
-constexpr int kRegsLo = 88, kRegsHi = 208;      // 128 * lo + 256 * hi is what the CTA was launched with (168 each)
+// 128 * lo + 256 * hi is at most what the CTA was launched with (168 each).  TMEM is read 16 columns at a time: with 32, as in the
+// plain product, the K loop spills (CTA pairs, 32768 x 4096 x 7168 in 32 groups: 1.40 ms, so 1.04 to 1.11).
+constexpr int kRegsLo = 112, kRegsHi = 192;
 static_assert(128 * kRegsLo + 256 * kRegsHi <= 64512, "register split");
 
 constexpr int A_BYTES = BM * BK;
-constexpr int B_HALF_BYTES = HN / 2 * BK;
-constexpr int STAGE_BYTES = A_BYTES + 2 * B_HALF_BYTES;
-constexpr int STAGES = 4;
 constexpr int CHUNKS = HN / 64;
 constexpr int SLAB_BYTES = 32 * 128;
 constexpr int SCALE_BYTES = 2 * NB * BM * 4;
-constexpr int BAR_BYTES = (2 * STAGES + 6 * NB) * 8 + 16;
+
+constexpr int B_HALF_BYTES = HN * BK;
+constexpr int STAGE_BYTES = A_BYTES + 2 * B_HALF_BYTES;
+constexpr int STAGES = 3;
+constexpr int BAR_BYTES = (2 * STAGES + 4 * NB) * 8 + 16;
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * CHUNKS * SLAB_BYTES + SCALE_BYTES + BAR_BYTES +
                            (int)sizeof(GroupTable) + 1024;
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
@@ -48,28 +56,26 @@ __device__ __forceinline__ void fma_f32x2(F32x2& acc, float x, float y, float s)
     acc = (F32x2)__float_as_uint(r.x) | ((F32x2)__float_as_uint(r.y) << 32);
 }
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
-fp8_grouped_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
+__global__ void __launch_bounds__(THREADS, 1)
+fp8_grouped_many_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
                         const __grid_constant__ CUtensorMap tma_c, const GroupedParams p) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t slab_base = smem_base + STAGES * STAGE_BYTES;
     const uint32_t scale_base = slab_base + EPI_WARPS * CHUNKS * SLAB_BYTES;
     const uint32_t bar_base = scale_base + SCALE_BYTES;
-    auto full_bar = [&](uint32_t s) { return bar_base + 8u * s; };                // leader's: bytes of both CTAs
+    auto full_bar = [&](uint32_t s) { return bar_base + 8u * s; };
     auto empty_bar = [&](uint32_t s) { return bar_base + 8u * (STAGES + s); };
     auto tmem_full_bar = [&](uint32_t b) { return bar_base + 8u * (2 * STAGES + b); };           // b = half * NB + i
-    auto tmem_empty_bar = [&](uint32_t b) { return bar_base + 8u * (2 * STAGES + 2 * NB + b); };  // leader's: both CTAs
-    auto scale_empty_bar = [&](uint32_t b) { return bar_base + 8u * (2 * STAGES + 4 * NB + b); };
-    const uint32_t tmem_slot = bar_base + 8u * (2 * STAGES + 6 * NB);
+    auto tmem_empty_bar = [&](uint32_t b) { return bar_base + 8u * (2 * STAGES + 2 * NB + b); };
+    const uint32_t tmem_slot = bar_base + 8u * (2 * STAGES + 4 * NB);
     GroupTable& table = *reinterpret_cast<GroupTable*>(smem_raw + (tmem_slot + 16 - smem_u32(smem_raw)));
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     griddep_launch_dependents();
-    const int rank = (int)cluster_ctarank();       // 0 = leader of the pair
-    const int unit = (int)(blockIdx.x >> 1);
-    const int n_units = (int)(gridDim.x >> 1);
+    const int unit = (int)blockIdx.x;
+    const int n_units = (int)gridDim.x;
 
     if (threadIdx.x == 0) {
         tma_prefetch_desc(&tma_a);
@@ -81,20 +87,18 @@ fp8_grouped_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_
         }
         for (int b = 0; b < 2 * NB; ++b) {
             mbar_init(tmem_full_bar(b), 2);                // the MMAs' commit and the scale warp
-            mbar_init(tmem_empty_bar(b), EPI_WARPS);       // four warps of each CTA
-            mbar_init(scale_empty_bar(b), EPI_WARPS / 2);  // the half's four
+            mbar_init(tmem_empty_bar(b), EPI_WARPS / 2);   // the half's four warps
         }
         mbar_fence_init();
     }
     if (warp == 1) {
-        tmem_alloc_2cta(tmem_slot, 512);
-        tmem_relinquish_2cta();
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
     }
     griddep_wait();
-    build_group_table(table, p, 2 * BM);
+    build_group_table(table, p, BM);
     tc_fence_before();
     __syncthreads();
-    cluster_sync_all();      // both CTAs' barriers exist before any remote arrive, byte count or commit
     tc_fence_after();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(smem_raw + (tmem_slot - smem_u32(smem_raw)));
 
@@ -111,29 +115,26 @@ fp8_grouped_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_
                 bool ok = true;
                 for (int w = unit; ok && w < total; w += n_units) {
                     const GroupedTile t = decode_grouped(table, p, w, tiles_n);
-                    const int a_row0 = table.lo[t.group] + (t.m_blk * 2 + rank) * BM;
-                    const int b_row0 = t.group * p.n + t.n_blk * BN + rank * (HN / 2);
+                    const int a_row0 = table.lo[t.group] + t.m_blk * BM;
+                    const int b_row0 = t.group * p.n + t.n_blk * BN;
                     int x = 0;
                     for (const uint32_t end = it + kb_total; it != end; ++it, x += BK) {
                         ok = mbar_wait(empty_bar(s), ph, p.status, kErrProducerWait, p.launch_tag);
                         if (!ok) break;
                         const uint32_t sa = smem_base + s * STAGE_BYTES;
-                        const uint32_t bar = mapa_cluster(full_bar(s), 0);
-                        if (rank == 0) mbar_expect_tx(full_bar(s), 2 * STAGE_BYTES);
-                        tma_load_2d_pair(sa, &tma_a, bar, x, a_row0);
-                        tma_load_2d_pair(sa + A_BYTES, &tma_b, bar, x, b_row0);
-                        tma_load_2d_pair(sa + A_BYTES + B_HALF_BYTES, &tma_b, bar, x, b_row0 + HN);
+                        mbar_expect_tx(full_bar(s), STAGE_BYTES);
+                        tma_load_2d(sa, &tma_a, full_bar(s), x, a_row0);
+                        tma_load_2d(sa + A_BYTES, &tma_b, full_bar(s), x, b_row0);       // both halves' rows
                         if (++s == STAGES) { s = 0; ph ^= 1; }
                     }
                 }
-                // (the leader's commits arrive on this CTA's stage barriers)
                 finish_producer(ok, it, STAGES, empty_bar(0), p.status, kErrProducerWait, p.launch_tag);
             }
             __syncwarp();
         } else if (warp == 1) {
-            if (rank == 0 && elect_one()) {
+            if (elect_one()) {
                 // ---------------------------------------------------- MMA issuer
-                constexpr uint32_t idesc = make_idesc(2 * BM, HN, /*e4m3*/ 0, /*e4m3*/ 0, 0, 0);
+                constexpr uint32_t idesc = make_idesc(BM, HN, /*e4m3*/ 0, /*e4m3*/ 0, 0, 0);
                 const uint64_t desc0 = smem_desc_kmajor_sw128(smem_base);
                 uint32_t it = 0, s = 0, ph = 0;
                 bool ok = true;
@@ -156,12 +157,12 @@ fp8_grouped_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_
                             if (h == 0 || both) {
 #pragma unroll
                                 for (int j = 0; j < BK / UMMA_K; ++j)
-                                    umma_f8_2cta(d + h * (NB * HN), adesc + 2 * j, bdesc + 2 * j, idesc, j > 0 ? 1u : 0u);
+                                    umma_f8(d + h * (NB * HN), adesc + 2 * j, bdesc + 2 * j, idesc, j > 0 ? 1u : 0u);
                             }
-                            umma_commit_2cta_multicast(tmem_full_bar(h * NB + buf), 0x3);
+                            umma_commit(tmem_full_bar(h * NB + buf));
                         }
                         if (!ok) break;
-                        umma_commit_2cta_multicast(empty_bar(s), 0x3);
+                        umma_commit(empty_bar(s));
                         if (++s == STAGES) { s = 0; ph ^= 1; }
                     }
                 }
@@ -169,7 +170,7 @@ fp8_grouped_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_
             __syncwarp();
         } else {
             // ------------------------------------------------------ scales
-            // One warp per half: the products a_s * b_s of this CTA's 128 rows, one K block at a time, into the slot of the
+            // One warp per half: the products a_s * b_s of the tile's 128 rows, one K block at a time, into the slot of the
             // block's accumulator buffer.  Its loads run PF K blocks ahead, across tiles.  (Rows behind the group's end take
             // the last row's scales: what they are multiplied with is not stored.)
             const int half = warp - 2;
@@ -182,7 +183,7 @@ fp8_grouped_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_
                 if (w >= total) return false;
                 const GroupedTile t = decode_grouped(table, p, w, tiles_n);
                 const int col0 = t.n_blk * BN + half * HN;
-                const int row0 = table.lo[t.group] + (t.m_blk * 2 + rank) * BM + 4 * lane;
+                const int row0 = table.lo[t.group] + t.m_blk * BM + 4 * lane;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) ar[i] = (uint32_t)min(row0 + i, p.m - 1) * (uint32_t)kb_total;
                 br = ((uint32_t)t.group * (uint32_t)((p.n + HN - 1) / HN) + (uint32_t)(col0 < p.n ? col0 / HN : 0)) *
@@ -208,10 +209,10 @@ fp8_grouped_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_
 #pragma unroll
                 for (int d = 0; d < PF; ++d) {
                     if (q >= n_loaded) break;
-                    // (the slot for K block q - NB has been read: an order that the accumulator's hand-back does not give)
+                    // (the epilogue gives accumulator and slot back together)
                     const uint32_t buf = half * NB + q % NB;
                     if (q >= NB) {
-                        ok = __all_sync(0xffffffffu, mbar_wait(scale_empty_bar(buf), (q / NB - 1) & 1, p.status,
+                        ok = __all_sync(0xffffffffu, mbar_wait(tmem_empty_bar(buf), (q / NB - 1) & 1, p.status,
                                                                kErrSchedWait, p.launch_tag));
                         if (!ok) break;
                     }
@@ -246,24 +247,21 @@ fp8_grouped_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_
                 if (!mbar_wait(tmem_full_bar(buf), (it / NB) & 1, p.status, kErrEpilogueWait, p.launch_tag)) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t taddr = lane_addr + (it % NB) * HN;
-                float v[2][32];
-                tmem_ld32_async(taddr, v[0]);
+                float v[2][16];
+                tmem_ld16_async(taddr, v[0]);
                 const float s = __uint_as_float(ld_shared_u32(my_scale + (it % NB) * (BM * 4)));
 #pragma unroll
-                for (int c = 0; c < HN / 32; ++c) {
-                    tmem_ld_fence(v[c % 2]);
-                    if (c + 1 < HN / 32) tmem_ld32_async(taddr + (c + 1) * 32, v[(c + 1) % 2]);
-                    if (c + 1 == HN / 32) {
+                for (int c = 0; c < HN / 16; ++c) {
+                    tmem_ld16_fence(v[c % 2]);
+                    if (c + 1 < HN / 16) tmem_ld16_async(taddr + (c + 1) * 16, v[(c + 1) % 2]);
+                    if (c + 1 == HN / 16) {
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) {
-                            mbar_arrive_cluster_relaxed(mapa_cluster(tmem_empty_bar(buf), 0));
-                            mbar_arrive(scale_empty_bar(buf));
-                        }
+                        if (lane == 0) mbar_arrive(tmem_empty_bar(buf));
                     }
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        fma_f32x2(acc[c * 16 + j], v[c % 2][2 * j], v[c % 2][2 * j + 1], s);
+                    for (int j = 0; j < 8; ++j)
+                        fma_f32x2(acc[c * 8 + j], v[c % 2][2 * j], v[c % 2][2 * j + 1], s);
                 }
             }
             if (!ok) break;
@@ -289,7 +287,7 @@ fp8_grouped_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_
             __syncwarp();
             const GroupedTile t = decode_grouped(table, p, w, tiles_n);
             const int col0 = t.n_blk * BN + half * HN;
-            const int row0 = table.lo[t.group] + (t.m_blk * 2 + rank) * BM + quad * 32;
+            const int row0 = table.lo[t.group] + t.m_blk * BM + quad * 32;
             const int rows = table.hi[t.group] - row0;
             if (rows >= 32) {
                 if (lane == 0) {
@@ -316,27 +314,25 @@ fp8_grouped_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_
 
     tc_fence_before();
     __syncthreads();
-    cluster_sync_all();      // the peer no longer touches this CTA's barriers, shared memory or TMEM
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc_2cta(tmem_base, 512);
+        tmem_dealloc(tmem_base, 512);
     }
 }
 
 }  // namespace
 
-cudaError_t fp8_grouped_pair_launch(const CUtensorMap& tma_a, const CUtensorMap& tma_b, const CUtensorMap& tma_c,
+cudaError_t fp8_grouped_many_launch(const CUtensorMap& tma_a, const CUtensorMap& tma_b, const CUtensorMap& tma_c,
                                     const GroupedParams& p, int num_sms, cudaStream_t stream) {
     static bool attr_set[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 64 && !attr_set[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(fp8_grouped_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+        const cudaError_t e = cudaFuncSetAttribute(fp8_grouped_many_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
         if (e != cudaSuccess) return e;
         attr_set[dev] = true;
     }
-    const unsigned pairs = num_sms >= 2 ? (unsigned)num_sms / 2 : 1;
-    return launch_kernel(fp8_grouped_pair_kernel, dim3(2 * pairs), THREADS, SMEM_BYTES, stream, true, tma_a, tma_b, tma_c, p);
+    return launch_kernel(fp8_grouped_many_kernel, dim3((unsigned)num_sms), THREADS, SMEM_BYTES, stream, true, tma_a, tma_b, tma_c, p);
 }
 
 }  // namespace rf
@@ -367,21 +363,23 @@ int rf_fp8_grouped_gemm(const void* a, const void* b, const float* as, const flo
     p.m = m; p.n = n; p.k = k; p.groups = n_groups;
     p.out_f16 = c_dtype == RF_F16;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    const int mean = m / n_groups;
+    // Few rows a group, or too few tiles of 128 x 256 for the chip, run transposed (us, transposed / not): 1536 rows in 32 groups, n 4096,
+    // k 2048 50 / 56, 2048 rows 55 / 57, 4096 rows of k 7168 278 / 230; 1777 rows in 8 groups, n 576, k 2048 12.8 / 13.6.  The counts
+    // are on the device: the rule goes by the mean.
+    const bool few = m <= 64LL * n_groups || ((long long)m / 128 + n_groups) * ((n + 255) / 256) <= st->num_sms;
     cudaError_t e;
     CUtensorMap ta, tb, tc;
-    if (mean < 128) {
-        const int tile = mean <= 8 ? 16 : mean <= 20 ? 32 : mean <= 48 ? 64 : 128;
+    if (few) {
         if (!rf::encode_tma_2d(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, b, (uint64_t)n_groups * n, (uint64_t)k, (uint64_t)k, 128, 128, true) ||
-            !rf::encode_tma_2d(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a, (uint64_t)m, (uint64_t)k, (uint64_t)k, (uint32_t)tile, 128, true))
+            !rf::encode_tma_2d(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a, (uint64_t)m, (uint64_t)k, (uint64_t)k, rf::kGroupedFewRows, 128, true))
             return RF_ERR_CUDA;
-        e = rf::fp8_grouped_few_launch(tb, ta, p, tile, st->num_sms, s);
+        e = rf::fp8_grouped_few_launch(tb, ta, p, st->num_sms, s);
     } else {
         if (!rf::encode_tma_2d(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a, (uint64_t)m, (uint64_t)k, (uint64_t)k, 128, 128, true) ||
-            !rf::encode_tma_2d(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, b, (uint64_t)n_groups * n, (uint64_t)k, (uint64_t)k, 64, 128, true) ||
+            !rf::encode_tma_2d(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, b, (uint64_t)n_groups * n, (uint64_t)k, (uint64_t)k, 256, 128, true) ||
             !rf::encode_tma_2d(&tc, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, c, (uint64_t)m, (uint64_t)n, (uint64_t)n * 2, 32, 64, true))
             return RF_ERR_CUDA;
-        e = rf::fp8_grouped_pair_launch(ta, tb, tc, p, st->num_sms, s);
+        e = rf::fp8_grouped_many_launch(ta, tb, tc, p, st->num_sms, s);
     }
     if (e != cudaSuccess) {
         fprintf(stderr, "rf_b200: grouped fp8 gemm launch failed: %s\n", cudaGetErrorString(e));

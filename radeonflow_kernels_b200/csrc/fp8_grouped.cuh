@@ -79,9 +79,12 @@ __device__ __forceinline__ GroupedTile decode_grouped(const GroupTable& t, const
     return GroupedTile{lo, first_m + in_band - n_blk * rows, n_blk};
 }
 
-cudaError_t fp8_grouped_few_launch(const CUtensorMap& tma_w, const CUtensorMap& tma_x, const GroupedParams& p, int tile_rows,
-                                   int num_sms, cudaStream_t stream);
-cudaError_t fp8_grouped_pair_launch(const CUtensorMap& tma_a, const CUtensorMap& tma_b, const CUtensorMap& tma_c,
+// tma_w: boxes of 128 weight rows, tma_x: of kGroupedFewRows rows of a
+constexpr int kGroupedFewRows = 64;
+cudaError_t fp8_grouped_few_launch(const CUtensorMap& tma_w, const CUtensorMap& tma_x, const GroupedParams& p, int num_sms,
+                                   cudaStream_t stream);
+// tma_a: boxes of 128 rows of a, tma_b: of 256 weight rows, tma_c: 32 x 64
+cudaError_t fp8_grouped_many_launch(const CUtensorMap& tma_a, const CUtensorMap& tma_b, const CUtensorMap& tma_c,
                                     const GroupedParams& p, int num_sms, cudaStream_t stream);
 
 }  // namespace rf

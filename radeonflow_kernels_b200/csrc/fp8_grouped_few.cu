@@ -2,15 +2,19 @@
 //
 //   c[r, n] = sum_kb a_s[r, kb] b_s[g, n/128, kb] sum_{j < 128} a[r, 128 kb + j] b[g, n, 128 kb + j],   r in group g
 //
-// The product is computed transposed: 128 rows of a group's weight are the MMA's M, the group's rows (up to NT in a tile) its
-// N in steps of 16, so that a dozen rows cost a 16-wide MMA beside the weight stream, which bounds the kernel: every weight
-// byte is read once from HBM and none waits for another.  Scales differ per accumulator column then (one product a_s * b_s
-// per row of a), and a scale warp leaves them in shared memory, from where they are broadcast to the promotion's FMAs.
+// The product is computed transposed: 128 rows of a group's weight are the MMA's M, the group's rows (up to 64 in a tile) its N in
+// steps of 16, so that a dozen rows cost a 16-wide MMA beside the weight stream, which bounds the kernel: 512 rows in 32 groups,
+// n 7168, k 2048 take 79 us, 6.0 TB/s of what cannot be left out.  Scales differ per accumulator column then (one product a_s * b_s
+// per row of a), and a scale warp leaves them in shared memory, from where they are broadcast to the promotion's FMAs.  (Those
+// reads are what larger tiles fail at: 256 rows a tile, 32768 rows of k 7168, 1.33 ms where fp8_grouped.cu takes 0.92.)
 // Warps of the one persistent CTA per SM:
-//   warp 0      TMA producer: 16 KB of weights and NT rows of a, 128 deep, per stage
+//   warp 0      TMA producer: 16 KB of weights and 64 rows of a, 128 deep, per stage
 //   warp 1      MMA issuer: 4 x tcgen05.mma (M 128) per K block into one of four accumulator buffers
 //   warp 2      scales of the next K blocks
 //   warps 4-11  epilogue, two per lane quadrant with half of the columns each: fp32 promotion in registers, direct stores
+// Tiles of 16 and 32 rows were measured beside those of 64 (us, 16 / 32 / 64): 512 rows in 32 groups as above 82 / 80 / 79; 128
+// rows in 32 groups, n 4096, k 7168 145 / 143 / 140; 1777 rows in 64 uneven groups, n 1472, k 1024 33 / 26 / 24; 8 rows in 8
+// groups, n 4096, k 2048 12.4 / 13.0 / 13.5.
 #include "fp8_grouped.cuh"
 #include "launch.h"
 
@@ -25,29 +29,22 @@ constexpr int NB = 4;                       // accumulator buffers
 constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 32 * (4 + EPI_WARPS);
 
-template <int NT>
-struct FewCfg {
-    static constexpr int kXBytes = NT * BK;
-    static constexpr int kStageBytes = W_BYTES + kXBytes;
-    static constexpr int kStages = 200 * 1024 / kStageBytes;
-    static constexpr int kTmemCols = NB * NT < 32 ? 32 : NB * NT;
-    static constexpr int kSmemBytes = kStages * kStageBytes + NB * NT * 4 + (2 * kStages + 2 * NB) * 8 + 16 +
-                                      (int)sizeof(GroupTable) + 1024;
-    static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
-};
+constexpr int NT = kGroupedFewRows;
+constexpr int HALF = NT / 2;                // columns of one epilogue warp: one TMEM load
+static_assert(HALF == 32, "tmem_ld32");
+constexpr int X_BYTES = NT * BK;
+constexpr int STAGE_BYTES = W_BYTES + X_BYTES;
+constexpr int STAGES = 8;
+constexpr int TMEM_COLS = NB * NT;
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + NB * NT * 4 + (2 * STAGES + 2 * NB) * 8 + 16 + (int)sizeof(GroupTable) + 1024;
+static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
 
-template <int NT>
 __global__ void __launch_bounds__(THREADS, 1)
 fp8_grouped_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_constant__ CUtensorMap tma_x,
                        const GroupedParams p) {
-    using Cfg = FewCfg<NT>;
-    constexpr int STAGES = Cfg::kStages;
-    constexpr int HALF = NT / 2;                            // columns of one epilogue warp
-    constexpr int CHUNK = HALF < 32 ? HALF : 32;            // of one TMEM load
-
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t scale_base = smem_base + STAGES * Cfg::kStageBytes;
+    const uint32_t scale_base = smem_base + STAGES * STAGE_BYTES;
     const uint32_t bar_base = scale_base + NB * NT * 4;
     auto full_bar = [&](uint32_t s) { return bar_base + 8u * s; };
     auto empty_bar = [&](uint32_t s) { return bar_base + 8u * (STAGES + s); };
@@ -73,7 +70,7 @@ fp8_grouped_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_c
         mbar_fence_init();
     }
     if (warp == 1) {
-        tmem_alloc(tmem_slot, Cfg::kTmemCols);
+        tmem_alloc(tmem_slot, TMEM_COLS);
         tmem_relinquish();
     }
     griddep_wait();
@@ -97,8 +94,8 @@ fp8_grouped_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_c
                 for (int kb = 0; kb < kb_total; ++kb, ++it) {
                     ok = mbar_wait(empty_bar(s), ph, p.status, kErrProducerWait, p.launch_tag);
                     if (!ok) break;
-                    const uint32_t st = smem_base + s * Cfg::kStageBytes;
-                    mbar_expect_tx(full_bar(s), Cfg::kStageBytes);
+                    const uint32_t st = smem_base + s * STAGE_BYTES;
+                    mbar_expect_tx(full_bar(s), STAGE_BYTES);
                     tma_load_2d(st, &tma_w, full_bar(s), kb * BK, w_row);
                     tma_load_2d(st + W_BYTES, &tma_x, full_bar(s), kb * BK, x_row);
                     if (++s == STAGES) { s = 0; ph ^= 1; }
@@ -122,7 +119,7 @@ fp8_grouped_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_c
                          mbar_wait(tmem_empty_bar(buf), ((it / NB) & 1) ^ 1, p.status, kErrMmaWaitTmem, p.launch_tag);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint64_t wdesc = desc0 + s * (Cfg::kStageBytes / 16), xdesc = wdesc + W_BYTES / 16;
+                    const uint64_t wdesc = desc0 + s * (STAGE_BYTES / 16), xdesc = wdesc + W_BYTES / 16;
 #pragma unroll
                     for (int j = 0; j < BK / UMMA_K; ++j)
                         umma_f8(tmem_base + buf * NT, wdesc + 2 * j, xdesc + 2 * j, idesc, j > 0 ? 1u : 0u);
@@ -135,7 +132,8 @@ fp8_grouped_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_c
         __syncwarp();
     } else if (warp == 2) {
         // The products a_s * b_s of the tile's rows, K block by K block; loads run PF K blocks ahead inside a tile.
-        constexpr int PER = (NT + 31) / 32;
+        // (Rows behind the group's end take the matrix's last row's: what they are multiplied with is not stored.)
+        constexpr int PER = NT / 32;
         constexpr int PF = 4;
         uint32_t it = 0;
         bool ok = true;
@@ -166,9 +164,7 @@ fp8_grouped_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_c
                                                            p.launch_tag));
                     if (!ok) break;
 #pragma unroll
-                    for (int i = 0; i < PER; ++i)
-                        if (NT >= 32 || lane < NT)
-                            st_shared_f32(scale_base + (buf * NT + i * 32 + lane) * 4, qa[d][i] * qb[d]);
+                    for (int i = 0; i < PER; ++i) st_shared_f32(scale_base + (buf * NT + i * 32 + lane) * 4, qa[d][i] * qb[d]);
                     __syncwarp();
                     if (lane == 0) mbar_arrive(tmem_full_bar(buf));
                     load(d, kb + PF);
@@ -191,21 +187,16 @@ fp8_grouped_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_c
                 ok = mbar_wait(tmem_full_bar(buf), (it / NB) & 1, p.status, kErrEpilogueWait, p.launch_tag);
                 if (!ok) break;
                 tc_fence_after();
+                float v[HALF];
+                tmem_ld32(lane_addr + buf * NT, v);
+                const uint32_t sc = scale_base + (buf * NT + half * HALF) * 4;
 #pragma unroll
-                for (int c = 0; c < HALF / CHUNK; ++c) {
-                    float v[CHUNK];
-                    tmem_ld(lane_addr + buf * NT + c * CHUNK, v);
-                    const uint32_t sc = scale_base + (buf * NT + half * HALF + c * CHUNK) * 4;
-#pragma unroll
-                    for (int j = 0; j < CHUNK / 4; ++j) {
-                        const uint4 s = ld_shared_v4(sc + 16 * j);
-                        float2& a0 = acc[(c * CHUNK + 4 * j) / 2];
-                        float2& a1 = acc[(c * CHUNK + 4 * j) / 2 + 1];
-                        a0 = __ffma2_rn(make_float2(v[4 * j], v[4 * j + 1]),
-                                        make_float2(__uint_as_float(s.x), __uint_as_float(s.y)), a0);
-                        a1 = __ffma2_rn(make_float2(v[4 * j + 2], v[4 * j + 3]),
-                                        make_float2(__uint_as_float(s.z), __uint_as_float(s.w)), a1);
-                    }
+                for (int j = 0; j < HALF / 4; ++j) {
+                    const uint4 s = ld_shared_v4(sc + 16 * j);
+                    acc[2 * j] = __ffma2_rn(make_float2(v[4 * j], v[4 * j + 1]),
+                                            make_float2(__uint_as_float(s.x), __uint_as_float(s.y)), acc[2 * j]);
+                    acc[2 * j + 1] = __ffma2_rn(make_float2(v[4 * j + 2], v[4 * j + 3]),
+                                                make_float2(__uint_as_float(s.z), __uint_as_float(s.w)), acc[2 * j + 1]);
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -233,35 +224,23 @@ fp8_grouped_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_c
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem_base, Cfg::kTmemCols);
+        tmem_dealloc(tmem_base, TMEM_COLS);
     }
-}
-
-template <int NT>
-cudaError_t launch_few(const CUtensorMap& tma_w, const CUtensorMap& tma_x, const GroupedParams& p, int num_sms,
-                       cudaStream_t stream) {
-    static bool attr_set[64] = {};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    auto kernel = fp8_grouped_few_kernel<NT>;
-    if (dev < 64 && !attr_set[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FewCfg<NT>::kSmemBytes);
-        if (e != cudaSuccess) return e;
-        attr_set[dev] = true;
-    }
-    return launch_kernel(kernel, dim3((unsigned)num_sms), THREADS, FewCfg<NT>::kSmemBytes, stream, true, tma_w, tma_x, p);
 }
 
 }  // namespace
 
-cudaError_t fp8_grouped_few_launch(const CUtensorMap& tma_w, const CUtensorMap& tma_x, const GroupedParams& p, int tile_rows,
-                                   int num_sms, cudaStream_t stream) {
-    switch (tile_rows) {
-        case 16: return launch_few<16>(tma_w, tma_x, p, num_sms, stream);
-        case 32: return launch_few<32>(tma_w, tma_x, p, num_sms, stream);
-        case 64: return launch_few<64>(tma_w, tma_x, p, num_sms, stream);
-        default: return launch_few<128>(tma_w, tma_x, p, num_sms, stream);
+cudaError_t fp8_grouped_few_launch(const CUtensorMap& tma_w, const CUtensorMap& tma_x, const GroupedParams& p, int num_sms,
+                                   cudaStream_t stream) {
+    static bool attr_set[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 64 && !attr_set[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(fp8_grouped_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+        if (e != cudaSuccess) return e;
+        attr_set[dev] = true;
     }
+    return launch_kernel(fp8_grouped_few_kernel, dim3((unsigned)num_sms), THREADS, SMEM_BYTES, stream, true, tma_w, tma_x, p);
 }
 
 }  // namespace rf

@@ -60,6 +60,7 @@ def run(counts, n, k, dtype=torch.bfloat16, head=0, tail=0, seed=0):
     return a, b, a_s, b_s, c
 
 
+# the kernel for many rows is chosen beyond 64 rows a group on the mean, if its tiles of 128 x 256 fill the chip
 FEW = [[1], [16], [17], [0, 0, 3, 0], [5] * 33, [1, 0, 40, 2, 15, 16, 17, 0], [0] * 1023 + [9], [33, 64, 31, 129], [127, 1, 120]]
 MANY = [[128], [129], [255, 256, 257], [1000, 0, 24, 512, 5], [0, 700], [2300], [384, 32, 31, 33, 640, 1]]
 
@@ -70,13 +71,25 @@ def test_against_64_bits(counts, n, k, dtype):
     run(counts, n, k, dtype, seed=sum(counts) + n)
 
 
-@pytest.mark.parametrize("counts", [[3, 0, 30], [200, 77]])
+WIDE = 10304            # 41 blocks of 256 columns, the last of them one of 64
+WIDE_COUNTS = [[255, 256, 257], [1000, 0, 24, 512, 5], [2300], [384, 32, 31, 33, 640, 1], [0, 513, 0, 64]]
+
+
+@pytest.mark.parametrize("counts", WIDE_COUNTS, ids=lambda c: f"{len(c)}g{sum(c)}")
+@pytest.mark.parametrize("n,k,dtype", [(WIDE, 128, torch.bfloat16), (WIDE, 640, torch.float16), (WIDE - 64, 384, torch.bfloat16),
+                                       (WIDE + 128, 256, torch.float16)])
+def test_many_rows_against_64_bits(counts, n, k, dtype):
+    assert sum(counts) > 64 * len(counts) and (sum(counts) // 128 + len(counts)) * ((n + 255) // 256) > 148
+    run(counts, n, k, dtype, seed=sum(counts) + n)
+
+
+@pytest.mark.parametrize("counts,n", [([3, 0, 30], 320), ([200, 77], 320), ([700, 800], WIDE)])
 @pytest.mark.parametrize("head,tail", [(0, 1), (5, 0), (19, 301)])
-def test_rows_outside_the_groups(counts, head, tail):
-    run(counts, 320, 256, head=head, tail=tail)
+def test_rows_outside_the_groups(counts, n, head, tail):
+    run(counts, n, 256, head=head, tail=tail)
 
 
-@pytest.mark.parametrize("counts,n,k", [([20] * 12, 1472, 2048), ([300] * 5, 1088, 2048), ([1] * 64, 4096, 1024)])
+@pytest.mark.parametrize("counts,n,k", [([20] * 12, 1472, 2048), ([300] * 5, 1088, 2048), ([300] * 12, 4160, 1024), ([1000, 30, 0, 777], 8192, 512), ([1] * 64, 4096, 1024)])
 def test_several_rounds(counts, n, k):
     run(counts, n, k, torch.float16)
 
@@ -94,30 +107,31 @@ def test_all_groups_empty():
 
 def test_offsets_outside_the_matrix_are_clipped():
     """No table leads outside the matrices: a negative start counts as 0, an end beyond m as m, a descending pair as empty."""
-    for m in (40, 600):
-        a, b, a_s, b_s = operands(m, 3, 128, 256, 2)
-        full = torch.full((m + 300, 128), 5.0, device=DEV, dtype=torch.bfloat16)
+    for m, n in ((40, 128), (600, WIDE)):
+        a, b, a_s, b_s = operands(m, 3, n, 256, 2)
+        full = torch.full((m + 300, n), 5.0, device=DEV, dtype=torch.bfloat16)
         off = torch.tensor([-7, 10, 4, 2 ** 31 - 1], dtype=torch.int32, device=DEV)
         grouped.fp8_grouped_mm(a, b, a_s, b_s, off, full[:m])
-        ref = torch.empty(m, 128, device=DEV, dtype=torch.bfloat16)
+        ref = torch.empty(m, n, device=DEV, dtype=torch.bfloat16)
         grouped.fp8_grouped_mm(a[:4], b, a_s[:4], b_s, torch.tensor([0, 4, 4, 4], dtype=torch.int32, device=DEV), ref[:4])
         torch.cuda.synchronize()
         assert gemm.device_status() == 0 and (full[m:] == 5).all()
-        assert torch.equal(full[:4], ref[:4])          # (rows 4 .. 9 are in two groups)
+        # (rows 4 .. 9 are in two groups; the two kernels add in one order)
+        assert torch.equal(full[:4], ref[:4])
         assert not (full[10:m] == 5).all(1).any()
 
 
 def test_nan_stays_in_its_rows():
-    for counts in ([5, 4, 7], [200, 130, 170]):
+    for counts, n in (([5, 4, 7], 192), ([200, 130, 170], WIDE)):
         m = sum(counts)
-        a, b, a_s, b_s = operands(m, 3, 192, 256, 3)
+        a, b, a_s, b_s = operands(m, 3, n, 256, 3)
         off = torch.tensor([0, *np.cumsum(counts)], dtype=torch.int32, device=DEV)
-        want = grouped.fp8_grouped_mm(a, b, a_s, b_s, off, torch.empty(m, 192, device=DEV, dtype=torch.bfloat16))
+        want = grouped.fp8_grouped_mm(a, b, a_s, b_s, off, torch.empty(m, n, device=DEV, dtype=torch.bfloat16))
         a_s = a_s.clone()
         a_s[counts[0]] = float("nan")
         b.view(torch.uint8)[2, 10, 7] = 0x7F
-        got = grouped.fp8_grouped_mm(a, b, a_s, b_s, off, torch.empty(m, 192, device=DEV, dtype=torch.bfloat16))
-        bad = torch.zeros(m, 192, dtype=torch.bool, device=DEV)
+        got = grouped.fp8_grouped_mm(a, b, a_s, b_s, off, torch.empty(m, n, device=DEV, dtype=torch.bfloat16))
+        bad = torch.zeros(m, n, dtype=torch.bool, device=DEV)
         bad[counts[0]] = True
         bad[counts[0] + counts[1]:, 10] = True
         assert got[bad].isnan().all() and torch.equal(got[~bad], want[~bad])
