@@ -30,6 +30,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
+// max(|a|, |b|, c)
+__device__ __forceinline__ float max_abs_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(c));
+    return r;
+}
 // Four values to four e4m3 bytes, the first in the lowest.
 __device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d) {
     uint16_t lo, hi;
@@ -68,6 +74,27 @@ struct Eight {
     __device__ __forceinline__ float f(int i) const { return to_f32(e[i]); }
 };
 
+__device__ __forceinline__ float largest_of(const float (&x)[8]) {
+    float a = max_nan(fabsf(x[0]), fabsf(x[1]));
+#pragma unroll
+    for (int i = 2; i < 8; i += 2) a = max_abs_nan(x[i], x[i + 1], a);
+    return a;
+}
+// (magnitudes of 16-bit types two at a time, before they are widened)
+__device__ __forceinline__ float largest_of(const Eight<float>& x) { return largest_of(x.e); }
+__device__ __forceinline__ float largest_of(const Eight<__half>& x) {
+    __half2 a = __habs2(__halves2half2(x.e[0], x.e[1]));
+#pragma unroll
+    for (int i = 2; i < 8; i += 2) a = __hmax2_nan(a, __habs2(__halves2half2(x.e[i], x.e[i + 1])));
+    return max_nan(__low2float(a), __high2float(a));
+}
+__device__ __forceinline__ float largest_of(const Eight<__nv_bfloat16>& x) {
+    __nv_bfloat162 a = __habs2(__halves2bfloat162(x.e[0], x.e[1]));
+#pragma unroll
+    for (int i = 2; i < 8; i += 2) a = __hmax2_nan(a, __habs2(__halves2bfloat162(x.e[i], x.e[i + 1])));
+    return max_nan(__low2float(a), __high2float(a));
+}
+
 // The half warp's largest value (16 lanes hold one block of 128).
 __device__ __forceinline__ float half_warp_max(float a) {
 #pragma unroll
@@ -101,14 +128,7 @@ __device__ __forceinline__ float silu(float g) {
     return g * r;
 }
 
-// This lane's eight of a block's 128 values -> its eight bytes, and the block's scale.
-__device__ __forceinline__ uint2 quantize_eight(const float (&x)[8], float* scale) {
-    float a = fabsf(x[0]);
-#pragma unroll
-    for (int i = 1; i < 8; ++i) a = max_nan(a, fabsf(x[i]));
-    a = max_nan(half_warp_max(a), kAmaxFloor);
-    *scale = over_448(a);
-    const float r = steps_per_unit(a);
+__device__ __forceinline__ uint2 to_e4m3x8(const float (&x)[8], float r) {
     return make_uint2(to_e4m3x4(x[0] * r, x[1] * r, x[2] * r, x[3] * r), to_e4m3x4(x[4] * r, x[5] * r, x[6] * r, x[7] * r));
 }
 
@@ -116,6 +136,11 @@ __device__ __forceinline__ uint2 quantize_eight(const float (&x)[8], float* scal
 // 16 lanes per block of 128 columns, PER blocks in a row per half warp: all their loads are in flight before the first is used.
 // PER is 4, or 1 where that fills the chip no more than twice over.  Row i of the result is row i of x, or row rows[i] mod n_src
 // (as an unsigned number, so that no index leaves x).
+//
+// Memory and instructions bound it alike: a thread's 32 elements were 496 instructions when every lane reduced each of its blocks
+// by itself, found its scale and checked each element for the end, and 32768 gathered rows of 7168 bf16 took 121 us.  So the four
+// blocks are reduced together (lane l ends with block l / 4's maximum, by 5 shuffles instead of 16) and each quad of lanes finds one
+// block's factors.
 constexpr int kRowThreads = 256;
 
 // SWIGLU: x is [gate | up], 2 k columns, and what is quantised is SiLU(gate) * up in fp32.
@@ -123,45 +148,70 @@ template <class T, bool VEC, bool SWIGLU, int PER>
 __global__ void __launch_bounds__(kRowThreads)
 quantize_rows_kernel(const T* x, long long row_stride, const int* rows, uint32_t n_src, uint32_t total, uint32_t kb, uint8_t* q,
                      float* scale) {
+    static_assert(PER == 1 || PER == 4, "");
     griddep_launch_dependents();
     griddep_wait();
     const int lane = threadIdx.x & 15;
     // (total < 2^31, and the last CTA reaches less than 64 beyond it)
     const uint32_t first = (blockIdx.x * (kRowThreads / 16) + (threadIdx.x >> 4)) * PER;
     if (first - (threadIdx.x & 16 ? PER : 0) >= total) return;       // whole warps leave: the shuffles need all lanes
-    uint32_t row = first / kb, col = first - row * kb;
+    auto source = [&](uint32_t row) {
+        if (rows == nullptr) return row;
+        const uint32_t src = (uint32_t)ld_global_s32(rows + row);
+        return src < n_src ? src : src % n_src;
+    };
     Eight<T> g[PER], u[SWIGLU ? PER : 1];
+    uint32_t at = min(first, total - 1), row = at / kb, col = at - row * kb;
+    const T* p = x + (long long)source(row) * row_stride + col * kBlock + lane * 8;
+    if (col + PER <= kb && first + PER <= total) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        if (first + i < total) {
-            uint32_t src = row;
-            if (rows != nullptr) {
-                src = (uint32_t)ld_global_s32(rows + row);
-                if (src >= n_src) src %= n_src;
-            }
-            const T* p = x + (long long)src * row_stride + col * kBlock + lane * 8;
+        for (int i = 0; i < PER; ++i) {
+            g[i].template load<VEC>(p + i * kBlock);
+            if (SWIGLU) u[i].template load<VEC>(p + (size_t)kb * kBlock + i * kBlock);
+        }
+    } else {                                                        // over the ends of rows; what lies behind the last repeats it
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
             g[i].template load<VEC>(p);
             if (SWIGLU) u[i].template load<VEC>(p + (size_t)kb * kBlock);
-        }
-        if (++col == kb) {
-            col = 0;
-            ++row;
+            if (at + 1 < total) {
+                ++at;
+                p += kBlock;
+                if (++col == kb) {
+                    col = 0;
+                    p = x + (long long)source(++row) * row_stride + lane * 8;
+                }
+            }
         }
     }
+    float v[PER][8], a[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const bool valid = first + i < total;
-        float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[j] = valid ? g[i].f(j) : 0.f;
-            if (SWIGLU) v[j] = silu(v[j]) * (valid ? u[i].f(j) : 0.f);
+        for (int j = 0; j < 8; ++j) v[i][j] = SWIGLU ? silu(g[i].f(j)) * u[i].f(j) : g[i].f(j);
+        a[i] = SWIGLU ? largest_of(v[i]) : largest_of(g[i]);
+    }
+    uint8_t* to = q + (size_t)first * kBlock + lane * 8;
+    if (PER == 4) {
+        const bool up8 = lane & 8, up4 = lane & 4;
+        float b = max_nan(up8 ? a[PER / 2] : a[0], __shfl_xor_sync(0xffffffffu, up8 ? a[0] : a[PER / 2], 8));
+        float c = max_nan(up8 ? a[PER - 1] : a[PER / 4], __shfl_xor_sync(0xffffffffu, up8 ? a[PER / 4] : a[PER - 1], 8));
+        b = max_nan(up4 ? c : b, __shfl_xor_sync(0xffffffffu, up4 ? b : c, 4));
+        b = max_nan(b, __shfl_xor_sync(0xffffffffu, b, 2));
+        b = max_nan(max_nan(b, __shfl_xor_sync(0xffffffffu, b, 1)), kAmaxFloor);
+        const float steps = steps_per_unit(b);
+        if ((lane & 3) == 0 && first + (lane >> 2) < total) scale[first + (lane >> 2)] = over_448(b);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const float r = __shfl_sync(0xffffffffu, steps, 4 * i, 16);
+            if (first + i < total) *reinterpret_cast<uint2*>(to + i * kBlock) = to_e4m3x8(v[i], r);
         }
-        float s;
-        const uint2 o = quantize_eight(v, &s);
-        if (valid) {
-            *reinterpret_cast<uint2*>(q + (size_t)(first + i) * kBlock + lane * 8) = o;
-            if (lane == 0) scale[first + i] = s;
+    } else {
+        const float b = max_nan(half_warp_max(a[0]), kAmaxFloor);
+        const uint2 o = to_e4m3x8(v[0], steps_per_unit(b));
+        if (first < total) {
+            *reinterpret_cast<uint2*>(to) = o;
+            if (lane == 0) scale[first] = over_448(b);
         }
     }
 }
