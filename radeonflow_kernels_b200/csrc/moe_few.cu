@@ -44,13 +44,13 @@ constexpr int DRAW_AHEAD = 4;           // stages before an item's last load at 
 constexpr int MAX_PAIRS = kFewMaxTokens * kFewMaxTopK;
 
 enum ItemKind { kRouter = 0, kFirst = 1, kSecond = 2, kEnd = 3 };
-// kind, expert slot (index into the active list, -1 = shared), column tile, K chunk
+// kind, expert slot (index into the active list; the shared expert's are -1, -2), column tile, K chunk
 using Item = int4;
 
 struct Routing {
     int n_active;
-    int active[kFewMaxExperts];         // experts with tokens, ascending
-    int base[kFewMaxExperts + 1];       // first pair of each of them; pairs are sorted by expert, then token
+    int active[MAX_PAIRS];              // experts with tokens, ascending, each once per kRows tokens
+    int base[MAX_PAIRS + 1];            // first pair of each of them; pairs are sorted by expert, then token
     int token[MAX_PAIRS];               // of a pair
     int expert[MAX_PAIRS];              // [token][rank]
     int pos[MAX_PAIRS];                 // pair of [token][rank]
@@ -63,10 +63,9 @@ template <bool FP8, int NG>
 struct Cfg {
     static constexpr int kStageK = FP8 ? 128 : 64;
     static constexpr int kRows = 8 * NG;
-    static constexpr int kMaxChunk = NG == 4 ? 512 : 1024;
     // beside fp16 weights x goes through ldmatrix (rows 16 bytes apart modulo 128), beside FP8 through 16-byte loads (64 bytes)
     static constexpr int kPad = FP8 ? 64 : 16;
-    static constexpr int kXStride = kMaxChunk * 2 + kPad;
+    static constexpr int kXStride = kFewMaxChunk * 2 + kPad;
     // ... and behind the rows the scales of the item's two boxes, one per 128 of K
     static constexpr int kXBytes = kRows * kXStride + (FP8 ? 64 : 0);
     // a router unit's partial sums of every MMA warp; later the sums that one group of them hands to the other
@@ -198,11 +197,12 @@ __device__ __forceinline__ bool idle_wait(uint32_t bar, uint32_t parity, int* st
 
 // How the work divides: known once the routing is.
 struct Shape {
+    int groups;                 // slots of the shared expert
     int tiles1, tiles1s;        // column tiles of the first product: of an expert, of the shared one
     int tiles2;
     int chunks1, chunks2, chunks2s;
-    __device__ __forceinline__ explicit Shape(const MoeFewParams& p)
-        : tiles1(p.f / 64), tiles1s(p.fs / 64), tiles2((p.d + 127) / 128), chunks1((p.d + p.kc1 - 1) / p.kc1),
+    __device__ __forceinline__ Shape(const MoeFewParams& p, int rows)
+        : groups((p.t + rows - 1) / rows), tiles1(p.f / 64), tiles1s(p.fs / 64), tiles2((p.d + 127) / 128), chunks1((p.d + p.kc1 - 1) / p.kc1),
           chunks2((p.f + p.kc2 - 1) / p.kc2), chunks2s((p.fs + p.kc2 - 1) / p.kc2) {}
 };
 
@@ -215,11 +215,12 @@ __device__ __forceinline__ Item decode_routed(int r, const Shape& s, int n_activ
         return make_int4(kFirst, e, i - c * s.tiles1, c);
     }
     r -= n_active * per1;
-    if (r < s.tiles2 * s.chunks2s) {
-        const int c = r / s.tiles2;
-        return make_int4(kSecond, -1, r - c * s.tiles2, c);
+    const int per2s = s.tiles2 * s.chunks2s;
+    if (r < s.groups * per2s) {
+        const int e = r / per2s, i = r - e * per2s, c = i / s.tiles2;
+        return make_int4(kSecond, -1 - e, i - c * s.tiles2, c);
     }
-    r -= s.tiles2 * s.chunks2s;
+    r -= s.groups * per2s;
     const int per2 = s.tiles2 * s.chunks2;
     if (r < n_active * per2) {
         const int e = r / per2, i = r - e * per2, c = i / s.tiles2;
@@ -325,6 +326,7 @@ __device__ __forceinline__ bool route_token(const MoeFewParams& p, Routing& rt, 
 
 // One warp: the experts' token lists, in an order that every CTA finds alike.  Ranks inside 32 pairs by match_any, pairs in order;
 // then the experts' offsets, eight experts a lane.
+template <int ROWS>
 __device__ __forceinline__ void build_lists(const MoeFewParams& p, Routing& rt) {
     const int lane = threadIdx.x & 31, pairs = p.t * p.top_k;
     for (int e = lane; e < kFewMaxExperts; e += 32) rt.count[e] = 0;
@@ -338,12 +340,12 @@ __device__ __forceinline__ void build_lists(const MoeFewParams& p, Routing& rt) 
         if (e >= 0 && before == 0) rt.count[e] += __popc(peers);
         __syncwarp();
     }
-    // pairs (low half) and active experts (high half) in front of this lane's eight experts
+    // pairs (low half) and slots (high half) in front of this lane's eight experts
     int n[8], mine = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         n[i] = rt.count[8 * lane + i];
-        mine += n[i] + ((n[i] > 0) << 16);
+        mine += n[i] + ((n[i] + ROWS - 1) / ROWS << 16);
     }
     int incl = mine;
 #pragma unroll
@@ -354,12 +356,12 @@ __device__ __forceinline__ void build_lists(const MoeFewParams& p, Routing& rt) 
     int run = incl - mine;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        if (n[i] > 0) {
+        rt.count[8 * lane + i] = run & 0xFFFF;          // now the expert's first pair
+        for (int left = n[i]; left > 0; left -= ROWS) {
             rt.active[run >> 16] = 8 * lane + i;
             rt.base[run >> 16] = run & 0xFFFF;
+            run += min(left, ROWS) + (1 << 16);
         }
-        rt.count[8 * lane + i] = run & 0xFFFF;          // now the expert's first pair
-        run += n[i] + ((n[i] > 0) << 16);
     }
     if (lane == 31) {
         rt.n_active = run >> 16;
@@ -444,8 +446,8 @@ moe_few_kernel(const MoeFewParams p) {
         return;
     }
 
-    const Shape shape(p);
-    const int shared_first = shape.tiles1s * shape.chunks1;
+    const Shape shape(p, C::kRows);
+    const int shared_first = shape.groups * shape.tiles1s * shape.chunks1;
     const int before_routed = p.router_units + shared_first;
     const int pairs = p.t * p.top_k;            // the shared expert's pairs come behind them, one per token
     const size_t rows = pairs + p.t;            // of h and the partial sums
@@ -466,8 +468,11 @@ moe_few_kernel(const MoeFewParams p) {
         *len = min(kc, k - *k0);
     };
     auto expert_of = [&](const Item& it) { return it.y < 0 ? p.experts : rt.active[it.y]; };
-    auto first_pair = [&](const Item& it) { return it.y < 0 ? pairs : rt.base[it.y]; };
-    auto pair_count = [&](const Item& it) { return it.y < 0 ? p.t : rt.base[it.y + 1] - rt.base[it.y]; };
+    auto first_token = [&](const Item& it) { return (-1 - it.y) * C::kRows; };       // (the shared expert's)
+    auto first_pair = [&](const Item& it) { return it.y < 0 ? pairs + first_token(it) : rt.base[it.y]; };
+    auto pair_count = [&](const Item& it) {
+        return it.y < 0 ? min(p.t - first_token(it), C::kRows) : rt.base[it.y + 1] - rt.base[it.y];
+    };
 
     bool lost = false;          // this thread's role gave a wait up
     if (warp == 0) {
@@ -481,8 +486,9 @@ moe_few_kernel(const MoeFewParams p) {
                 if (ticket < p.router_units) {
                     it = make_int4(kRouter, 0, ticket, 0);
                 } else if (ticket < before_routed) {
-                    const int i = ticket - p.router_units, c = i / shape.tiles1s;
-                    it = make_int4(kFirst, -1, i - c * shape.tiles1s, c);
+                    const int per = shape.tiles1s * shape.chunks1, r = ticket - p.router_units, e = r / per, i = r - e * per;
+                    const int c = i / shape.tiles1s;
+                    it = make_int4(kFirst, -1 - e, i - c * shape.tiles1s, c);
                 } else {
                     if (!routed) {
                         ok = wait_routed(kErrProducerWait);
@@ -568,7 +574,7 @@ moe_few_kernel(const MoeFewParams p) {
                     if (lane == 0) mbar_expect_tx_only(x_full_bar(b), (uint32_t)(n_rows * len * 2));
                     __syncwarp();
                     if (lane < n_rows) {
-                        const int row = it.y >= 0 ? rt.token[first + lane] : lane;
+                        const int row = it.y >= 0 ? rt.token[first + lane] : first_token(it) + lane;
                         bulk_load(dst + lane * C::kXStride, static_cast<const __half*>(p.x) + (size_t)row * p.d + k0, (uint32_t)len * 2,
                                   x_full_bar(b));
                     }
@@ -643,7 +649,8 @@ moe_few_kernel(const MoeFewParams p) {
             if (it.x == kRouter) {
                 // 16 experts x a chunk of K, 64 columns per warp and round.  A lane holds 16 consecutive k of its row (and token): the
                 // order of k inside a fragment is free as long as both operands share it.
-                const int e0 = it.z / p.router_chunks * 16, c = it.z % p.router_chunks;
+                const int c = it.z % p.router_chunks, et = it.z / p.router_chunks, e_tiles = (p.experts + 15) / 16;
+                const int e0 = et % e_tiles * 16, t0 = et / e_tiles * C::kRows;
                 float acc[NG][4] = {};
 #pragma unroll 1
                 for (int k = c * p.router_kc + w * 64; k < min((c + 1) * p.router_kc, p.d); k += MMA_WARPS * 64) {
@@ -656,7 +663,7 @@ moe_few_kernel(const MoeFewParams p) {
                     }
 #pragma unroll
                     for (int i = 0; i < NG; ++i) {
-                        const __half* row = static_cast<const __half*>(p.x) + (size_t)min(8 * i + g, p.t - 1) * p.d;
+                        const __half* row = static_cast<const __half*>(p.x) + (size_t)min(t0 + 8 * i + g, p.t - 1) * p.d;
 #pragma unroll
                         for (int v = 0; v < 2; ++v) b[i][v] = ld_global_cg_v4(row + k + 16 * q + 8 * v);
                     }
@@ -682,7 +689,7 @@ moe_few_kernel(const MoeFewParams p) {
                 ok = meet();
                 if (!ok) break;
                 for (int i = w * 32 + lane; i < 16 * C::kRows; i += 32 * MMA_WARPS) {
-                    const int e = e0 + i / C::kRows, t = i % C::kRows;
+                    const int e = e0 + i / C::kRows, t = t0 + i % C::kRows;
                     float v = 0.f;
 #pragma unroll
                     for (int o = 0; o < MMA_WARPS; ++o)
@@ -866,7 +873,7 @@ moe_few_kernel(const MoeFewParams p) {
             else ok = route_token<8>(p, rt, t, call, patience);
         }
         ok = named_barrier_all(BAR_SUM, 32 * SUM_WARPS, ok);
-        if (ok && w == 0) build_lists(p, rt);
+        if (ok && w == 0) build_lists<C::kRows>(p, rt);
         named_barrier(BAR_SUM, 32 * SUM_WARPS);
         if (ok && w == 0 && lane == 0) mbar_arrive(routed_bar);
         // ------------------------------------------------------------------------------ sums of complete tiles
@@ -964,11 +971,8 @@ cudaError_t launch_one(const MoeFewParams& p, int num_sms, cudaStream_t stream) 
 }  // namespace
 
 cudaError_t moe_few_launch(const MoeFewParams& p, bool fp8, int num_sms, cudaStream_t stream) {
-    switch (moe_few_groups(p.t)) {
-        case 1: return fp8 ? launch_one<true, 1>(p, num_sms, stream) : launch_one<false, 1>(p, num_sms, stream);
-        case 2: return fp8 ? launch_one<true, 2>(p, num_sms, stream) : launch_one<false, 2>(p, num_sms, stream);
-        default: return fp8 ? launch_one<true, 4>(p, num_sms, stream) : launch_one<false, 4>(p, num_sms, stream);
-    }
+    if (moe_few_rows(p.t) == 8) return fp8 ? launch_one<true, 1>(p, num_sms, stream) : launch_one<false, 1>(p, num_sms, stream);
+    return fp8 ? launch_one<true, 2>(p, num_sms, stream) : launch_one<false, 2>(p, num_sms, stream);
 }
 
 }  // namespace rf

@@ -35,10 +35,13 @@ struct MoeFewParams {
     int launch_tag;
 };
 
-// Rows of the widest MMA group that t tokens need: 1, 2 or 4 groups of 8.
-inline int moe_few_groups(int t) { return t <= 8 ? 1 : t <= 16 ? 2 : 4; }
-// Largest K chunk whose two operand buffers leave room for the weight stages.
-inline int moe_few_max_chunk(int t) { return t <= 16 ? 1024 : 512; }
+// Token rows of an item: 8, or 16.  An expert with more tokens than that (and the shared one) takes several items a tile, of which the
+// later find the weights in L2.  (Items of 32 rows leave room for chunks of 512 and an accumulator that spills: 32 tokens through
+// 8 of 256 FP8 experts of 7168 x 2048 took 1835 us so.)
+inline int moe_few_rows(int t) { return t <= 8 ? 8 : 16; }
+inline int moe_few_token_groups(int t) { return (t + 15) / 16; }
+// Largest K chunk: its two operand buffers leave room for the weight stages.
+constexpr int kFewMaxChunk = 1024;
 // K of a router unit: whole rounds of the eight MMA warps; longer for many experts, whose sums every CTA has to gather.
 inline int moe_few_router_chunk(int experts) { return experts <= 64 ? 512 : experts == 128 ? 1024 : 2048; }
 

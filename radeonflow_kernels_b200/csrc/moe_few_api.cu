@@ -48,11 +48,10 @@ Plan make_plan(const RfMoeFewConfig& c, int t) {
     const int num_sms = 148;
     const int fs = c.d_expert * c.n_shared_experts, width = fs > c.d_expert ? fs : c.d_expert;
     const int hit = c.n_routed_experts < t * c.n_experts_per_token ? c.n_routed_experts : t * c.n_experts_per_token;
-    const int most = rf::moe_few_max_chunk(t);
     const size_t pairs = (size_t)t * (c.n_experts_per_token + 1), d = c.d_hidden;
     Plan p;
-    p.kc1 = choose_chunk((hit * c.d_expert + fs) / 64, c.d_hidden, most, num_sms);
-    p.kc2 = choose_chunk((hit + (fs > 0)) * ((c.d_hidden + 127) / 128), c.d_expert, most, num_sms);
+    p.kc1 = choose_chunk((hit * c.d_expert + fs) / 64, c.d_hidden, rf::kFewMaxChunk, num_sms);
+    p.kc2 = choose_chunk((hit + (fs > 0)) * ((c.d_hidden + 127) / 128), c.d_expert, rf::kFewMaxChunk, num_sms);
     p.router_kc = rf::moe_few_router_chunk(c.n_routed_experts);
     p.router_chunks = (c.d_hidden + p.router_kc - 1) / p.router_kc;
     const size_t chunks1 = (d + p.kc1 - 1) / p.kc1, chunks2 = ((size_t)width + p.kc2 - 1) / p.kc2;
@@ -244,7 +243,7 @@ int rf_moe_few_forward(RfMoeFew* few, const void* x, int n_tokens, void* out, vo
     p.kc2 = plan.kc2;
     p.router_kc = plan.router_kc;
     p.router_chunks = plan.router_chunks;
-    p.router_units = (p.experts + 15) / 16 * p.router_chunks;
+    p.router_units = (p.experts + 15) / 16 * p.router_chunks * rf::moe_few_token_groups(p.t);
     p.status = st->status;
     p.launch_tag = rf::next_launch_tag();
     const cudaError_t e = rf::moe_few_launch(p, c.weight_type == RF_MOE_FEW_E4M3, st->num_sms, reinterpret_cast<cudaStream_t>(stream));
