@@ -190,9 +190,11 @@ fp8_grouped_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_c
                 float v[HALF];
                 tmem_ld32(lane_addr + buf * NT, v);
                 const uint32_t sc = scale_base + (buf * NT + half * HALF) * 4;
+                uint32_t seen = 0;
 #pragma unroll
                 for (int j = 0; j < HALF / 4; ++j) {
                     const uint4 s = ld_shared_v4(sc + 16 * j);
+                    seen |= s.x;
                     acc[2 * j] = __ffma2_rn(make_float2(v[4 * j], v[4 * j + 1]),
                                             make_float2(__uint_as_float(s.x), __uint_as_float(s.y)), acc[2 * j]);
                     acc[2 * j + 1] = __ffma2_rn(make_float2(v[4 * j + 2], v[4 * j + 3]),
@@ -200,7 +202,7 @@ fp8_grouped_few_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_c
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(tmem_empty_bar(buf));
+                if (lane == 0) mbar_arrive_after(tmem_empty_bar(buf), seen, (uint32_t)p.groups >> 16);
             }
             if (!ok) break;
             const GroupedTile t = decode_grouped(table, p, w, tiles_n);

@@ -8,6 +8,7 @@
 // multiplications.  So one persistent CTA per SM keeps a ring of TMA loads full from the first microsecond to the last, and all
 // that depends on something else happens beside it.  The work is a list of items, dealt out by a ticket in this order:
 //   router units   16 experts x a chunk of K of the logits, partial sums
+//   routes         a token's top-k, from its logits
 //   first product  64 columns of gate and the same of up x a chunk of K, the shared expert's first (they need no routing)
 //   second product 128 columns of the result x a chunk of K
 // An item depends on items with smaller tickets only, and a CTA works its tickets off in order, so whatever share of the grid is
@@ -17,13 +18,18 @@
 // polls for: no fence, no counter, one trip through L2.  (With partial sums behind fences and counters, each hand-over was four
 // or five trips of 1.2 us under load: one token through 9 experts of 1024 x 512 took 25 us, through 5 of 7168 x 2048 98.)  The
 // item with the last chunk of a column tile adds the chunks up in their order, and the last item of a result tile adds the
-// experts in rank order: results are the same bits whoever comes last.  Warps of a CTA:
+// experts in rank order: results are the same bits whoever comes last.  A token is routed by one CTA: every CTA for itself takes one
+// hand-over less, and for 32 tokens through 128 or 256 experts 10 us more.
+// One token through 9 fp16 experts of 1024 x 512 takes 18 us, through 5 of 7168 x 2048 70 (6.3 TB/s); 13 tokens through 86 of 256
+// FP8 experts 700 (5.5 TB/s), 32 through 164 1280 (5.7).  What holds FP8 below fp16's rate: the MMA warps are busy for two thirds of
+// the time, so that their waits and the stream's do not always overlap.  Warps of a CTA:
 //   0      draws tickets, issues the weight loads (16 KB stages)
 //   1-3    the items' token rows (or, for the second product, h) into shared memory
 //   4-11   mma.sync m16n8k16, weights as the 16-row operand, up to 8 tokens as the 8 columns: a warp owns 16 of the item's 128
 //          columns.  (The legacy tensor path on purpose: the stream feeds one such MMA per 21 cycles and SM, and its
 //          accumulators need no trip through TMEM.)  FP8 weights become fp16 on the way, their scale is applied per 128 of K.
-//   12-15  softmax, top-k and the experts' token lists, in every CTA for itself; then the sums of complete tiles
+//   12-15  softmax and top-k of a token (its ticket says whose), the experts' token lists (every CTA for itself), then the sums of
+//          complete tiles
 // h is rounded to fp16, the type of the second product's operand; everything else is fp32.
 #include "moe_few.h"
 #include "launch.h"
@@ -37,13 +43,12 @@ namespace {
 constexpr int WARP_X = 1, WARP_MMA = 4, WARP_SUM = 12, WARPS = 16;
 constexpr int X_WARPS = WARP_MMA - WARP_X, MMA_WARPS = WARP_SUM - WARP_MMA, SUM_WARPS = WARPS - WARP_SUM;
 constexpr int THREADS = 32 * WARPS;
-constexpr int BAR_SUM = 1;
 constexpr int STAGE_BYTES = 16384, BOX_BYTES = 8192;
 constexpr int ITEM_SLOTS = 8, SUM_SLOTS = 8;
 constexpr int DRAW_AHEAD = 4;           // stages before an item's last load at which the next ticket is drawn
 constexpr int MAX_PAIRS = kFewMaxTokens * kFewMaxTopK;
 
-enum ItemKind { kRouter = 0, kFirst = 1, kSecond = 2, kEnd = 3 };
+enum ItemKind { kRouter = 0, kFirst = 1, kSecond = 2, kEnd = 3, kRoute = 4, kLists = 5 };
 // kind, expert slot (index into the active list; the shared expert's are -1, -2), column tile, K chunk
 using Item = int4;
 
@@ -72,7 +77,7 @@ struct Cfg {
     static constexpr int kRedBytes = MMA_WARPS * 16 * kRows * 4;
     static_assert(kRedBytes == MMA_WARPS / 2 * 2 * NG * 4 * 128, "both uses");
     static constexpr int kStages = NG == 1 ? 11 : 8;
-    static constexpr int kBars = 2 * kStages + 4 + 2 * ITEM_SLOTS + 2 * SUM_SLOTS + 2 + MMA_WARPS;
+    static constexpr int kBars = 2 * kStages + 4 + 2 * ITEM_SLOTS + 2 * SUM_SLOTS + 3 + MMA_WARPS;
     static constexpr int kSmemBytes = kStages * STAGE_BYTES + 2 * kXBytes + kRedBytes + (ITEM_SLOTS + SUM_SLOTS) * 16 + kBars * 8 +
                                       (int)sizeof(Routing) + 1024;
     static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
@@ -229,64 +234,69 @@ __device__ __forceinline__ Item decode_routed(int r, const Shape& s, int n_activ
     return make_int4(kEnd, 0, 0, 0);
 }
 
-// One warp: a token's logits from their partial sums, softmax and top-k as topk_kernel (moe_route.cu) does them, on the same fp16
-// roundings.  Lane l owns experts l * VPT ..; a key is an fp16 probability, then the complement of the expert's number.
+// One warp: a token's logits over the K chunks c, c + SUM_WARPS, ..., two experts side by side a lane (512 bytes a load).
 template <int VPT>
-__device__ __forceinline__ bool route_token(const MoeFewParams& p, Routing& rt, int t, uint32_t call, Patience& patience) {
-    constexpr int BATCH = 32 / VPT < 8 ? 32 / VPT : 8;          // chunks whose loads are in flight together
-    const int lane = threadIdx.x & 31, e0 = lane * VPT;
-    const bool active = e0 < p.experts;
+__device__ __forceinline__ bool sum_logits(const MoeFewParams& p, int t, int c, uint32_t call, Patience& patience, float* row) {
+    constexpr int BATCH = 32 / VPT < 4 ? 32 / VPT : 4;          // chunks whose loads are in flight together
+    const int lane = threadIdx.x & 31;
     const unsigned long long* src = p.logits + (size_t)t * p.experts;
     const size_t step = (size_t)p.t * p.experts;
-    // The words are read side by side (two experts a lane, 512 bytes a load) ...
-    float* row = rt.logits[(threadIdx.x >> 5) % SUM_WARPS];
     float l[VPT];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) l[i] = 0.f;
-    for (int c0 = 0; c0 < p.router_chunks; c0 += BATCH) {
+    for (; c < p.router_chunks; c += BATCH * SUM_WARPS) {
         unsigned long long v[BATCH][VPT];
         for (;;) {
             bool here = true;
 #pragma unroll
-            for (int c = 0; c < BATCH; ++c) {
-                const unsigned long long* at = src + (size_t)min(c0 + c, p.router_chunks - 1) * step;
+            for (int b = 0; b < BATCH; ++b) {
+                const int cb = c + b * SUM_WARPS;
+                const unsigned long long* at = src + (size_t)(cb < p.router_chunks ? cb : c) * step;
                 if (VPT == 1) {
-                    v[c][0] = ld_word(at + min(lane, p.experts - 1));
+                    v[b][0] = ld_word(at + min(lane, p.experts - 1));
                 } else {
 #pragma unroll
                     for (int i = 0; i < VPT / 2; ++i) {
                         const ulonglong2 w = ld_words(at + 64 * i + 2 * lane);
-                        v[c][2 * i] = w.x;
-                        v[c][VPT == 1 ? 0 : 2 * i + 1] = w.y;
+                        v[b][2 * i] = w.x;
+                        v[b][VPT == 1 ? 0 : 2 * i + 1] = w.y;
                     }
                 }
             }
 #pragma unroll
-            for (int c = 0; c < BATCH; ++c)
+            for (int b = 0; b < BATCH; ++b)
 #pragma unroll
-                for (int i = 0; i < VPT; ++i) here = here && call_of(v[c][i]) == call;
+                for (int i = 0; i < VPT; ++i) here = here && call_of(v[b][i]) == call;
             if (__all_sync(0xffffffffu, here)) break;
             if (!__all_sync(0xffffffffu, patience.more())) return false;
         }
 #pragma unroll
-        for (int c = 0; c < BATCH; ++c)
-            if (c0 + c < p.router_chunks)
+        for (int b = 0; b < BATCH; ++b)
+            if (c + b * SUM_WARPS < p.router_chunks)
 #pragma unroll
-                for (int i = 0; i < VPT; ++i) l[i] += float_of(v[c][i]);
+                for (int i = 0; i < VPT; ++i) l[i] += float_of(v[b][i]);
     }
-    // ... and change places for the softmax
-    if (VPT > 1) {
+    if (VPT == 1) row[lane] = l[0];
 #pragma unroll
-        for (int i = 0; i < VPT / 2; ++i) *reinterpret_cast<float2*>(row + 64 * i + 2 * lane) = make_float2(l[2 * i], l[VPT == 1 ? 0 : 2 * i + 1]);
-        __syncwarp();
+    for (int i = 0; i < VPT / 2; ++i) *reinterpret_cast<float2*>(row + 64 * i + 2 * lane) = make_float2(l[2 * i], l[VPT == 1 ? 0 : 2 * i + 1]);
+    return true;
+}
+
+// One warp: a token's softmax and top-k from its logits' partial sums, as topk_kernel (moe_route.cu) does them, on the same fp16
+// roundings.  Lane l owns experts l * VPT ..; a key is an fp16 probability, then the complement of the expert's number, and
+// lane k < top_k returns the k-th largest.
+template <int VPT>
+__device__ __forceinline__ uint32_t pick(const MoeFewParams& p, const float (&sums)[SUM_WARPS][kFewMaxExperts]) {
+    const int lane = threadIdx.x & 31, e0 = lane * VPT;
+    const bool active = e0 < p.experts;
+    float l[VPT], mx = -65504.0f;
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) l[i] = row[e0 + i];
-        __syncwarp();
-    }
-    float mx = -65504.0f;
+    for (int i = 0; i < VPT; ++i) l[i] = 0.f;
     if (active)
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
+#pragma unroll
+            for (int w = 0; w < SUM_WARPS; ++w) l[i] += sums[w][e0 + i];
             if (p.router_bias != nullptr) l[i] += ld_global_f32(p.router_bias + e0 + i);
             l[i] = __half2float(__float2half_rn(l[i]));
             mx = fmaxf(mx, l[i]);
@@ -317,10 +327,42 @@ __device__ __forceinline__ bool route_token(const MoeFewParams& p, Routing& rt, 
         for (int i = 0; i < VPT; ++i)
             if (key[i] == best) key[i] = 0u;
     }
-    if (lane < p.top_k) {
-        rt.expert[t * p.top_k + lane] = (int)(0xFFFFu - (mine & 0xFFFFu));
-        rt.weight[t * p.top_k + lane] = __half2float(__ushort_as_half((unsigned short)(mine >> 16)));
+    return mine;
+}
+
+// The routing warps together: token t's top-k for everyone. `meet` is their barrier, with its parity.
+template <int VPT, class Meet>
+__device__ __forceinline__ bool route_token(const MoeFewParams& p, Routing& rt, int t, uint32_t call, Patience& patience, Meet meet) {
+    const int w = (threadIdx.x >> 5) - WARP_SUM, lane = threadIdx.x & 31;
+    if (!sum_logits<VPT>(p, t, w, call, patience, rt.logits[w]) || !meet(0)) return false;
+    if (w == 0) {
+        const uint32_t key = pick<VPT>(p, rt.logits);
+        if (lane < p.top_k) st_word(p.routes + t * p.top_k + lane, key, call);
     }
+    return meet(1);     // (the next token's sums go where these were)
+}
+
+// One warp: every token's top-k.
+template <int BATCH>
+__device__ __forceinline__ bool read_routes(const MoeFewParams& p, Routing& rt, uint32_t call, Patience& patience) {
+    const int lane = threadIdx.x & 31, pairs = p.t * p.top_k;
+    unsigned long long v[BATCH];
+    for (;;) {
+        bool here = true;
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) v[i] = ld_word(p.routes + min(32 * i + lane, pairs - 1));
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) here = here && call_of(v[i]) == call;
+        if (__all_sync(0xffffffffu, here)) break;
+        if (!__all_sync(0xffffffffu, patience.more())) return false;
+    }
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+        if (32 * i + lane < pairs) {
+            rt.expert[32 * i + lane] = (int)(0xFFFFu - ((uint32_t)v[i] & 0xFFFFu));
+            rt.weight[32 * i + lane] = __half2float(__ushort_as_half((unsigned short)((uint32_t)v[i] >> 16)));
+        }
+    __syncwarp();
     return true;
 }
 
@@ -399,9 +441,9 @@ moe_few_kernel(const MoeFewParams p) {
     auto sum_bar = [&](uint32_t j) { return bar_base + 8u * (2 * STAGES + 4 + 2 * ITEM_SLOTS + j % SUM_SLOTS); };
     auto sum_free_bar = [&](uint32_t j) { return bar_base + 8u * (2 * STAGES + 4 + 2 * ITEM_SLOTS + SUM_SLOTS + j % SUM_SLOTS); };
     const uint32_t routed_bar = bar_base + 8u * (2 * STAGES + 4 + 2 * ITEM_SLOTS + 2 * SUM_SLOTS);
-    const uint32_t meet_bar = routed_bar + 8;
-    auto merge_bar = [&](uint32_t i) { return meet_bar + 8u * (1 + i); };
-    auto merge_free_bar = [&](uint32_t i) { return meet_bar + 8u * (1 + MMA_WARPS / 2 + i); };
+    const uint32_t meet_bar = routed_bar + 8, sum_meet_bar = routed_bar + 16;
+    auto merge_bar = [&](uint32_t i) { return routed_bar + 8u * (3 + i); };
+    auto merge_free_bar = [&](uint32_t i) { return routed_bar + 8u * (3 + MMA_WARPS / 2 + i); };
     Routing& rt = *reinterpret_cast<Routing*>(smem_raw + (bar_base + 8u * C::kBars - smem_u32(smem_raw)));
 
     const int warp = threadIdx.x >> 5;
@@ -430,6 +472,7 @@ moe_few_kernel(const MoeFewParams p) {
         }
         mbar_init(routed_bar, 1);
         mbar_init(meet_bar, MMA_WARPS);
+        mbar_init(sum_meet_bar, SUM_WARPS);
         mbar_fence_init();
     }
     if (warp == WARP_SUM && lane < 3 && p.fs > 0) tma_prefetch_desc(p.maps + 3 * p.experts + lane);
@@ -448,18 +491,28 @@ moe_few_kernel(const MoeFewParams p) {
 
     const Shape shape(p, C::kRows);
     const int shared_first = shape.groups * shape.tiles1s * shape.chunks1;
-    const int before_routed = p.router_units + shared_first;
+    const int before_shared = p.router_units + p.t, before_routed = before_shared + shared_first;
     const int pairs = p.t * p.top_k;            // the shared expert's pairs come behind them, one per token
     const size_t rows = pairs + p.t;            // of h and the partial sums
     auto wait_routed = [&](int code) { return idle_wait(routed_bar, 0, p.status, code, p.launch_tag); };
+    // A barrier of a role's warps with a limit: a warp that gave a wait up does not come.
+    auto meet_at = [&](uint32_t bar, uint32_t parity, int code) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, code, p.launch_tag)) != 0;
+    };
     auto wait_item = [&](uint32_t j, int code) {
         return mbar_wait(item_bar(j), (j / ITEM_SLOTS) & 1, p.status, code, p.launch_tag);
     };
-    auto read_item = [&](uint32_t addr) {
+    const uint32_t zero = (uint32_t)p.t >> 16;
+    // The item in a slot, which is free for the next.
+    auto take = [&](uint32_t addr, uint32_t bar) {
         const uint4 v = ld_shared_v4(addr);
+        __syncwarp();
+        if (lane == 0) mbar_arrive_after(bar, v.x, zero);
         return make_int4((int)v.x, (int)v.y, (int)v.z, (int)v.w);
     };
-    auto get_item = [&](uint32_t j) { return read_item(item_base + 16u * (j % ITEM_SLOTS)); };
+    auto take_item = [&](uint32_t j) { return take(item_base + 16u * (j % ITEM_SLOTS), free_bar(j)); };
     // K range of an item
     auto k_range = [&](const Item& it, int* k0, int* len) {
         const int kc = it.x == kFirst ? p.kc1 : p.kc2;
@@ -479,14 +532,27 @@ moe_few_kernel(const MoeFewParams p) {
         // ------------------------------------------------------------------------------ tickets, weight loads
         if (lane == 0) {
             uint32_t st = 0, s = 0, ph = 1;
-            bool ok = true, routed = false;
+            bool ok = true, routed = false, lists = false;
             uint32_t sums = 0;
+            auto push_sum = [&](const Item& it) {
+                ok = idle_wait(sum_free_bar(sums), ((sums / SUM_SLOTS) & 1) ^ 1, p.status, kErrProducerWait, p.launch_tag);
+                if (!ok) return;
+                st_shared_v4(sum_base + 16u * (sums % SUM_SLOTS), it.x, it.y, it.z, it.w);
+                mbar_arrive(sum_bar(sums++));
+            };
             for (uint32_t j = 0; ok; ++j) {
                 Item it;
+                for (; ok && ticket >= p.router_units && ticket < before_shared; ticket = atomicAdd(p.head + kFewTicket, 1))
+                    push_sum(make_int4(kRoute, 0, ticket - p.router_units, 0));
+                if (ok && ticket >= before_shared && !lists) {
+                    push_sum(make_int4(kLists, 0, 0, 0));
+                    lists = true;
+                }
+                if (!ok) break;
                 if (ticket < p.router_units) {
                     it = make_int4(kRouter, 0, ticket, 0);
                 } else if (ticket < before_routed) {
-                    const int per = shape.tiles1s * shape.chunks1, r = ticket - p.router_units, e = r / per, i = r - e * per;
+                    const int per = shape.tiles1s * shape.chunks1, r = ticket - before_shared, e = r / per, i = r - e * per;
                     const int c = i / shape.tiles1s;
                     it = make_int4(kFirst, -1 - e, i - c * shape.tiles1s, c);
                 } else {
@@ -504,10 +570,8 @@ moe_few_kernel(const MoeFewParams p) {
                 // the last chunk of a column tile, the last item of a result tile
                 if (it.x == kEnd || (it.x == kFirst && it.w == shape.chunks1 - 1) ||
                     (it.x == kSecond && it.y == rt.n_active - 1 && it.w == shape.chunks2 - 1)) {
-                    ok = idle_wait(sum_free_bar(sums), ((sums / SUM_SLOTS) & 1) ^ 1, p.status, kErrProducerWait, p.launch_tag);
+                    push_sum(it);
                     if (!ok) break;
-                    st_shared_v4(sum_base + 16u * (sums % SUM_SLOTS), it.x, it.y, it.z, it.w);
-                    mbar_arrive(sum_bar(sums++));
                 }
                 if (it.x == kEnd) break;
                 if (it.x == kRouter) {
@@ -545,9 +609,7 @@ moe_few_kernel(const MoeFewParams p) {
         for (uint32_t j = 0; ok; ++j) {
             ok = __all_sync(0xffffffffu, idle_wait(item_bar(j), (j / ITEM_SLOTS) & 1, p.status, kErrMmaWaitFull, p.launch_tag));
             if (!ok) break;
-            const Item it = get_item(j);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(free_bar(j));
+            const Item it = take_item(j);
             if (it.x == kEnd) break;
             if (it.x == kRouter) continue;
             if (it.y >= 0 && !routed) {
@@ -628,18 +690,11 @@ moe_few_kernel(const MoeFewParams p) {
         const uint32_t box = (w >> 2) * BOX_BYTES;      // (fp16: 16 columns a warp)
         bool ok = true, routed = false;
         uint32_t n = 0, s = 0, ph = 0, met = 0;
-        // A barrier of the MMA warps with a limit: a warp that gave a wait up does not come.
-        auto meet = [&] {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(meet_bar);
-            return __all_sync(0xffffffffu, mbar_wait(meet_bar, met++ & 1, p.status, kErrMmaWaitFull, p.launch_tag)) != 0;
-        };
+        auto meet = [&] { return meet_at(meet_bar, met++ & 1, kErrMmaWaitFull); };
         for (uint32_t j = 0;; ++j) {
             ok = ok && __all_sync(0xffffffffu, wait_item(j, kErrMmaWaitFull));
             if (!ok) break;
-            const Item it = get_item(j);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(free_bar(j));
+            const Item it = take_item(j);
             if (it.x == kEnd) break;
             if (it.x != kRouter && it.y >= 0 && !routed) {
                 ok = __all_sync(0xffffffffu, wait_routed(kErrMmaWaitFull));
@@ -708,14 +763,15 @@ moe_few_kernel(const MoeFewParams p) {
             const int groups = (n_rows + 7) >> 3;
             float acc[FP8 ? 2 * NG : NG][4] = {};       // FP8: two tiles of 16 columns for each 8 tokens
             const int n_stages = len / C::kStageK;
+            // A stage is free when what it held has become a sum.  (Freed when its loads had been issued, one call in twenty with 24
+            // tokens multiplied some of the next weights: those that come from L2 are there before the loads.)
+            auto give_back = [&](uint32_t bar, float sum) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive_after(bar, __float_as_uint(sum), zero);
+            };
             auto next_stage = [&] {
                 const bool here = __all_sync(0xffffffffu, mbar_wait(full_bar(s), ph, p.status, kErrMmaWaitFull, p.launch_tag));
                 return here;
-            };
-            auto give_back = [&] {
-                __syncwarp();
-                if (lane == 0) mbar_arrive(empty_bar(s));
-                if (++s == STAGES) { s = 0; ph ^= 1; }
             };
             if (FP8) {
                 // Two groups of four warps take the item's stages in turn, 32 columns a warp: while one group waits and loads, the
@@ -723,38 +779,41 @@ moe_few_kernel(const MoeFewParams p) {
                 // barrier, loads, conversions and MMAs of a stage come one after the other, 540 cycles; so 360.)  Which of the
                 // MMA's 16 rows is which column, and the order of k inside it, are free as long as both operands and the result
                 // agree: rows g and g + 8 are columns 2g and 2g + 1 (their 8-byte pieces lie in banks of their own), a lane
-                // takes 8 consecutive k for two MMAs.  Rows of x that hold no token are not read.
+                // takes 8 consecutive k for two MMAs.  Rows of x that hold no token repeat the last one (nobody takes their sums), and x
+                // is read ahead of the stage's barrier: a group spends 1050 cycles on a stage between waits without either, 860 with both.  Four
+                // chains of MMAs instead of two, and scales and h read before their buffer is free, changed nothing.
                 const int group = w >> 2, c0 = (w & 3) * 32 + 2 * g;
+                const uint32_t w_lo = smem_base + c0 * 128 + (((q >> 1) ^ (c0 & 7)) << 4) + 8 * (q & 1);
                 const uint32_t scales = xb + C::kRows * C::kXStride + ((w >> 1) & 1) * 32;
+                const uint32_t x_row = xb + min(g, n_rows - 1) * C::kXStride + 16 * q;
                 for (int i = group; i < n_stages; i += 2) {
                     const bool wrap = s + i >= (uint32_t)STAGES;
                     const uint32_t si = s + i - (wrap ? STAGES : 0);
+                    uint4 x[4];
+                    auto load_x = [&](int u) {
+#pragma unroll
+                        for (int b = 0; b < 4; ++b)
+                            x[b] = ld_shared_v4((u == 0 ? x_row : xb + min(8 * u + g, n_rows - 1) * C::kXStride + 16 * q) + 2 * (i * 128 + b * 32));
+                    };
+                    load_x(0);
                     ok = __all_sync(0xffffffffu, mbar_wait(full_bar(si), ph ^ (wrap ? 1u : 0u), p.status, kErrMmaWaitFull, p.launch_tag));
                     if (!ok) break;
                     uint2 l[2][4], h[2][4];
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
-                        const int col = c0 + 16 * t;            // (64 columns to a box of 8 KB)
-                        const uint32_t row = smem_base + si * STAGE_BYTES + col * 128 + 8 * (q & 1);
+                        // (64 columns to a box of 8 KB; 16-byte pieces are swizzled by their column modulo 8)
 #pragma unroll
                         for (int b = 0; b < 4; ++b) {
-                            l[t][b] = ld_shared_v2(row + (((2 * b + (q >> 1)) ^ (col & 7)) << 4));
-                            h[t][b] = ld_shared_v2(row + 128 + (((2 * b + (q >> 1)) ^ ((col + 1) & 7)) << 4));
+                            l[t][b] = ld_shared_v2(((w_lo + si * STAGE_BYTES) ^ (b << 5)) + t * 2048);
+                            h[t][b] = ld_shared_v2((((w_lo + si * STAGE_BYTES) ^ (b << 5)) ^ 16) + 128 + t * 2048);
                         }
                     }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(empty_bar(si));
                     const float sc = __uint_as_float(ld_shared_u32(scales + i * 4));
 #pragma unroll
                     for (int u = 0; u < NG; ++u) {
                         if (u >= groups) break;
                         float part[2][4] = {};
-                        uint4 x[4];
-#pragma unroll
-                        for (int b = 0; b < 4; ++b) {
-                            x[b] = make_uint4(0, 0, 0, 0);
-                            if (8 * u + g < n_rows) x[b] = ld_shared_v4(xb + (8 * u + g) * C::kXStride + 2 * (i * 128 + b * 32 + 8 * q));
-                        }
+                        if (u > 0) load_x(u);
                         auto convert = [](uint32_t lo, uint32_t hi, uint32_t (&a)[4]) {
                             a[0] = f16x2_of_e4m3x2((uint16_t)lo);
                             a[1] = f16x2_of_e4m3x2((uint16_t)hi);
@@ -779,6 +838,7 @@ moe_few_kernel(const MoeFewParams p) {
                         for (int t = 0; t < 2; ++t)
 #pragma unroll
                             for (int v = 0; v < 4; ++v) acc[2 * u + t][v] = fmaf(sc, part[t][v], acc[2 * u + t][v]);
+                        if (u == 0) give_back(empty_bar(si), part[0][0] + part[1][0]);
                     }
                 }
                 s += n_stages;
@@ -801,12 +861,17 @@ moe_few_kernel(const MoeFewParams p) {
                 } else {
                     ok = ok && __all_sync(0xffffffffu, mbar_wait(merge_bar(w & 3), n & 1, p.status, kErrMmaWaitFull, p.launch_tag));
                     if (ok) {
+                        uint32_t seen = 0;
 #pragma unroll
                         for (int i = 0; i < 2 * NG; ++i)
 #pragma unroll
-                            for (int v = 0; v < 4; ++v) acc[i][v] += __uint_as_float(ld_shared_u32(mine + (4 * i + v) * 128));
+                            for (int v = 0; v < 4; ++v) {
+                                const uint32_t other = ld_shared_u32(mine + (4 * i + v) * 128);
+                                acc[i][v] += __uint_as_float(other);
+                                seen |= other;
+                            }
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(merge_free_bar(w & 3));
+                        if (lane == 0) mbar_arrive_after(merge_free_bar(w & 3), seen, zero);
                     }
                 }
             } else {
@@ -826,12 +891,13 @@ moe_few_kernel(const MoeFewParams p) {
 #pragma unroll
                         for (int u = 0; u < NG; ++u)
                             if (u < groups) ldmatrix_x4(xa + u * 8 * C::kXStride + v * 64, x[v][u]);
-                    give_back();
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
                         for (int u = 0; u < NG; ++u)
                             if (u < groups) mma_f16(acc[u], a[kk], x[kk >> 1][u][2 * (kk & 1)], x[kk >> 1][u][2 * (kk & 1) + 1]);
+                    give_back(empty_bar(s), acc[0][0]);
+                    if (++s == STAGES) { s = 0; ph ^= 1; }
                 }
             }
             if (ok && (!FP8 || w < 4)) {
@@ -862,31 +928,33 @@ moe_few_kernel(const MoeFewParams p) {
         }
         lost = !ok;
     } else {
-        // ------------------------------------------------------------------------------ routing
+        // ------------------------------------------------------------------------------ routing, sums of complete tiles
         const int w = warp - WARP_SUM;
-        Patience patience(p.status, p.launch_tag);
         bool ok = true;
-        for (int t = w; t < p.t && ok; t += SUM_WARPS) {
-            if (p.experts <= 32) ok = route_token<1>(p, rt, t, call, patience);
-            else if (p.experts == 64) ok = route_token<2>(p, rt, t, call, patience);
-            else if (p.experts == 128) ok = route_token<4>(p, rt, t, call, patience);
-            else ok = route_token<8>(p, rt, t, call, patience);
-        }
-        ok = named_barrier_all(BAR_SUM, 32 * SUM_WARPS, ok);
-        if (ok && w == 0) build_lists<C::kRows>(p, rt);
-        named_barrier(BAR_SUM, 32 * SUM_WARPS);
-        if (ok && w == 0 && lane == 0) mbar_arrive(routed_bar);
-        // ------------------------------------------------------------------------------ sums of complete tiles
+        auto meet = [&](uint32_t parity) { return meet_at(sum_meet_bar, parity, kErrEpilogueWait); };
         for (uint32_t j = 0; ok; ++j) {
             ok = __all_sync(0xffffffffu, idle_wait(sum_bar(j), (j / SUM_SLOTS) & 1, p.status, kErrEpilogueWait, p.launch_tag));
             if (!ok) break;
-            const Item it = read_item(sum_base + 16u * (j % SUM_SLOTS));
-            __syncwarp();
-            if (lane == 0) mbar_arrive(sum_free_bar(j));
+            const Item it = take(sum_base + 16u * (j % SUM_SLOTS), sum_free_bar(j));
             if (it.x == kEnd) break;
-            Patience wait(p.status, p.launch_tag);
-            if (it.x == kFirst) {
+            if (it.x == kRoute) {
+                Patience wait(p.status, p.launch_tag);
+                if (p.experts <= 32) ok = route_token<1>(p, rt, it.z, call, wait, meet);
+                else if (p.experts == 64) ok = route_token<2>(p, rt, it.z, call, wait, meet);
+                else if (p.experts == 128) ok = route_token<4>(p, rt, it.z, call, wait, meet);
+                else ok = route_token<8>(p, rt, it.z, call, wait, meet);
+            } else if (it.x == kLists) {
+                if (w == 0) {
+                    Patience wait(p.status, p.launch_tag);
+                    ok = pairs <= 32 ? read_routes<1>(p, rt, call, wait) : read_routes<MAX_PAIRS / 32>(p, rt, call, wait);
+                    if (ok) build_lists<C::kRows>(p, rt);
+                    if (ok && lane == 0) mbar_arrive(routed_bar);
+                } else {
+                    ok = __all_sync(0xffffffffu, wait_routed(kErrEpilogueWait));
+                }
+            } else if (it.x == kFirst) {
                 // a warp per row, two columns a lane
+                Patience wait(p.status, p.launch_tag);
                 const int n_rows = pair_count(it), first = first_pair(it);
                 for (int r = w; r < n_rows && ok; r += SUM_WARPS) {
                     const unsigned long long* src = p.part1 + (size_t)(first + r) * 2 * p.width + it.z * 128 + 2 * lane;
@@ -900,6 +968,7 @@ moe_few_kernel(const MoeFewParams p) {
                 // two warps per token, two columns a lane; the words of two chunks of every expert and of the shared one are in flight
                 const int col = it.z * 128 + (w & 1) * 64 + 2 * lane;
                 const size_t step = rows * p.d;
+                Patience wait(p.status, p.launch_tag);
                 for (int t = w >> 1; t < p.t && it.z * 128 + (w & 1) * 64 < p.d && ok; t += SUM_WARPS / 2) {
                     float2 y[kFewMaxTopK + 1];
 #pragma unroll

@@ -23,6 +23,7 @@ struct MoeFewParams {
     // workspace: words of 32 bits of data and the call's number
     int* head;                      // kFewHeadWords
     unsigned long long* logits;     // [router_chunks][t][experts] partial sums
+    unsigned long long* routes;     // [t][top_k] fp16 probability | 0xFFFF - expert
     unsigned long long* part1;      // [chunks1][pairs][2 * width] partial sums of gate | up, 64 + 64 columns per tile
     unsigned long long* h;          // [pairs][width / 2] two fp16 values each
     unsigned long long* part2;      // [chunks2][pairs][d] partial sums
@@ -42,8 +43,8 @@ inline int moe_few_rows(int t) { return t <= 8 ? 8 : 16; }
 inline int moe_few_token_groups(int t) { return (t + 15) / 16; }
 // Largest K chunk: its two operand buffers leave room for the weight stages.
 constexpr int kFewMaxChunk = 1024;
-// K of a router unit: whole rounds of the eight MMA warps; longer for many experts, whose sums every CTA has to gather.
-inline int moe_few_router_chunk(int experts) { return experts <= 64 ? 512 : experts == 128 ? 1024 : 2048; }
+// K of a router unit: a round of the eight MMA warps.
+constexpr int kFewRouterChunk = 512;
 
 cudaError_t moe_few_launch(const MoeFewParams& p, bool fp8, int num_sms, cudaStream_t stream);
 

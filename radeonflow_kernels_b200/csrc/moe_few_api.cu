@@ -24,7 +24,7 @@ size_t align_up(size_t v) { return (v + 255) / 256 * 256; }
 // What a call of t tokens needs: K chunks, and where the parts of the workspace lie.
 struct Plan {
     int kc1, kc2, router_kc, router_chunks;
-    size_t logits, part1, h, part2, bytes;
+    size_t logits, routes, part1, h, part2, bytes;
 };
 
 // The K chunk for `tiles` column tiles: least rounds of items over the SMs x (chunk + what an item costs beside its weights, about
@@ -52,12 +52,13 @@ Plan make_plan(const RfMoeFewConfig& c, int t) {
     Plan p;
     p.kc1 = choose_chunk((hit * c.d_expert + fs) / 64, c.d_hidden, rf::kFewMaxChunk, num_sms);
     p.kc2 = choose_chunk((hit + (fs > 0)) * ((c.d_hidden + 127) / 128), c.d_expert, rf::kFewMaxChunk, num_sms);
-    p.router_kc = rf::moe_few_router_chunk(c.n_routed_experts);
+    p.router_kc = rf::kFewRouterChunk;
     p.router_chunks = (c.d_hidden + p.router_kc - 1) / p.router_kc;
     const size_t chunks1 = (d + p.kc1 - 1) / p.kc1, chunks2 = ((size_t)width + p.kc2 - 1) / p.kc2;
     size_t b = rf::kFewHeadWords * sizeof(int);
     auto take = [&](size_t words) { const size_t at = b; b += align_up(words * 8); return at; };
     p.logits = take((size_t)p.router_chunks * t * c.n_routed_experts);
+    p.routes = take((size_t)t * c.n_experts_per_token);
     p.part1 = take(chunks1 * pairs * 2 * width);
     p.h = take(pairs * width / 2);
     p.part2 = take(chunks2 * pairs * d);
@@ -229,6 +230,7 @@ int rf_moe_few_forward(RfMoeFew* few, const void* x, int n_tokens, void* out, vo
     p.out = out;
     p.head = reinterpret_cast<int*>(ws);
     p.logits = reinterpret_cast<unsigned long long*>(ws + plan.logits);
+    p.routes = reinterpret_cast<unsigned long long*>(ws + plan.routes);
     p.part1 = reinterpret_cast<unsigned long long*>(ws + plan.part1);
     p.h = reinterpret_cast<unsigned long long*>(ws + plan.h);
     p.part2 = reinterpret_cast<unsigned long long*>(ws + plan.part2);

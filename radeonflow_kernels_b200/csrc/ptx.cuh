@@ -74,6 +74,10 @@ __device__ __forceinline__ void mbar_expect_tx_only(uint32_t bar, uint32_t bytes
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// An arrival that gives back shared memory which this warp has read: it may overtake loads that were issued before it and have not
+// returned, and the next contents then reach them.  So its address is made to depend on `seen`, made of what was loaded, through a
+// mask that is zero at run time without the compiler knowing.
+__device__ __forceinline__ void mbar_arrive_after(uint32_t bar, uint32_t seen, uint32_t zero) { mbar_arrive(bar + (seen & zero)); }
 __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(

@@ -167,6 +167,18 @@ def test_nan_stays_in_its_token(fp8):
     assert gemm.device_status() == 0
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("t", [8, 16, 24, 32])
+def test_same_bits_every_time(t, fp8):
+    """Weights that stay in L2, so that a stage of them is refilled as soon as it is given back: a warp that still read it when it
+    gave it back would multiply some of the next one's (one call in twenty did)."""
+    x, w, cfg, _ = make(t, 1024, 512, 32, 4, 1, fp8, seed=t)
+    layer = moe_few.FewTokenMoE(w, cfg)
+    runs = torch.stack([layer.forward(x) for _ in range(400)])
+    assert not (runs != runs[0]).any()
+    assert gemm.device_status() == 0
+
+
 def test_beside_the_layer():
     """The same layer through moe_forward, whose intermediate roundings (fp16 gate, up, outputs of the experts) are more: the
     layer's own tolerance, 1e-2 absolute and relative.  Both choose on the logits that they compute themselves."""
