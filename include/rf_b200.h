@@ -564,7 +564,8 @@ int rf_moe_few_workspace_alloc(size_t bytes, void **workspace);
 int rf_moe_few_workspace_free(void *workspace);
 /* *id = 0: the stream is not being captured; else a number of its own for each capture.              */
 int rf_stream_capture_id(rf_stream_t stream, unsigned long long *id);
-/* x fp16 [n_tokens, d_hidden] -> out fp16 [n_tokens, d_hidden], 16-byte aligned, workspace 256.  One kernel, asynchronous.  */
+/* x fp16 [n_tokens, d_hidden] -> out fp16 [n_tokens, d_hidden], 16-byte aligned, workspace 256.  One kernel, asynchronous.  x and
+ * out must not overlap (RF_ERR_UNSUPPORTED).                                                         */
 int rf_moe_few_forward(RfMoeFew *few, const void *x, int n_tokens, void *out, void *workspace, size_t workspace_bytes,
                        rf_stream_t stream);
 

@@ -4,6 +4,7 @@
 #include "host_util.h"
 #include "moe_few.h"
 
+#include <cstdint>
 #include <cstdio>
 #include <new>
 #include <vector>
@@ -154,9 +155,9 @@ int rf_moe_few_create(const RfMoeFewConfig* config, const void* router_weight, c
 
 int rf_moe_few_destroy(RfMoeFew* few) {
     if (!few) return RF_OK;
-    const cudaError_t e = cudaFree(few->maps);
+    const int rc = rf_moe_few_workspace_free(few->maps);       // (may come from a garbage collector during a capture)
     delete few;
-    return e == cudaSuccess ? RF_OK : RF_ERR_CUDA;
+    return rc;
 }
 
 size_t rf_moe_few_workspace_bytes(const RfMoeFewConfig* config, int n_tokens) {
@@ -213,6 +214,9 @@ int rf_moe_few_forward(RfMoeFew* few, const void* x, int n_tokens, void* out, vo
     if (n_tokens == 0) return RF_OK;
     if (!x || !out || !workspace) return RF_ERR_NULL_POINTER;
     if (rf::misaligned({x, out}, 16) || rf::misaligned({workspace}, 256)) return RF_ERR_MISALIGNED;
+    // (x is read until the kernel's end)
+    const uintptr_t xa = reinterpret_cast<uintptr_t>(x), oa = reinterpret_cast<uintptr_t>(out);
+    if ((xa < oa ? oa - xa : xa - oa) < (uintptr_t)n_tokens * few->cfg.d_hidden * 2) return RF_ERR_UNSUPPORTED;
     int dev = -1;
     if (cudaGetDevice(&dev) != cudaSuccess || dev != few->device) return RF_ERR_UNSUPPORTED;
     const RfMoeFewConfig& c = few->cfg;

@@ -53,8 +53,6 @@ class FewTokenMoE:
         d, f, e = (int(config[k]) for k in ("d_hidden", "d_expert", "n_routed_experts"))
         n_shared = int(config["n_shared_experts"])
         self._handle = None
-        self._capture = ctypes.c_ulonglong()
-        self._capture_ref = ctypes.byref(self._capture)
         self.fp8 = "experts.gate_up.weight" in weights
         self.config = _lib.RfMoeFewConfig(d, f, e, int(config["n_experts_per_token"]), n_shared, int(self.fp8))
         self.d_hidden, self._held, self._sizes = d, {}, {}
@@ -123,8 +121,9 @@ class FewTokenMoE:
         size = self._sizes.get(n_tokens)
         if size is None:
             size = self._sizes[n_tokens] = L.rf_moe_few_workspace_bytes(ctypes.byref(self.config), n_tokens)
-        _lib.check(L.rf_stream_capture_id(stream, self._capture_ref), "rf_stream_capture_id")
-        key = (self.device.index, stream, self._capture.value)
+        capture = ctypes.c_ulonglong()          # (of this call: another thread's may come in between)
+        _lib.check(L.rf_stream_capture_id(stream, ctypes.byref(capture)), "rf_stream_capture_id")
+        key = (self.device.index, stream, capture.value)
         ws = self._held.get(key)
         if ws is None or ws[-1].size < size:
             shared = _workspaces.get(key)
@@ -143,7 +142,8 @@ class FewTokenMoE:
         self._held.clear()
 
     def forward(self, x, out=None):
-        """x fp16 [..., d_hidden], 1 to 32 tokens -> out, same shape.  Enqueues one kernel on the current stream."""
+        """x fp16 [..., d_hidden], 1 to 32 tokens -> out, same shape (given, it must not overlap x).  Enqueues one kernel on the
+        current stream."""
         if not (x.is_cuda and x.dtype == torch.float16 and x.is_contiguous() and x.device == self.device):
             raise ValueError("moe: input must be a contiguous CUDA fp16 tensor on the weights' device (there is no CPU path)")
         self._check_device("the input")
@@ -156,6 +156,8 @@ class FewTokenMoE:
             out = torch.empty_like(x)
         elif not (out.dtype == torch.float16 and out.shape == x.shape and out.is_contiguous() and out.device == x.device):
             raise ValueError("moe: out must be a contiguous fp16 tensor like the input")
+        elif abs(out.data_ptr() - x.data_ptr()) < 2 * x.numel():
+            raise ValueError("moe: out must not overlap the input, which is read until the kernel's end")
         if n_tokens == 0:
             return out
         stream = _lib.current_stream()

@@ -9,13 +9,14 @@ every step, and 40 more additions of partial sums:
     dy <= sum dh |Wd| + s(f) sum |h||Wd|;  dout <= u |out| + 2^-25 + (1 + 2^-20) sum_i p_i dy_i
 """
 import ctypes
+import threading
 
 import numpy as np
 import pytest
 import torch
 
 from oracle import moe as o
-from radeonflow_kernels_b200 import gemm, moe, moe_few, quant
+from radeonflow_kernels_b200 import _lib, gemm, moe, moe_few, quant
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -266,3 +267,39 @@ def test_weights_are_read_at_every_call():
     dense = {n: [m[0], m[1], -2 * m[2]] for n, m in dense.items()}
     ref, tol, _ = reference(x, w, cfg, dense)
     check(layer.forward(x), ref, tol)
+
+
+def test_out_that_overlaps_the_input_is_refused():
+    x, w, cfg, _ = make(3, 256, 128, 8, 2, 1, False, seed=1)
+    layer = moe_few.FewTokenMoE(w, cfg)
+    both = torch.cat([x, x])
+    for out in (both[:3], both[1:4], both[2:5]):
+        with pytest.raises(ValueError, match="overlap"):
+            layer.forward(both[:3], out=out)
+    ws = layer._workspace(3, torch.cuda.current_stream().cuda_stream)
+    assert _lib.lib().rf_moe_few_forward(layer._handle, both.data_ptr(), 3, both[2:].data_ptr(), ws.ptr, ws.size, 0) == 7
+    assert torch.equal(layer.forward(both[:3], out=both[3:]), layer.forward(x))
+
+
+def test_host_threads_at_once():
+    """One layer, called from threads with a stream each."""
+    x, w, cfg, _ = make(20, 512, 256, 16, 4, 1, False, seed=2)
+    layer = moe_few.FewTokenMoE(w, cfg)
+    inputs = [x[i:i + 5].contiguous() for i in range(0, 20, 5)]
+    want = [layer.forward(v) for v in inputs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(100):
+                if not torch.equal(layer.forward(inputs[i]), want[i]):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    assert gemm.device_status() == 0

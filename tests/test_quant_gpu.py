@@ -104,7 +104,7 @@ def test_special_values(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("m,f", [(1, 128), (5, 384), (131, 2048)])
+@pytest.mark.parametrize("m,f", [(1, 128), (5, 384), (131, 2048), (1201, 640), (1024, 768)])
 def test_swiglu(dtype, m, f):
     gu = data((m, 2 * f), dtype, m + f).clamp_(-60, 60)
     gu = torch.cat([gu, gu[:, :8]], 1)[:, :2 * f]               # rows 2f + 8 apart
@@ -113,6 +113,31 @@ def test_swiglu(dtype, m, f):
     h = x[:, :f] / (1 + np.exp(-x[:, :f])) * x[:, f:]
     hb = blocks_of(h)
     check(q, s, hb, np.abs(hb).max(-1), slack=2.0 ** -21)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k,pad", [(640, 0), (640, 3), (384, 8), (128, 0), (1024, 0)])
+def test_long_calls_are_short_ones(dtype, k, pad):
+    """Long calls reduce four blocks together: the same bits as calls of a few rows, which take one block at a time.  With blocks that
+    run over the ends of rows, a rest of one to three blocks, special values in single blocks, and (pad 3) rows at odd addresses."""
+    m = 40003 if k == 128 else 8191
+    x = data((m, k + pad), dtype, k)[:, pad:]
+    x[5, 129 % k], x[77, k - 1], x[m - 1, 0] = float("nan"), float("inf"), float("nan")
+    x[100:103] = 0
+    rows = torch.randint(0, m, (m + 2,), device=DEV, dtype=torch.int32)
+    pieces = list(range(0, m, 500))
+
+    def bits(*calls):
+        return torch.cat([q.view(torch.uint8) for q, _ in calls]), torch.cat([s.view(torch.int32) for _, s in calls])
+
+    for got, want in ((bits(quant.fp8_quantize(x)), bits(*(quant.fp8_quantize(x[i:i + 500]) for i in pieces))),
+                      (bits(quant.fp8_quantize(x, rows=rows)),
+                       bits(*(quant.fp8_quantize(x, rows=rows[i:i + 500]) for i in range(0, m + 2, 500))))):
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    if k % 256 == 0:
+        x = x.clamp(-60, 60)
+        got, want = bits(quant.fp8_swiglu_quantize(x)), bits(*(quant.fp8_swiglu_quantize(x[i:i + 500]) for i in pieces))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
