@@ -77,7 +77,8 @@ struct Cfg {
     // a router unit's partial sums of every MMA warp; later the sums that one group of them hands to the other
     static constexpr int kRedBytes = MMA_WARPS * 16 * kRows * 4;
     static_assert(kRedBytes == MMA_WARPS / 2 * 2 * NG * 4 * 128, "both uses");
-    static constexpr int kStages = NG == 1 ? 11 : 8;
+    static constexpr int kStages = few_stages(FP8, NG);
+    static_assert(!FP8 || kStages % 2 == 0, "two groups, each with slots of its own");
     static constexpr int kBars = 2 * kStages + 4 + 2 * ITEM_SLOTS + 2 * SUM_SLOTS + 3 + MMA_WARPS;
     static constexpr int kSmemBytes = kStages * STAGE_BYTES + 2 * kXBytes + kRedBytes + (ITEM_SLOTS + SUM_SLOTS) * 16 + kBars * 8 +
                                       (int)sizeof(Routing) + 1024;
@@ -775,8 +776,8 @@ moe_few_kernel(const MoeFewParams p) {
                 return here;
             };
             if (FP8) {
-                // Two groups of four warps take the item's stages in turn, 32 columns a warp: while one group waits and loads, the
-                // other multiplies, and a row of x is read by half as many warps.  (All eight on every stage, 16 columns each:
+                // Two groups of four warps take the item's stages in turn (by their slots of the ring, few_first_stage), 32 columns a
+                // warp: while one group waits and loads, the other multiplies, and a row of x is read by half as many warps.  (All eight on every stage, 16 columns each:
                 // barrier, loads, conversions and MMAs of a stage come one after the other, 540 cycles; so 360.)  Which of the
                 // MMA's 16 rows is which column, and the order of k inside it, are free as long as both operands and the result
                 // agree: rows g and g + 8 are columns 2g and 2g + 1 (their 8-byte pieces lie in banks of their own), a lane
@@ -787,7 +788,7 @@ moe_few_kernel(const MoeFewParams p) {
                 const uint32_t w_lo = smem_base + c0 * 128 + (((q >> 1) ^ (c0 & 7)) << 4) + 8 * (q & 1);
                 const uint32_t scales = xb + C::kRows * C::kXStride + ((w >> 1) & 1) * 32;
                 const uint32_t x_row = xb + min(g, n_rows - 1) * C::kXStride + 16 * q;
-                for (int i = group; i < n_stages; i += 2) {
+                for (int i = few_first_stage(group, (int)s); i < n_stages; i += 2) {
                     const bool wrap = s + i >= (uint32_t)STAGES;
                     const uint32_t si = s + i - (wrap ? STAGES : 0);
                     uint4 x[4];

@@ -46,6 +46,14 @@ constexpr int kFewMaxChunk = 1024;
 // K of a router unit: a round of the eight MMA warps.
 constexpr int kFewRouterChunk = 512;
 
+// The ring of weight stages, for items of 8 * ng token rows: what fits beside the operand buffers.  FP8 stages are taken in turn by two
+// groups of MMA warps, and a group waits for its own stages only.  A wait on a stage's barrier knows odd phases from even ones
+// and nothing else: whoever has not seen the phase before would take "not yet there" for "there".  So a slot of the ring
+// belongs to one group for good, which an even number of slots makes possible.
+__host__ __device__ constexpr int few_stages(bool fp8, int ng) { return ng > 1 ? 8 : fp8 ? 10 : 11; }
+// The first stage of an item that is `group`'s, where stage 0 lies in slot s; from there every other one is.
+__host__ __device__ constexpr int few_first_stage(int group, int s) { return (group ^ s) & 1; }
+
 cudaError_t moe_few_launch(const MoeFewParams& p, bool fp8, int num_sms, cudaStream_t stream);
 
 }  // namespace rf
