@@ -21,7 +21,27 @@ bool load_encode() {
     g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
     return true;
 }
+
+// What `enqueue` puts on a stream of its own is done when this returns.
+template <class Enqueue>
+cudaError_t on_own_stream(Enqueue enqueue) {
+    cudaStream_t s = nullptr;
+    cudaError_t e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
+    if (e != cudaSuccess) return e;
+    e = enqueue(s);
+    const cudaError_t done = cudaStreamSynchronize(s);
+    cudaStreamDestroy(s);
+    return e != cudaSuccess ? e : done;
+}
 }  // namespace
+
+cudaError_t upload(void* dst, const void* src, size_t bytes) {
+    return on_own_stream([&](cudaStream_t s) { return cudaMemcpyAsync(dst, src, bytes, cudaMemcpyHostToDevice, s); });
+}
+
+cudaError_t upload_zeroes(void* dst, size_t bytes) {
+    return on_own_stream([&](cudaStream_t s) { return cudaMemsetAsync(dst, 0, bytes, s); });
+}
 
 DeviceState* device_state() {
     int dev = 0;
@@ -39,7 +59,7 @@ DeviceState* device_state() {
     }
     st->num_sms = prop.multiProcessorCount;
     if (cudaMalloc(&st->status, sizeof(int) * kStatusWords) != cudaSuccess) return nullptr;
-    if (cudaMemset(st->status, 0, sizeof(int) * kStatusWords) != cudaSuccess) return nullptr;
+    if (upload_zeroes(st->status, sizeof(int) * kStatusWords) != cudaSuccess) return nullptr;
     if (!load_encode()) return nullptr;
     st->init = true;
     return st;

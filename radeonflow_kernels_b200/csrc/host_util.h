@@ -54,6 +54,12 @@ unsigned next_streamk_epoch();
 // freeing and re-allocating; synchronises the device when it grows).
 void* device_scratch(size_t bytes, int slot = kScratchGemm);
 
+// Copies host memory to the device and waits for it.  (cudaMemcpy from pageable memory may return before the copy has arrived, and
+// what it is ordered with is the legacy default stream: a kernel on a non-blocking stream could read what was there before.)
+cudaError_t upload(void* dst, const void* src, size_t bytes);
+// The same for zeroes; cudaMemset waits for nothing at all.
+cudaError_t upload_zeroes(void* dst, size_t bytes);
+
 // 2-D row-major tensor map: `rows` x `cols` elements of `elem_bytes`, row
 // pitch `pitch_bytes`; box = box_rows x box_cols; 128-byte swizzle when
 // `swizzle128`.  dtype is one of CU_TENSOR_MAP_DATA_TYPE_*.

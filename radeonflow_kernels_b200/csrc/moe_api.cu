@@ -105,7 +105,7 @@ const CUtensorMap* weight_maps(const void* const* ptrs, int count, int rows, int
     m.dev_maps = nullptr;
     m.last_call = g_map_call;
     if (cudaMalloc(&m.dev_maps, sizeof(CUtensorMap) * count) != cudaSuccess) return nullptr;
-    if (cudaMemcpy(m.dev_maps, host.data(), sizeof(CUtensorMap) * count, cudaMemcpyHostToDevice) != cudaSuccess) {
+    if (rf::upload(m.dev_maps, host.data(), sizeof(CUtensorMap) * count) != cudaSuccess) {
         cudaFree(m.dev_maps);
         return nullptr;
     }

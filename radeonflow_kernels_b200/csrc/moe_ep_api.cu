@@ -176,7 +176,7 @@ int rf_moe_ep_create(const RfMoeEpConfig* c, RfMoeEp** out) {
     ep->h = reinterpret_cast<__half*>(L + o_h);
     ep->sort_scratch = L + o_sort;
     const int so[2] = {0, c->n_tokens};
-    if (cudaMemcpy(ep->single_offsets, so, sizeof(so), cudaMemcpyHostToDevice) != cudaSuccess) {
+    if (rf::upload(ep->single_offsets, so, sizeof(so)) != cudaSuccess) {
         release(ep);
         return RF_ERR_CUDA;
     }

@@ -143,8 +143,8 @@ int rf_moe_few_create(const RfMoeFewConfig* config, const void* router_weight, c
     }
     few->maps = reinterpret_cast<CUtensorMap*>(dev);
     few->scales = reinterpret_cast<const float**>(dev + map_bytes);
-    if (cudaMemcpy(dev, maps.data(), map_bytes, cudaMemcpyHostToDevice) != cudaSuccess ||
-        cudaMemcpy(dev + map_bytes, scales.data(), scale_bytes, cudaMemcpyHostToDevice) != cudaSuccess) {
+    if (rf::upload(dev, maps.data(), map_bytes) != cudaSuccess ||
+        rf::upload(dev + map_bytes, scales.data(), scale_bytes) != cudaSuccess) {
         cudaFree(dev);
         delete few;
         return RF_ERR_CUDA;
@@ -173,12 +173,8 @@ int rf_moe_few_workspace_alloc(size_t bytes, void** out) {
     cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
     if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return RF_ERR_CUDA;
     void* p = nullptr;
-    cudaStream_t s = nullptr;
     cudaError_t e = cudaMalloc(&p, bytes);
-    if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
-    if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, bytes, s);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-    if (s) cudaStreamDestroy(s);
+    if (e == cudaSuccess) e = rf::upload_zeroes(p, bytes);
     if (e != cudaSuccess) {
         cudaGetLastError();
         if (p) cudaFree(p);

@@ -84,3 +84,13 @@ def test_dependent_launches_wait():
             assert body.count("griddep_wait()") == 1, (f, name)
     s = _text(os.path.join(CSRC, "moe_route.cu"))
     assert re.search(r"launch\(sort_count_kernel, [^;]*?, stream, false,", s) and "tile_list_kernel<<<" in s
+
+
+def test_tables_have_arrived_before_anyone_is_told_of_them():
+    """What the host writes for kernels of any stream goes through `upload`, which waits for the copy: cudaMemcpy from pageable memory
+    and cudaMemset may return before, and a non-blocking stream is ordered behind neither."""
+    for name in ("moe_few_api.cu", "moe_api.cu", "moe_ep_api.cu"):
+        s = _text(os.path.join(CSRC, name))
+        assert "rf::upload(" in s and not re.search(r"cudaMemcpy\w*\([^;]*HostToDevice", s), name
+    s = _text(os.path.join(CSRC, "host_util.cu"))
+    assert "cudaMemset(" not in s and "cudaStreamNonBlocking" in s and s.index("e = enqueue(s)") < s.index("cudaStreamSynchronize(s)")

@@ -303,3 +303,22 @@ def test_host_threads_at_once():
         t.join()
     assert not wrong
     assert gemm.device_status() == 0
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_first_call_on_a_stream_of_its_own(fp8):
+    """A layer is made and called at once on a stream that is ordered behind nothing, then freed: the next one's tables lie where
+    its tables lay."""
+    made = [make(4, 512, 256, 16, 4, 1, fp8, seed=20 + i) for i in range(2)]
+    want = [reference(x, w, cfg, dense) for x, w, cfg, dense in made]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for i in range(40):
+        x, w, cfg, _ = made[i % 2]
+        layer = moe_few.FewTokenMoE(w, cfg)
+        with torch.cuda.stream(side):
+            got = layer.forward(x)
+        side.synchronize()
+        check(got, *want[i % 2][:2])
+        del layer
+    assert gemm.device_status() == 0
