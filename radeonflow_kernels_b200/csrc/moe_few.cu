@@ -477,7 +477,6 @@ moe_few_kernel(const MoeFewParams p) {
         mbar_init(sum_meet_bar, SUM_WARPS);
         mbar_fence_init();
     }
-    if (warp == WARP_SUM && lane < 3 && p.fs > 0) tma_prefetch_desc(p.maps + 3 * p.experts + lane);
     griddep_wait();
     // The number of this call: zero, which fresh words hold, is left out.  (A word that no call has written for the 2^32 - 1 calls
     // before this one could pass for this call's.)
@@ -536,6 +535,7 @@ moe_few_kernel(const MoeFewParams p) {
             uint32_t st = 0, s = 0, ph = 1;
             bool ok = true, routed = false, lists = false;
             uint32_t sums = 0;
+            const CUtensorMap* acquired = nullptr;
             auto push_sum = [&](const Item& it) {
                 ok = idle_wait(sum_free_bar(sums), ((sums / SUM_SLOTS) & 1) ^ 1, p.status, kErrProducerWait, p.launch_tag);
                 if (!ok) return;
@@ -585,6 +585,11 @@ moe_few_kernel(const MoeFewParams p) {
                 k_range(it, &k0, &len);
                 const CUtensorMap* m0 = p.maps + 3 * e + (it.x == kFirst ? 0 : 2);
                 const CUtensorMap* m1 = it.x == kFirst ? m0 + 1 : m0;
+                if (m0 != acquired) {
+                    tma_acquire_desc(m0);
+                    if (m1 != m0) tma_acquire_desc(m1);
+                    acquired = m0;
+                }
                 const int n0 = it.x == kFirst ? it.z * 64 : it.z * 128, n1 = it.x == kFirst ? n0 : n0 + 64;
                 const int n_stages = len / C::kStageK;
                 for (int i = 0; i < n_stages; ++i, ++st) {

@@ -155,6 +155,7 @@ moe_gemm_kernel(const __grid_constant__ MoeRowMaps x, const __grid_constant__ Mo
         // ------------------------------------------------------ TMA producer
         uint32_t it = 0, j = 0;
         bool ok = true;
+        const CUtensorMap* acquired = nullptr;
         for (int w = unit; w < total_work;) {
             int nb;
             const MoeTile t = decode_item(w, p.tiles, nbn, &nb);
@@ -163,6 +164,14 @@ moe_gemm_kernel(const __grid_constant__ MoeRowMaps x, const __grid_constant__ Mo
             const int first = rank * half;                      // of this CTA's rows inside the tile
             const CUtensorMap* mw = p.w_maps + t.group;
             const CUtensorMap* mw2 = SWIGLU ? p.w2_maps + t.group : mw;
+            if (mw != acquired) {
+                if (elect_one()) {              // (the lane that issues the loads)
+                    tma_acquire_desc(mw);
+                    if (mw2 != mw) tma_acquire_desc(mw2);
+                }
+                __syncwarp();
+                acquired = mw;
+            }
             const int n0 = nb * TILE_N + rank * CTA_N;
             const int n1 = SWIGLU ? n0 : n0 + 64;               // columns of the second box
             // one box holds the CTA's rows, or eight more (one load a stage: with boxes of 16 rows, seven for a tile

@@ -229,6 +229,11 @@ __device__ __forceinline__ float4 ld_global_cg_v4_f32(const void* p) {
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* m) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
 }
+// For a map in device memory that the host has written (a __grid_constant__ one needs none): by the thread that issues the copies,
+// before the first.  Maps are read through a cache of their own, which may still hold what an earlier table had at that address.
+__device__ __forceinline__ void tma_acquire_desc(const CUtensorMap* m) {
+    asm volatile("fence.proxy.tensormap::generic.acquire.sys [%0], 128;" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
+}
 // Untiled bulk copies (both addresses 16-byte aligned, size a multiple of 16 bytes).
 // global -> this CTA's shared memory, completion counted on an mbarrier:
 __device__ __forceinline__ void bulk_load(uint32_t dst_smem, const void* src, uint32_t bytes, uint32_t bar) {

@@ -94,3 +94,23 @@ def test_tables_have_arrived_before_anyone_is_told_of_them():
         assert "rf::upload(" in s and not re.search(r"cudaMemcpy\w*\([^;]*HostToDevice", s), name
     s = _text(os.path.join(CSRC, "host_util.cu"))
     assert "cudaMemset(" not in s and "cudaStreamNonBlocking" in s and s.index("e = enqueue(s)") < s.index("cudaStreamSynchronize(s)")
+
+
+def test_maps_in_device_memory_are_acquired():
+    """Tensor maps that are no kernel parameters: the lane that issues the copies runs the tensor-map proxy's acquire fence on each
+    before the first of them, and on the next one when the expert changes."""
+    found = set()
+    for f, name, params, body in KERNELS:
+        for maps in set(re.findall(r"const CUtensorMap\* (\w+) = p\.\w*maps\b", body)) | set(
+                re.findall(r"const CUtensorMap\* (\w+) = [^;]*\bm0 \+ 1", body)) | set(
+                re.findall(r"const CUtensorMap\* (\w+) = SWIGLU \? p\.w2_maps", body)):
+            found.add((name, maps))
+            load = re.search(r"tma_load_2d\w*\([^,]+, " + maps + r",", body)
+            fence = body.index(f"tma_acquire_desc({maps})")
+            assert load and body.rindex("if (m", 0, fence) < fence < load.start(), (f, maps)
+            assert not re.search(r"tma_prefetch_desc\((p\.|" + maps + ")", body), f      # (nor fetched before that)
+    assert found == {("moe_few_kernel", "m0"), ("moe_few_kernel", "m1"), ("moe_gemm_kernel", "mw"), ("moe_gemm_kernel", "mw2")}
+    # nowhere else are maps read through a pointer
+    for f, name, params, body in KERNELS:
+        if name not in ("moe_few_kernel", "moe_gemm_kernel"):
+            assert not re.search(r"p\.\w*maps\b", body) and not re.search(r"CUtensorMap\s*\*", params), (f, name)
