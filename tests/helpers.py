@@ -24,3 +24,10 @@ def canary_output(m: int, n: int, pad_rows: int = 8):
 def canary_intact(full, m: int, n: int) -> bool:
     tail = full[m * n:]
     return bool((tail == CANARY).all().item())
+
+
+def assert_within(got, ref, tol):
+    """|got - ref| <= tol everywhere, where ref is finite.  (`err > tol` is false for a NaN, so it is asked the other way round.)"""
+    err = (got.double() - ref).abs()
+    bad = ~(err <= tol)
+    assert not bad.any(), (int(bad.sum()), int(err.isnan().sum()), float(err.nan_to_num(0.0).max()))

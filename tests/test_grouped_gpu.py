@@ -10,6 +10,7 @@ import pytest
 import torch
 
 from radeonflow_kernels_b200 import gemm, grouped, quant
+from tests.helpers import assert_within
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -220,3 +221,28 @@ def test_same_bits_every_time(m, e, n, k):
     for _ in range(200):
         grouped.fp8_grouped_mm(a, b, a_s, b_s, offsets, runs[1])
         assert torch.equal(runs[0], runs[1])
+
+
+EVERY = [(c, n, k, dtype, 0, 0) for c in FEW + MANY for n, k, dtype in ((64, 128, torch.bfloat16), (192, 384, torch.float16), (448, 640, torch.bfloat16))]
+EVERY += [(c, n, k, dtype, 0, 0) for c in WIDE_COUNTS for n, k, dtype in ((WIDE, 128, torch.bfloat16), (WIDE, 640, torch.float16),
+                                                                       (WIDE - 64, 384, torch.bfloat16), (WIDE + 128, 256, torch.float16))]
+EVERY += [(c, n, 256, torch.bfloat16, head, tail) for c, n in (([3, 0, 30], 320), ([200, 77], 320), ([700, 800], WIDE))
+          for head, tail in ((0, 1), (5, 0), (19, 301))]
+EVERY += [([20] * 12, 1472, 2048, torch.float16, 0, 0), ([300] * 5, 1088, 2048, torch.float16, 0, 0), ([300] * 12, 4160, 1024, torch.float16, 0, 0)]
+
+
+@pytest.mark.parametrize("chunk", range(6))
+def test_no_element_is_nan(chunk):
+    """The comparison in `run` lets a NaN pass; the same calls again, element by element in a comparison that does not.  Every element
+    starts as NaN, so that one which is not written shows too."""
+    for counts, n, k, dtype, head, tail in EVERY[chunk::6]:
+        offsets = np.concatenate([[head], head + np.cumsum(counts)]).tolist()
+        m = offsets[-1] + tail
+        a, b, a_s, b_s = operands(m, len(counts), n, k, sum(counts) + n)
+        c = torch.full((m, n), float("nan"), device=DEV, dtype=dtype)
+        grouped.fp8_grouped_mm(a, b, a_s, b_s, torch.tensor(offsets, dtype=torch.int32, device=DEV), c)
+        ref, mag = reference(a, b, a_s, b_s, offsets)
+        rows = slice(offsets[0], offsets[-1])
+        assert_within(c[rows], ref[rows], torch.finfo(dtype).eps / 2 * ref[rows].abs() + 2.0 ** -11 * mag[rows] + 2.0 ** -24)
+        assert c[:offsets[0]].isnan().all() and c[offsets[-1]:].isnan().all()
+    assert gemm.device_status() == 0
