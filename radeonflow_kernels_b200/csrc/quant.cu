@@ -102,15 +102,20 @@ __device__ __forceinline__ float half_warp_max(float a) {
     return a;
 }
 
-// 448 / a for 2^-100 <= a, within two units in the last place, zero for an infinity: the reciprocal of a scaled value, so that
-// neither it nor the reciprocal leaves the range of normal numbers.
+// Both factors of a block are quotients corrected by their remainder (Markstein): q0 within two units in the last place, then
+// q0 + (numerator - q0 * divisor) / divisor in fused operations.
+//
+// 448 / a rounded to nearest for 2^-100 <= a, zero for an infinity; so values that lie on a tie of two e4m3 ones go where the
+// formula sends them.  (The reciprocal is that of a scaled value: neither leaves the range of normal numbers.  That one correction is
+// enough for every a is tested: powers of two aside there are 2^23 of them.  A division costs the kernels for 16-bit rows, which have 32
+// registers, a stack frame.)
 __device__ __forceinline__ float steps_per_unit(float a) {
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a * 0x1p-20f));
-    return r * (kE4m3Max * 0x1p-20f);
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(a * 0x1p-20f));
+    const float q = y * (kE4m3Max * 0x1p-20f);
+    return isinf(a) ? 0.f : fmaf(fmaf(-q, a, kE4m3Max) * 0x1p-20f, y, q);
 }
-// a / 448 rounded to nearest: a quotient corrected by its exact remainder (Markstein), for a divisor whose reciprocal is rounded to
-// nearest.  An infinity stays one.
+// a / 448 rounded to nearest: here the divisor's reciprocal itself is.  An infinity stays one.
 __device__ __forceinline__ float over_448(float a) {
     constexpr float inv = 1.0f / kE4m3Max;
     const float q = a * inv;

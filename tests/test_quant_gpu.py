@@ -10,6 +10,7 @@ import pytest
 import torch
 
 from radeonflow_kernels_b200 import _lib, gemm, quant
+from tests.helpers import assert_within
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -248,3 +249,61 @@ def test_refusals_on_the_gpu(native, monkeypatch):
         quant.fp8_swiglu_quantize(x[:, :128])
     with pytest.raises(ValueError, match="contiguous"):
         quant.fp8_quantize_blocks(torch.zeros(2, 256, 512, device=DEV)[:, ::2, ::2])
+
+
+def formula_bits(x, amax):
+    """Blocks [..., 128] of fp32 values and their largest magnitudes, numpy -> bytes and scale by the formula in fp32."""
+    a = np.maximum(amax, np.float32(2.0 ** -100)).astype(np.float32)
+    v = x * (np.float32(448) / a)[..., None]
+    return torch.from_numpy(v).to(torch.float8_e4m3fn).view(torch.uint8).numpy(), a / np.float32(448)
+
+
+def near_ties(n, seed):
+    """n blocks of fp32 whose elements, times 448 / a, fall on the middle between two e4m3 values or a unit or two beside it."""
+    rng = np.random.default_rng(seed)
+    a = (rng.uniform(1, 2, n) * 2.0 ** rng.integers(-90, 90, n)).astype(np.float32)
+    e4m3 = torch.arange(0x08, 0x7E, dtype=torch.uint8).view(torch.float8_e4m3fn).float().numpy()        # normal values to 448
+    middle = (e4m3[1:] + e4m3[:-1]) / 2
+    x = (middle[rng.integers(0, len(middle), (n, 128))] / (np.float32(448) / a)[:, None]).astype(np.float32)
+    x = (x.view(np.int32) + rng.integers(-2, 3, x.shape, dtype=np.int32)).view(np.float32) * rng.choice([-1, 1], x.shape).astype(np.float32)
+    x[np.arange(n), rng.integers(0, 128, n)] = a
+    return x
+
+
+@pytest.mark.parametrize("m,k", [(60, 128), (700, 384), (9000, 1024)])
+def test_ties_go_where_the_formula_sends_them(m, k):
+    """q is e4m3(x * (448 / a)) with both operations rounded to nearest in fp32, to the bit: short calls, long ones, gathered ones."""
+    x = near_ties(m * k // 128, m).reshape(m, k // 128, 128)
+    want, scale = formula_bits(x, np.abs(x).max(-1))
+    t = torch.from_numpy(x.reshape(m, k)).to(DEV)
+    rows = torch.randperm(m, device=DEV, dtype=torch.int32)
+    for (q, s), order in ((quant.fp8_quantize(t), slice(None)), (quant.fp8_quantize(t, rows=rows), rows.cpu().numpy())):
+        assert np.array_equal(q.view(torch.uint8).cpu().numpy(), want.reshape(m, k)[order])
+        assert np.array_equal(s.cpu().numpy(), scale[order])
+
+
+@pytest.mark.parametrize("turned", [False, True])
+def test_ties_of_blocks(turned):
+    n, k = 300, 512
+    x = near_ties(n * k // 128, 3).reshape(n, k // 128, 128) if not turned else near_ties(n * k // 128, 4).reshape(n, k // 128, 128)
+    x /= np.abs(x).max(-1, keepdims=True)                       # one magnitude for the block: ties of its largest are a few
+    want, scale = [], []
+    for b in range(0, n, 128):
+        p = x[b:b + 128]
+        a = np.abs(p).max((0, 2))
+        q, s = formula_bits(p, np.broadcast_to(a, p.shape[:2]))
+        want.append(q.reshape(-1, k))
+        scale.append(s[0])
+    t = torch.from_numpy(x.reshape(n, k)).to(DEV)
+    q, s = quant.fp8_quantize_blocks(t.t().contiguous().t() if turned else t)
+    assert np.array_equal(q.view(torch.uint8).cpu().numpy(), np.concatenate(want)) and np.array_equal(s.cpu().numpy(), np.stack(scale))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_every_type_to_the_bit(dtype):
+    for m, k in ((3, 128), (700, 1152), (3000, 2048)):
+        x = data((m, k), dtype, m)
+        xb = blocks_of(x.float().cpu().numpy())
+        want, scale = formula_bits(xb, np.abs(xb).max(-1))
+        q, s = quant.fp8_quantize(x)
+        assert np.array_equal(q.view(torch.uint8).cpu().numpy(), want.reshape(m, k)) and np.array_equal(s.cpu().numpy(), scale)
