@@ -121,16 +121,24 @@ __device__ __forceinline__ float over_448(float a) {
     const float q = a * inv;
     return isinf(a) ? a : fmaf(fmaf(-q, kE4m3Max, a), inv, q);
 }
-// g / (1 + exp(-g)).  exp(-g) = 2^t (1 + d ln 2) with t = fl(-g log2 e) and d what its rounding left out.
+// g / (1 + exp(-g)) for g >= kSiluLow, where the reciprocal is a normal number.  exp(-g) = 2^t (1 + d ln 2) with t = fl(-g log2 e) and d
+// what that left out: the product's rounding, and what log2 e has beyond 24 bits.  Off by 2^-20.7 at most: ten times 2^-24, of which 2^t
+// has four and the reciprocal two.
+constexpr float kSiluLow = -87.0f;
 __device__ __forceinline__ float silu(float g) {
-    constexpr float log2e = 1.44269504f, ln2 = 0.693147181f;
-    const float t = -g * log2e, d = fmaf(-g, log2e, -t);
+    constexpr float log2e = 1.44269502f, log2e_rest = 1.92596303e-8f, ln2 = 0.693147181f;
+    const float t = -g * log2e, d = fmaf(-g, log2e_rest, fmaf(-g, log2e, -t));
     float e, r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-    // (where t is infinite, or 2^t, d says nothing)
+    // (where 2^t is no normal number, d may be none either)
     if (fabsf(t) < 126.0f) e = fmaf(e, d * ln2, e);
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
     return g * r;
+}
+// SiLU(g) * u below that: 1 / (1 + exp(-g)) is exp(g) there, which leaves the normal numbers; its root does not before g u exp(g) does.
+__device__ __forceinline__ float swiglu_low(float g, float u) {
+    const float root = expf(0.5f * g);
+    return (g * root) * (root * u);
 }
 
 __device__ __forceinline__ uint2 to_e4m3x8(const float (&x)[8], float r) {
@@ -198,6 +206,15 @@ quantize_rows_kernel(const T* x, long long row_stride, const int* rows, uint32_t
     for (int i = 0; i < PER; ++i) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] = SWIGLU ? silu(g[i].f(j)) * u[i].f(j) : g[i].f(j);
+        if (SWIGLU) {
+            float low = g[i].f(0);
+#pragma unroll
+            for (int j = 1; j < 8; ++j) low = fminf(low, g[i].f(j));
+            if (low < kSiluLow)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (g[i].f(j) < kSiluLow) v[i][j] = swiglu_low(g[i].f(j), u[i].f(j));
+        }
         a[i] = SWIGLU ? largest_of(v[i]) : largest_of(g[i]);
     }
     uint8_t* to = q + (size_t)first * kBlock + lane * 8;

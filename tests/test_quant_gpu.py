@@ -307,3 +307,46 @@ def test_every_type_to_the_bit(dtype):
         want, scale = formula_bits(xb, np.abs(xb).max(-1))
         q, s = quant.fp8_quantize(x)
         assert np.array_equal(q.view(torch.uint8).cpu().numpy(), want.reshape(m, k)) and np.array_equal(s.cpu().numpy(), scale)
+
+
+# SwiGLU far below zero.  Its fp32 arithmetic, as quant.cu has it: 2^t within 2^-22, the reciprocal within 2^-23, four roundings of
+# 2^-24 on the way to SiLU, one for the product with up: 11 * 2^-24 < 2^-20.  Below -87: twice an exponential of (g / 2) within 2
+# ulp = 2^-22 each, three products, and 1 / (1 + exp(-g)) = exp(g) (1 - 2^-125): 2^-21 + 3 * 2^-24 < 2^-20.  The magnitude of a
+# block, and so its scale, is off by as much; x * r by two more roundings.
+SWIGLU = 2.0 ** -20
+
+
+def check_swiglu(gu, q, s):
+    f = gu.shape[1] // 2
+    x = gu.double()
+    h = blocks_of(x[:, :f] / (1 + torch.exp(-x[:, :f])) * x[:, f:])
+    a = h.abs().amax(-1).clamp(min=2.0 ** -100)
+    assert_within(s, a / 448, (2.0 ** -24 * 1.01 + SWIGLU) * a / 448)
+    v = h * (448 / a)[..., None]
+    assert_within(blocks_of(q.float()), v, 2.0 ** -4 * v.abs() * (1 + 2.0 ** -22 + 2 * SWIGLU) + 2.0 ** -10)
+
+
+@pytest.mark.parametrize("dtype,size", [(torch.float32, 1e36), (torch.bfloat16, 1e36), (torch.float32, 1.0), (torch.bfloat16, 1.0),
+                                        (torch.float16, 6e4)])
+@pytest.mark.parametrize("lo,hi", [(-60, -30), (-86.9, -80), (-95, -85), (-104, -87), (80, 95), (-1e-3, 1e-3)])
+@pytest.mark.parametrize("m", [4, 1500])
+def test_swiglu_of_far_gates(dtype, size, lo, hi, m):
+    f = 256
+    g = torch.Generator(device=DEV).manual_seed(m)
+    gate = lo + (hi - lo) * torch.rand(m, f, generator=g, device=DEV)
+    up = torch.randn(m, f, generator=g, device=DEV) * (size / 6 if hi < 0 or size == 6e4 else 1.0)
+    gu = torch.cat([gate, up], 1).to(dtype)
+    check_swiglu(gu, *quant.fp8_swiglu_quantize(gu))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_swiglu_at_the_ends(dtype):
+    """SiLU(-inf) is -inf * 0, the largest negative gate gives zero, +inf infinity."""
+    top = torch.finfo(dtype).max
+    gu = torch.ones(5, 256, device=DEV, dtype=dtype)
+    gu[0, 3], gu[1, 3], gu[2, :128], gu[3, 3], gu[4, 3] = -float("inf"), float("inf"), -top, float("nan"), -top
+    q, s = quant.fp8_swiglu_quantize(gu)
+    assert s[0, 0].isnan() and s[1, 0].isinf() and s[3, 0].isnan()
+    assert (q[2].float() == 0).all() and s[2, 0] == 2.0 ** -100 / 448
+    one = 1 / (1 + np.exp(-1.0))
+    assert q[4, 3].float() == 0 and (q[4, 4:].float() == 448).all() and abs(float(s[4, 0]) * 448 / one - 1) < SWIGLU
