@@ -7,6 +7,7 @@ to fp16, equal ones by the lowest index.  Unlike the layer it rounds nothing bet
 vector between an expert's two products, to fp16.
 """
 import ctypes
+import threading
 import weakref
 
 import torch
@@ -34,6 +35,7 @@ class _Workspace:
 
 # (device, stream, capture) -> workspace.  The layers of a model run one after the other on a stream, so they share them.
 _workspaces = weakref.WeakValueDictionary()
+_lock = threading.Lock()        # over both maps of workspaces while one is looked for and made
 
 
 class FewTokenMoE:
@@ -124,22 +126,26 @@ class FewTokenMoE:
         capture = ctypes.c_ulonglong()          # (of this call: another thread's may come in between)
         _lib.check(L.rf_stream_capture_id(stream, ctypes.byref(capture)), "rf_stream_capture_id")
         key = (self.device.index, stream, capture.value)
-        ws = self._held.get(key)
-        if ws is None or ws[-1].size < size:
+        held = self._held.get(key)
+        if held is not None and held[-1].size >= size:
+            return held[-1]
+        with _lock:             # threads may share a stream
             shared = _workspaces.get(key)
             if shared is None or shared.size < size:
                 # (one that has become too small stays: earlier calls, or a graph, may still use it)
                 shared = _workspaces[key] = _Workspace(1 << (size - 1).bit_length())
-            ws = self._held.setdefault(key, [])
-            ws.append(shared)
-        return ws[-1]
+            held = self._held.get(key, ())
+            if not held or held[-1] is not shared:
+                self._held[key] = (*held, shared)       # never seen empty
+        return shared
 
     def reset(self):
         """Forgets the workspaces of this process's layers.  Needed after `gemm.device_status()` has told of a lost wait: until then
         every call with a workspace that such a call left behind refuses to run and reports a lost wait again.  The other layers
         have to be reset too.  Graphs captured before it must not be replayed after it."""
-        _workspaces.clear()
-        self._held.clear()
+        with _lock:
+            _workspaces.clear()
+            self._held.clear()
 
     def forward(self, x, out=None):
         """x fp16 [..., d_hidden], 1 to 32 tokens -> out, same shape (given, it must not overlap x).  Enqueues one kernel on the

@@ -1,5 +1,8 @@
 """Refusals of the layer for a few tokens, all before any device work, and the arithmetic of its workspace."""
 import ctypes
+import sys
+import threading
+import weakref
 
 import pytest
 import torch
@@ -85,3 +88,115 @@ def test_python_weights(monkeypatch):
             moe_few.FewTokenMoE({**good8, name: bad}, cfg)
     with pytest.raises(ValueError, match="multiples of 128"):
         moe_few.FewTokenMoE(good8, {**cfg, "d_expert": 64})
+
+
+class FakeLibrary:
+    """What `_workspace` asks of the library: a size for a number of tokens, a stream's capture."""
+
+    def __init__(self, capture=0):
+        self.capture = capture
+
+    def rf_moe_few_workspace_bytes(self, config, n_tokens):
+        return 1000 * n_tokens
+
+    def rf_stream_capture_id(self, stream, out):
+        out._obj.value = self.capture
+        return 0
+
+
+class FakeWorkspace:
+    made = []
+
+    def __init__(self, size):
+        self.size = size
+        FakeWorkspace.made.append(size)
+
+
+@pytest.fixture
+def bare_layer(monkeypatch):
+    """A layer without weights, and its workspaces without a GPU."""
+    monkeypatch.setattr(_lib, "lib", lambda library=FakeLibrary(): library)
+    monkeypatch.setattr(moe_few, "_Workspace", FakeWorkspace)
+    monkeypatch.setattr(moe_few, "_workspaces", weakref.WeakValueDictionary())
+    FakeWorkspace.made.clear()
+
+    def make():
+        layer = moe_few.FewTokenMoE.__new__(moe_few.FewTokenMoE)
+        layer._handle, layer.config, layer.device, layer._held, layer._sizes = None, config(), torch.device("cuda", 0), {}, {}
+        return layer
+    return make
+
+
+def lines_of(fn):
+    """How many lines of `_workspace` a call runs."""
+    count = []
+    code = moe_few.FewTokenMoE._workspace.__code__
+
+    def trace(frame, event, arg):
+        if frame.f_code is code:
+            count.append(event == "line")
+            return trace
+        return None
+    sys.settrace(trace)
+    try:
+        fn()
+    finally:
+        sys.settrace(None)
+    return sum(count)
+
+
+@pytest.mark.parametrize("first,second", [(4, 4), (4, 9), (9, 4)])
+def test_two_threads_on_one_stream(bare_layer, first, second):
+    """A thread is stopped in front of each line of `_workspace` in turn while another thread calls it, for the same stream."""
+    code = moe_few.FewTokenMoE._workspace.__code__
+    total = lines_of(lambda: bare_layer()._workspace(first, 7))
+    assert total > 8
+    stops = 0
+    for stop in range(total):
+        layer, got, left = bare_layer(), [], [stop]
+
+        def other():
+            try:
+                got.append(layer._workspace(second, 7))
+            except Exception as e:          # what the test is for
+                got.append(e)
+
+        thread = threading.Thread(target=other)
+
+        def trace(frame, event, arg):
+            if frame.f_code is not code:
+                return None
+            if event == "line":
+                if left[0] == 0:
+                    thread.start()
+                    thread.join(0.1)        # (it may have to wait for this thread)
+                left[0] -= 1
+            return trace
+
+        sys.settrace(trace)
+        try:
+            mine = layer._workspace(first, 7)
+        finally:
+            sys.settrace(None)
+        if left[0] >= 0:            # fewer lines than before
+            break
+        thread.join(10)
+        assert not thread.is_alive() and mine.size >= 1000 * first
+        assert got and not isinstance(got[0], Exception) and got[0].size >= 1000 * second, (stop, got)
+        stops += 1
+        # the stream's calls to come share one
+        assert layer._workspace(first, 7) is layer._workspace(second, 7) is layer._workspace(max(first, second), 7)
+        del layer, mine, got
+        moe_few._workspaces.clear()
+    assert stops >= total - 2
+
+
+def test_layers_share_a_streams_workspace(bare_layer):
+    a, b = bare_layer(), bare_layer()
+    one = a._workspace(4, 7)
+    assert b._workspace(4, 7) is one and b._workspace(3, 7) is one and FakeWorkspace.made == [4096]
+    large = b._workspace(5, 7)
+    assert large.size == 8192 and a._workspace(4, 7) is one and a._workspace(5, 7) is large
+    assert a._workspace(4, 8) is not one
+    a.reset()
+    assert a._workspace(4, 7) is not one
