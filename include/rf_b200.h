@@ -562,6 +562,12 @@ size_t rf_moe_few_workspace_bytes(const RfMoeFewConfig *config, int n_tokens);
  * of the graph).                                                                                     */
 int rf_moe_few_workspace_alloc(size_t bytes, void **workspace);
 int rf_moe_few_workspace_free(void *workspace);
+/* The same for calls in the capture that `stream` is part of: the memory belongs to the captured graph and to the executables made
+ * of it, and is not the caller's to free.  It goes when the last of them has, at the next call of this function,
+ * rf_moe_few_workspace_alloc, _free or _reap.  RF_ERR_UNSUPPORTED: the stream is not being captured. */
+int rf_moe_few_workspace_alloc_captured(rf_stream_t stream, size_t bytes, void **workspace);
+/* Frees what graphs that are gone have left; *bytes (or NULL): how much is still with living ones.  May synchronise the device. */
+int rf_moe_few_workspace_reap(size_t *bytes);
 /* *id = 0: the stream is not being captured; else a number of its own for each capture.              */
 int rf_stream_capture_id(rf_stream_t stream, unsigned long long *id);
 /* x fp16 [n_tokens, d_hidden] -> out fp16 [n_tokens, d_hidden], 16-byte aligned, workspace 256.  One kernel, asynchronous.  x and

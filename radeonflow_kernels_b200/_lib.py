@@ -300,6 +300,10 @@ def _declare_fp8(L: ctypes.CDLL) -> None:
     L.rf_moe_few_workspace_alloc.argtypes = [sz, ctypes.POINTER(vp)]
     L.rf_moe_few_workspace_free.restype = ci
     L.rf_moe_few_workspace_free.argtypes = [vp]
+    L.rf_moe_few_workspace_alloc_captured.restype = ci
+    L.rf_moe_few_workspace_alloc_captured.argtypes = [vp, sz, ctypes.POINTER(vp)]
+    L.rf_moe_few_workspace_reap.restype = ci
+    L.rf_moe_few_workspace_reap.argtypes = [ctypes.POINTER(sz)]
     L.rf_stream_capture_id.restype = ci
     L.rf_stream_capture_id.argtypes = [vp, ctypes.POINTER(ctypes.c_ulonglong)]
     L.rf_moe_few_forward.restype = ci

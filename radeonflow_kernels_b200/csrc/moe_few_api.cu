@@ -4,6 +4,7 @@
 #include "host_util.h"
 #include "moe_few.h"
 
+#include <atomic>
 #include <cstdint>
 #include <cstdio>
 #include <new>
@@ -76,6 +77,64 @@ int check_config(const RfMoeFewConfig& c) {
     if (e < 1 || e > rf::kFewMaxExperts || (e & (e - 1)) != 0) return RF_ERR_UNSUPPORTED;
     if (c.n_experts_per_token < 1 || c.n_experts_per_token > rf::kFewMaxTopK || c.n_experts_per_token > e) return RF_ERR_UNSUPPORTED;
     return RF_OK;
+}
+
+// Memory that belongs to a captured graph (a CUDA user object of it, which its executables own too).  When the last of them has gone,
+// the object's destructor runs on a thread of CUDA's that may call nothing of CUDA: it only says so, and a later call frees.
+struct GraphMemory {
+    void* ptr;
+    size_t bytes;
+    GraphMemory* next;
+};
+std::atomic<GraphMemory*> g_left{nullptr};
+std::atomic<size_t> g_with_graphs{0};
+
+void CUDART_CB graph_gone(void* p) {
+    GraphMemory* m = static_cast<GraphMemory*>(p);
+    m->next = g_left.load(std::memory_order_relaxed);
+    while (!g_left.compare_exchange_weak(m->next, m, std::memory_order_release, std::memory_order_relaxed)) {
+    }
+}
+
+// (in relaxed capture mode)
+cudaError_t free_left() {
+    cudaError_t e = cudaSuccess;
+    for (GraphMemory* m = g_left.exchange(nullptr, std::memory_order_acquire); m != nullptr;) {
+        GraphMemory* next = m->next;
+        const cudaError_t f = cudaFree(m->ptr);
+        if (f != cudaSuccess) e = f;
+        g_with_graphs -= m->bytes;
+        delete m;
+        m = next;
+    }
+    return e;
+}
+
+// While a stream of this thread is being captured: what runs inside touches none that is.
+class Relaxed {
+public:
+    Relaxed() { ok_ = cudaThreadExchangeStreamCaptureMode(&mode_) == cudaSuccess; }
+    ~Relaxed() {
+        if (ok_) cudaThreadExchangeStreamCaptureMode(&mode_);
+    }
+    bool ok() const { return ok_; }
+
+private:
+    cudaStreamCaptureMode mode_ = cudaStreamCaptureModeRelaxed;
+    bool ok_;
+};
+
+cudaError_t zeroed(size_t bytes, void** out) {
+    void* p = nullptr;
+    cudaError_t e = cudaMalloc(&p, bytes);
+    if (e == cudaSuccess) e = rf::upload_zeroes(p, bytes);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        if (p) cudaFree(p);
+        p = nullptr;
+    }
+    *out = p;
+    return e;
 }
 
 bool encode(CUtensorMap* m, bool fp8, const void* base, int k, int n) {
@@ -169,27 +228,59 @@ int rf_moe_few_workspace_alloc(size_t bytes, void** out) {
     if (!out) return RF_ERR_NULL_POINTER;
     *out = nullptr;
     if (!rf::device_state()) return RF_ERR_CUDA;
-    // Allowed while a stream of this thread is being captured: nothing here touches that stream.
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return RF_ERR_CUDA;
-    void* p = nullptr;
-    cudaError_t e = cudaMalloc(&p, bytes);
-    if (e == cudaSuccess) e = rf::upload_zeroes(p, bytes);
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        if (p) cudaFree(p);
-        p = nullptr;
+    Relaxed relaxed;
+    if (!relaxed.ok()) return RF_ERR_CUDA;
+    free_left();
+    return zeroed(bytes, out) == cudaSuccess ? RF_OK : RF_ERR_CUDA;
+}
+
+int rf_moe_few_workspace_alloc_captured(rf_stream_t stream, size_t bytes, void** out) {
+    if (!out) return RF_ERR_NULL_POINTER;
+    *out = nullptr;
+    if (!rf::device_state()) return RF_ERR_CUDA;
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    cudaGraph_t graph = nullptr;
+    if (cudaStreamGetCaptureInfo_v2(reinterpret_cast<cudaStream_t>(stream), &status, nullptr, &graph) != cudaSuccess)
+        return RF_ERR_CUDA;
+    if (status != cudaStreamCaptureStatusActive || graph == nullptr) return RF_ERR_UNSUPPORTED;
+    GraphMemory* m = new (std::nothrow) GraphMemory{nullptr, bytes, nullptr};
+    if (!m) return RF_ERR_CUDA;
+    Relaxed relaxed;
+    if (relaxed.ok()) free_left();
+    if (!relaxed.ok() || zeroed(bytes, &m->ptr) != cudaSuccess) {
+        delete m;
+        return RF_ERR_CUDA;
     }
-    cudaThreadExchangeStreamCaptureMode(&mode);
-    *out = p;
-    return e == cudaSuccess ? RF_OK : RF_ERR_CUDA;
+    cudaUserObject_t object = nullptr;
+    if (cudaUserObjectCreate(&object, m, graph_gone, 1, cudaUserObjectNoDestructorSync) != cudaSuccess) {
+        cudaFree(m->ptr);
+        delete m;
+        return RF_ERR_CUDA;
+    }
+    g_with_graphs += bytes;
+    if (cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove) != cudaSuccess) {
+        cudaUserObjectRelease(object, 1);
+        return RF_ERR_CUDA;
+    }
+    *out = m->ptr;
+    return RF_OK;
 }
 
 int rf_moe_few_workspace_free(void* workspace) {
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return RF_ERR_CUDA;
-    const cudaError_t e = cudaFree(workspace);
-    cudaThreadExchangeStreamCaptureMode(&mode);
+    Relaxed relaxed;
+    if (!relaxed.ok()) return RF_ERR_CUDA;
+    const cudaError_t left = free_left(), e = cudaFree(workspace);
+    return left == cudaSuccess && e == cudaSuccess ? RF_OK : RF_ERR_CUDA;
+}
+
+int rf_moe_few_workspace_reap(size_t* bytes) {
+    cudaError_t e = cudaSuccess;
+    if (g_left.load(std::memory_order_relaxed) != nullptr) {
+        Relaxed relaxed;
+        if (!relaxed.ok()) return RF_ERR_CUDA;
+        e = free_left();
+    }
+    if (bytes) *bytes = g_with_graphs.load(std::memory_order_relaxed);
     return e == cudaSuccess ? RF_OK : RF_ERR_CUDA;
 }
 

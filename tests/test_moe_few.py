@@ -115,7 +115,8 @@ class FakeWorkspace:
 @pytest.fixture
 def bare_layer(monkeypatch):
     """A layer without weights, and its workspaces without a GPU."""
-    monkeypatch.setattr(_lib, "lib", lambda library=FakeLibrary(): library)
+    library = FakeLibrary()
+    monkeypatch.setattr(_lib, "lib", lambda: library)
     monkeypatch.setattr(moe_few, "_Workspace", FakeWorkspace)
     monkeypatch.setattr(moe_few, "_workspaces", weakref.WeakValueDictionary())
     FakeWorkspace.made.clear()
@@ -200,3 +201,34 @@ def test_layers_share_a_streams_workspace(bare_layer):
     assert a._workspace(4, 8) is not one
     a.reset()
     assert a._workspace(4, 7) is not one
+
+
+def test_captures_leave_nothing_with_the_layer(bare_layer, monkeypatch):
+    """A capture's workspace is the graph's: layers share it while it is being captured and hold nothing of it."""
+    class FakeCaptureWorkspace:
+        def __init__(self, stream, capture, size):
+            self.stream, self.capture, self.size = stream, capture, size
+
+    library = FakeLibrary()
+    monkeypatch.setattr(_lib, "lib", lambda: library)
+    monkeypatch.setattr(moe_few, "_CaptureWorkspace", FakeCaptureWorkspace)
+    monkeypatch.setattr(moe_few, "_captured", {})
+    a, b = bare_layer(), bare_layer()
+    eager = a._workspace(4, 7)
+    for capture in range(1, 40):
+        library.capture = capture
+        one = a._workspace(4, 7)
+        assert (one.stream, one.capture, one.size) == (7, capture, 4000)
+        assert a._workspace(3, 7) is one and b._workspace(4, 7) is one
+        assert b._workspace(4, 8) is not one            # a branch of the capture
+        more = b._workspace(9, 7)
+        assert more.size == 9000 and a._workspace(4, 7) is more
+    library.capture = 0
+    assert a._workspace(4, 7) is eager and len(moe_few._captured) == 2 and len(a._held) == 1 and not b._held
+
+
+def test_captured_workspace_entry(rf_lib):
+    assert rf_lib.rf_moe_few_workspace_alloc_captured(None, 100, None) == 2
+    n = ctypes.c_size_t(5)
+    assert rf_lib.rf_moe_few_workspace_reap(ctypes.byref(n)) == 0 and n.value == 0
+    assert rf_lib.rf_moe_few_workspace_reap(None) == 0

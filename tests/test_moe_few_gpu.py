@@ -9,7 +9,9 @@ every step, and 40 more additions of partial sums:
     dy <= sum dh |Wd| + s(f) sum |h||Wd|;  dout <= u |out| + 2^-25 + (1 + 2^-20) sum_i p_i dy_i
 """
 import ctypes
+import gc
 import threading
+import time
 
 import numpy as np
 import pytest
@@ -322,3 +324,87 @@ def test_first_call_on_a_stream_of_its_own(fp8):
         check(got, *want[i % 2][:2])
         del layer
     assert gemm.device_status() == 0
+
+
+def settled(want):
+    """Bytes that graphs hold, once CUDA has told of those that are gone (it does so on a thread of its own)."""
+    for _ in range(200):
+        gc.collect()
+        if moe_few.captured_workspace_bytes() == want:
+            return True
+        time.sleep(0.02)
+    return False
+
+
+def capture(layer, x):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer.forward(x)
+    return graph, out
+
+
+def test_a_graphs_workspace_goes_with_it():
+    x, w, cfg, _ = make(32, 1024, 512, 32, 4, 1, False, seed=13)
+    layer, other = moe_few.FewTokenMoE(w, cfg), moe_few.FewTokenMoE(w, cfg)
+    size = lambda t: _lib.lib().rf_moe_few_workspace_bytes(ctypes.byref(layer.config), t)
+    want = {t: layer.forward(x[:t]).clone() for t in (1, 8, 32)}
+    torch.cuda.synchronize()
+    gc.collect()
+    time.sleep(0.2)
+    before = moe_few.captured_workspace_bytes()
+    graphs = {t: capture(layer, x[:t]) for t in want}
+    assert settled(before + sum(size(t) for t in want))
+    both = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(both):            # two layers and two sizes in one graph: one workspace, and the larger one
+        outs = layer.forward(x[:8]), other.forward(x[:8]), other.forward(x[:32]), layer.forward(x[:1])
+    assert settled(before + sum(size(t) for t in want) + size(8) + size(32))
+    both.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[o.shape[0]]) for o in outs)
+    # one goes; the others stay whole while what it had is used again
+    del graphs[8], both, outs
+    assert settled(before + size(1) + size(32))
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        assert torch.equal(layer.forward(x), want[32])
+    for t, (graph, out) in graphs.items():
+        for _ in range(5):
+            out.zero_()
+            graph.replay()
+            assert torch.equal(out, want[t])
+    graphs[32][0].replay()                  # (gone while it runs)
+    del graph, out, graphs
+    assert settled(before) and gemm.device_status() == 0
+    # captured over and over
+    free = torch.cuda.mem_get_info()[0]
+    for _ in range(30):
+        graph, out = capture(layer, x)
+        graph.replay()
+        assert torch.equal(out, want[32])
+        del graph, out
+    assert settled(before) and torch.cuda.mem_get_info()[0] >= free - 4 * size(32) - (8 << 20)
+    assert len(layer._held) == 2 and gemm.device_status() == 0
+
+
+def test_a_capture_that_fails_leaves_nothing():
+    x, w, cfg, _ = make(4, 256, 128, 8, 2, 1, False, seed=14)
+    layer = moe_few.FewTokenMoE(w, cfg)
+    want = layer.forward(x).clone()
+    gc.collect()
+    time.sleep(0.2)
+    before = moe_few.captured_workspace_bytes()
+    with pytest.raises(RuntimeError, match="given up"):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            layer.forward(x)
+            raise RuntimeError("given up")
+    del graph
+    assert settled(before)
+    graph, out = capture(layer, x)
+    graph.replay()
+    assert torch.equal(out, want) and torch.equal(layer.forward(x), want)
+
+
+def test_workspaces_of_captures_only(rf_lib):
+    got = ctypes.c_void_p()
+    assert rf_lib.rf_moe_few_workspace_alloc_captured(torch.cuda.Stream().cuda_stream, 1000, ctypes.byref(got)) == 7 and not got
