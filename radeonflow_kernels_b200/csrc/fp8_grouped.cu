@@ -257,7 +257,8 @@ fp8_grouped_many_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_
                     if (c + 1 == HN / 16) {
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(tmem_empty_bar(buf));
+                        // (the scales' slot goes back with the accumulator)
+                        if (lane == 0) mbar_arrive_after(tmem_empty_bar(buf), __float_as_uint(s), (uint32_t)p.groups >> 16);
                     }
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
