@@ -124,3 +124,16 @@ def test_grouped_scale_slots_are_given_back_after_they_were_read():
         assert "mbar_arrive(tmem_empty_bar" not in body, kernel
     # the mask is zero: at most 1024 groups
     assert re.search(r"kGroupedMaxGroups = 1024;", _text(os.path.join(CSRC, "fp8_grouped.cuh")))
+
+
+def test_kernels_launched_through_the_helper_wait():
+    """`launch_kernel(..., true, ...)` launches as a programmatic dependent: the same rule as above for the files that use it."""
+    assert "programmaticStreamSerializationAllowed" in _text(os.path.join(CSRC, "launch.h"))
+    through = [(f, name, body) for f, name, _, body in KERNELS if "launch_kernel(" in _text(os.path.join(CSRC, f))]
+    assert {name for _, name, _ in through} >= {"quantize_rows_kernel", "quantize_blocks_kernel", "fp8_grouped_few_kernel",
+                                                "fp8_grouped_many_kernel", "moe_few_kernel"}
+    for f, name, body in through:
+        assert body.count("griddep_wait()") == 1, (f, name)
+        # nothing of another kernel's before it: what stands there are barriers, TMEM, indices and maps
+        before = body[:body.index("griddep_wait()")]
+        assert not re.search(r"ld_global|ld_word|atomic|tma_load|bulk_load|st_word", before), (f, name)
