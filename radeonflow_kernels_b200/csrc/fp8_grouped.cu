@@ -250,6 +250,9 @@ fp8_grouped_many_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_
                 float v[2][16];
                 tmem_ld16_async(taddr, v[0]);
                 const float s = __uint_as_float(ld_shared_u32(my_scale + (it % NB) * (BM * 4)));
+                // (the scales' slot goes back with the accumulator: behind this load, mbar_arrive_after's rule.  Made at the arrival itself
+                // the address cost 4 % of 32768 rows, here 1)
+                const uint32_t back = tmem_empty_bar(buf) + (__float_as_uint(s) & ((uint32_t)p.groups >> 16));
 #pragma unroll
                 for (int c = 0; c < HN / 16; ++c) {
                     tmem_ld16_fence(v[c % 2]);
@@ -257,8 +260,7 @@ fp8_grouped_many_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_
                     if (c + 1 == HN / 16) {
                         tc_fence_before();
                         __syncwarp();
-                        // (the scales' slot goes back with the accumulator)
-                        if (lane == 0) mbar_arrive_after(tmem_empty_bar(buf), __float_as_uint(s), (uint32_t)p.groups >> 16);
+                        if (lane == 0) mbar_arrive(back);
                     }
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
