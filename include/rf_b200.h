@@ -526,7 +526,7 @@ int rf_fp8_quantize_blocks(const void *w, int dtype, int e, int n, int k, long l
 /* Grouped FP8 block-scaled product: the rows offsets[g] .. offsets[g+1] - 1 of a by the g-th weight,
  *   c[r,n] = sum_kb as[r,kb] * bs[g,n/128,kb] * (A_kb . B_g,kb^T), rounded once to c_dtype (RF_BF16 or RF_F16).
  * a : e4m3fn [m,k], as : fp32 [m,k/128], b : e4m3fn [n_groups,n,k], bs : fp32 [n_groups,ceil(n/128),k/128], offsets : int32
- * [n_groups+1] on the device, ascending in 0 .. m (clipped to that), c [m,n]; all dense.  n % 64 == 0, k % 128 == 0,
+ * [n_groups+1] on the device, ascending in 0 .. m (clipped to that; one below an earlier one counts as that), c [m,n]; all dense.  n % 64 == 0, k % 128 == 0,
  * n_groups <= 1024; groups may be empty.  Rows in no group are not written.  Needs no workspace; calls may overlap.  */
 int rf_fp8_grouped_gemm(const void *a, const void *b, const float *as, const float *bs, const int *offsets, void *c,
                         int c_dtype, int m, int n_groups, int n, int k, rf_stream_t stream);

@@ -24,16 +24,22 @@ struct GroupTable {
     int sums[33];
 };
 
+__device__ __forceinline__ int clipped_offset(const GroupedParams& p, int g) {
+    return min(max(ld_global_s32(p.offsets + g), 0), p.m);
+}
+
 // Every thread of the CTA calls it (the caller synchronises behind it).  A group's rows are cut into tiles of `tile_rows`.
-// Offsets are clipped to 0 .. m and to ascending order, so that no table leads outside the matrices.
+// Offsets are clipped to 0 .. m, and one below an earlier one counts as that: no table leads outside the matrices, no row is in two
+// groups, and there are m / tile_rows + groups tiles at most.
 __device__ __forceinline__ void build_group_table(GroupTable& t, const GroupedParams& p, int tile_rows) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_warps = blockDim.x >> 5;
     const int per = (p.groups + blockDim.x - 1) / blockDim.x;
     const int g0 = min(tid * per, p.groups), g1 = min(g0 + per, p.groups);
     int mine = 0;
+    bool descends = false;
     for (int g = g0; g < g1; ++g) {
-        const int lo = min(max(ld_global_s32(p.offsets + g), 0), p.m);
-        const int hi = min(max(ld_global_s32(p.offsets + g + 1), lo), p.m);
+        const int lo = clipped_offset(p, g), hi = clipped_offset(p, g + 1);
+        descends = descends || hi < lo;
         t.lo[g] = lo;
         t.hi[g] = hi;
         mine += (hi - lo + tile_rows - 1) / tile_rows;
@@ -45,7 +51,21 @@ __device__ __forceinline__ void build_group_table(GroupTable& t, const GroupedPa
         if (lane >= s) incl += o;
     }
     if (lane == 31) t.sums[warp] = incl;
-    __syncthreads();
+    if (__syncthreads_or(descends)) {           // no table that a permutation makes: one thread takes its time
+        if (tid == 0) {
+            int at = clipped_offset(p, 0), run = 0;
+            for (int g = 0; g < p.groups; ++g) {
+                const int end = max(at, clipped_offset(p, g + 1));
+                t.lo[g] = at;
+                t.hi[g] = end;
+                t.start[g] = run;
+                run += (end - at + tile_rows - 1) / tile_rows;
+                at = end;
+            }
+            t.start[p.groups] = run;
+        }
+        return;
+    }
     int before = 0, all = 0;
     for (int w = 0; w < n_warps; ++w) {
         if (w < warp) before += t.sums[w];

@@ -16,7 +16,8 @@ def fp8_grouped_mm(a, b, a_scale, b_scale, offsets, c):
     """c[r] = sum_kb a_scale[r, kb] * b_scale[g, :, kb] * (a[r] . b[g]^T)_kb for the rows r in offsets[g] .. offsets[g + 1] - 1.
 
     a [m, k] e4m3fn, b [groups, n, k] e4m3fn, a_scale [m, k/128] fp32, b_scale [groups, ceil(n/128), k/128] fp32, offsets
-    [groups + 1] int32 on the device, ascending, in 0 .. m (others are clipped to that); c [m, n] bf16 or fp16, returned.
+    [groups + 1] int32 on the device, ascending, in 0 .. m (others are clipped to that, and one below an earlier one counts as the
+    earlier one); c [m, n] bf16 or fp16, returned.
     All contiguous, on the current device.  n % 64 == 0, k % 128 == 0, at most 1024 groups, which may be empty.  Rows in no
     group are left as they were.  The counts stay on the device: nothing is synchronised, and a captured call follows the
     offsets of its replay.

@@ -246,3 +246,24 @@ def test_no_element_is_nan(chunk):
         assert_within(c[rows], ref[rows], torch.finfo(dtype).eps / 2 * ref[rows].abs() + 2.0 ** -11 * mag[rows] + 2.0 ** -24)
         assert c[:offsets[0]].isnan().all() and c[offsets[-1]:].isnan().all()
     assert gemm.device_status() == 0
+
+
+@pytest.mark.parametrize("m,n", [(60, 192), (700, WIDE)])
+@pytest.mark.parametrize("table", ["back", "once", "all", "wild"])
+def test_descending_offsets_count_as_the_largest_before(m, n, table):
+    """A row is in one group whatever the table says: the bits of the table's running maximum."""
+    e = 12
+    a, b, a_s, b_s = operands(m, e, n, 256, m)
+    steps = np.linspace(0, m, e + 1).astype(np.int64)
+    off = {"back": np.concatenate([steps[:7], [steps[3], steps[4]], steps[9:]]), "once": np.concatenate([steps[:-1], [0]]), "all": steps[::-1],
+           "wild": np.array([5, m, -3, 2 ** 31 - 1, 0, m // 2, -2 ** 31, m, 1, m - 1, 0, 7, m])}[table]
+    want_off = np.maximum.accumulate(np.clip(off, 0, m))
+    dev = lambda t: torch.from_numpy(t.astype(np.int32)).to(DEV)
+    got, want = (torch.full((m + 70, n), 5.0, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    grouped.fp8_grouped_mm(a, b, a_s, b_s, dev(off), got[:m])
+    grouped.fp8_grouped_mm(a, b, a_s, b_s, dev(want_off), want[:m])
+    assert torch.equal(got, want) and gemm.device_status() == 0
+    ref, mag = reference(a, b, a_s, b_s, want_off.tolist())
+    rows = slice(int(want_off[0]), int(want_off[-1]))
+    assert_within(got[rows], ref[rows], 2.0 ** -8 * ref[rows].abs() + 2.0 ** -11 * mag[rows] + 2.0 ** -24)
+    assert (got[:rows.start] == 5).all() and (got[rows.stop:] == 5).all()
