@@ -95,6 +95,26 @@ __device__ __forceinline__ float largest_of(const Eight<__nv_bfloat16>& x) {
     return max_nan(__low2float(a), __high2float(a));
 }
 
+// The smallest of eight, NaN left out.
+__device__ __forceinline__ float lowest_of(const Eight<float>& x) {
+    float a = x.e[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) a = fminf(a, x.e[i]);
+    return a;
+}
+__device__ __forceinline__ float lowest_of(const Eight<__half>& x) {
+    __half2 a = __halves2half2(x.e[0], x.e[1]);
+#pragma unroll
+    for (int i = 2; i < 8; i += 2) a = __hmin2(a, __halves2half2(x.e[i], x.e[i + 1]));
+    return fminf(__low2float(a), __high2float(a));
+}
+__device__ __forceinline__ float lowest_of(const Eight<__nv_bfloat16>& x) {
+    __nv_bfloat162 a = __halves2bfloat162(x.e[0], x.e[1]);
+#pragma unroll
+    for (int i = 2; i < 8; i += 2) a = __hmin2(a, __halves2bfloat162(x.e[i], x.e[i + 1]));
+    return fminf(__low2float(a), __high2float(a));
+}
+
 // The half warp's largest value (16 lanes hold one block of 128).
 __device__ __forceinline__ float half_warp_max(float a) {
 #pragma unroll
@@ -106,14 +126,16 @@ __device__ __forceinline__ float half_warp_max(float a) {
 // q0 + (numerator - q0 * divisor) / divisor in fused operations.
 //
 // 448 / a rounded to nearest for 2^-100 <= a, zero for an infinity; so values that lie on a tie of two e4m3 ones go where the
-// formula sends them.  (The reciprocal is that of a scaled value: neither leaves the range of normal numbers.  That one correction is
+// formula sends them.  (On a scaled value: neither it nor its reciprocal leaves the range of normal numbers.  That one correction is
 // enough for every a is tested: powers of two aside there are 2^23 of them.  A division costs the kernels for 16-bit rows, which have 32
 // registers, a stack frame.)
 __device__ __forceinline__ float steps_per_unit(float a) {
+    constexpr float top = kE4m3Max * 0x1p-20f;
+    const float b = a * 0x1p-20f;
     float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(a * 0x1p-20f));
-    const float q = y * (kE4m3Max * 0x1p-20f);
-    return isinf(a) ? 0.f : fmaf(fmaf(-q, a, kE4m3Max) * 0x1p-20f, y, q);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(b));
+    const float q = y * top;
+    return fmaf(fmaf(-q, fminf(b, 0x1p120f), top), y, q);         // (an infinity: 0 * finite)
 }
 // a / 448 rounded to nearest: here the divisor's reciprocal itself is.  An infinity stays one.
 __device__ __forceinline__ float over_448(float a) {
@@ -121,24 +143,25 @@ __device__ __forceinline__ float over_448(float a) {
     const float q = a * inv;
     return isinf(a) ? a : fmaf(fmaf(-q, kE4m3Max, a), inv, q);
 }
-// g / (1 + exp(-g)) for g >= kSiluLow, where the reciprocal is a normal number.  exp(-g) = 2^t (1 + d ln 2) with t = fl(-g log2 e) and d
-// what that left out: the product's rounding, and what log2 e has beyond 24 bits.  Off by 2^-20.7 at most: ten times 2^-24, of which 2^t
-// has four and the reciprocal two.
+// g / (1 + exp(-g)) for g >= kSiluLow, where the reciprocal is a normal number.  exp(-g) = 2^t exp(c) with t = fl(-g log2 e) and
+// c = -g - t ln 2 what that left out, 2^-18 at most: 1 + c.  Off by 2^-20.7 at most: ten times 2^-24, of which 2^t has four and the
+// reciprocal two.
 constexpr float kSiluLow = -87.0f;
 __device__ __forceinline__ float silu(float g) {
-    constexpr float log2e = 1.44269502f, log2e_rest = 1.92596303e-8f, ln2 = 0.693147181f;
-    const float t = -g * log2e, d = fmaf(-g, log2e_rest, fmaf(-g, log2e, -t));
+    constexpr float log2e = 1.44269504f, ln2 = 0.693147182f, ln2_rest = -1.90465421e-9f;
+    const float t = -g * log2e, c = fmaf(-t, ln2_rest, fmaf(-t, ln2, -g));
     float e, r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-    // (where 2^t is no normal number, d may be none either)
-    if (fabsf(t) < 126.0f) e = fmaf(e, d * ln2, e);
+    // (where 2^t is no normal number, c may be none either)
+    if (fabsf(t) < 126.0f) e = fmaf(e, c, e);
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
     return g * r;
 }
-// SiLU(g) * u below that: 1 / (1 + exp(-g)) is exp(g) there, which leaves the normal numbers; its root does not before g u exp(g) does.
-__device__ __forceinline__ float swiglu_low(float g, float u) {
+// SiLU(g) * u for every g.  Below kSiluLow 1 / (1 + exp(-g)) is exp(g), which leaves the normal numbers; its root does not before
+// g u exp(g) does.
+__device__ __forceinline__ float swiglu_far(float g, float u) {
     const float root = expf(0.5f * g);
-    return (g * root) * (root * u);
+    return g < kSiluLow ? (g * root) * (root * u) : silu(g) * u;
 }
 
 __device__ __forceinline__ uint2 to_e4m3x8(const float (&x)[8], float r) {
@@ -202,21 +225,26 @@ quantize_rows_kernel(const T* x, long long row_stride, const int* rows, uint32_t
         }
     }
     float v[PER][8], a[PER];
+    bool far = false;               // a gate that takes the long way: then all of the thread's do
+    if (SWIGLU) {
+        float low = lowest_of(g[0]);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = SWIGLU ? silu(g[i].f(j)) * u[i].f(j) : g[i].f(j);
-        if (SWIGLU) {
-            float low = g[i].f(0);
-#pragma unroll
-            for (int j = 1; j < 8; ++j) low = fminf(low, g[i].f(j));
-            if (low < kSiluLow)
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (g[i].f(j) < kSiluLow) v[i][j] = swiglu_low(g[i].f(j), u[i].f(j));
-        }
-        a[i] = SWIGLU ? largest_of(v[i]) : largest_of(g[i]);
+        for (int i = 1; i < PER; ++i) low = fminf(low, lowest_of(g[i]));
+        far = low < kSiluLow;
     }
+    if (far) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = swiglu_far(g[i].f(j), u[SWIGLU ? i : 0].f(j));
+    } else {
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = SWIGLU ? silu(g[i].f(j)) * u[SWIGLU ? i : 0].f(j) : g[i].f(j);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) a[i] = SWIGLU ? largest_of(v[i]) : largest_of(g[i]);
     uint8_t* to = q + (size_t)first * kBlock + lane * 8;
     if (PER == 4) {
         const bool up8 = lane & 8, up4 = lane & 4;

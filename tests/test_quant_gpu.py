@@ -350,3 +350,15 @@ def test_swiglu_at_the_ends(dtype):
     assert (q[2].float() == 0).all() and s[2, 0] == 2.0 ** -100 / 448
     one = 1 / (1 + np.exp(-1.0))
     assert q[4, 3].float() == 0 and (q[4, 4:].float() == 448).all() and abs(float(s[4, 0]) * 448 / one - 1) < SWIGLU
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_far_gates_in_long_calls_are_those_of_short_ones(dtype):
+    """A thread takes the long way for all of its gates when one needs it: what it does beside that is the same arithmetic."""
+    m, f = 8191, 640
+    gu = torch.randn(m, 2 * f, device=DEV).mul_(40).clamp_(-104, 104).to(dtype)
+    q, s = quant.fp8_swiglu_quantize(gu)
+    for i in (0, 500, 4000, m - 300):
+        q1, s1 = quant.fp8_swiglu_quantize(gu[i:i + 300])
+        assert torch.equal(q[i:i + 300].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s[i:i + 300], s1)
+    check_swiglu(gu, q, s)
