@@ -23,6 +23,8 @@ def _check_input(what, name, x):
         raise ValueError(f"{what}: {name} must be float16, bfloat16 or float32")
     if x.device.index != torch.cuda.current_device():
         raise ValueError(f"{what}: {name} must be on the current device")
+    if max(x.shape, default=0) >= 2 ** 31:
+        raise ValueError(f"{what}: {name} must have fewer than 2^31 rows and columns")
 
 
 def _outputs(what, out, q_shape, scale_shape, device):

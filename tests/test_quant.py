@@ -94,3 +94,20 @@ def test_the_library_is_built_where_the_extension_cannot_be(rf_lib, monkeypatch,
     monkeypatch.setenv("CXX", "false")
     monkeypatch.setattr(build, "TENSORS_PATH", build.TENSORS_PATH + ".other")
     assert build.build() == build.LIB_PATH and "without its extension" in capsys.readouterr().err
+
+
+def test_more_than_31_bits_of_a_size_are_refused(monkeypatch):
+    """Sizes go to the library as 32-bit integers: 2^32 + 128 columns would count as 128.  (The memory is never touched.)"""
+    monkeypatch.setattr(_lib, "_tensors", _lib._NoTensors)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: None)
+    called = []
+    monkeypatch.setattr(quant, "_outputs", lambda *a: called.append(a))
+    cuda = lambda t: t.as_subclass(Meta)
+    long = torch.empty(1, 2 ** 32 + 256, dtype=torch.float16)
+    windows = torch.empty(2 ** 32 + 200, dtype=torch.float16).unfold(0, 128, 1)         # 2^32 + 73 rows
+    for fn, x in ((quant.fp8_quantize, long), (quant.fp8_swiglu_quantize, long), (quant.fp8_quantize_blocks, long),
+                  (quant.fp8_quantize_blocks, long.unsqueeze(0)), (quant.fp8_quantize, long[:, :2 ** 31]),
+                  (lambda x: quant.fp8_quantize(x, rows=torch.zeros(3, dtype=torch.int32)), windows)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            fn(cuda(x))
+    assert not called
