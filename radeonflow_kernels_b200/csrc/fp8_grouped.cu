@@ -8,7 +8,7 @@
 //
 // What bounds it: as the plain product the power cap and the epilogue's K block, and here the rows that tiles hold beyond their
 // groups' ends, half a tile a group.  32768 rows, n 4096, k 7168: one group 0.89 ms (the plain product's CTA pairs 0.81 to 0.90 on
-// that box), 32 uneven groups, which need a ninth tile every other time, 0.96 to 1.15 between runs.  The same on CTA pairs with
+// that box), 32 uneven groups, which need a ninth tile every other time, 0.97 to 1.14 between runs.  The same on CTA pairs with
 // 256 x 256 tiles: 1.01 to 1.19; 8192 rows in 32 groups 368 us, here 331; they win in one group only, 870 / 887.
 #include "fp8_grouped.cuh"
 #include "host_util.h"

@@ -20,10 +20,10 @@
 // item with the last chunk of a column tile adds the chunks up in their order, and the last item of a result tile adds the
 // experts in rank order: results are the same bits whoever comes last.  A token is routed by one CTA: every CTA for itself takes one
 // hand-over less, and for 32 tokens through 128 or 256 experts 10 us more.
-// One token through 9 fp16 experts of 1024 x 512 takes 18 us, through 5 of 7168 x 2048 70 (6.3 TB/s); 13 tokens through 86 of 256
-// FP8 experts 700 (5.5 TB/s), 32 through 164 1280 (5.7).  What holds FP8 below fp16's rate: the MMA warps are busy for two thirds of
-// the time, so that their waits and the stream's do not always overlap (the stream alone would take 641 us for those 13 tokens); a third
-// group of four, at 96 registers, is slower.  Warps of a CTA:
+// One token through 9 fp16 experts of 1024 x 512 takes 18 us, through 5 of 7168 x 2048 71 to 76 (5.8 to 6.2 TB/s); 13 tokens through 86 of
+// 256 FP8 experts 710 to 780 (5.0 to 5.4 TB/s), 32 through 164 1340 to 1400 (5.3).  What holds FP8 below fp16's rate: the MMA warps are busy for
+// two thirds of the time, so that their waits and the stream's do not always overlap (the stream alone took 641 us of 729 for those 13
+// tokens); a third group of four, at 96 registers, is slower.  Warps of a CTA:
 //   0      draws tickets, issues the weight loads (16 KB stages)
 //   1-3    the items' token rows (or, for the second product, h) into shared memory
 //   4-11   mma.sync m16n8k16, weights as the 16-row operand, up to 8 tokens as the 8 columns: a warp owns 16 of the item's 128

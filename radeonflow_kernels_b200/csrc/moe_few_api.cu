@@ -47,7 +47,7 @@ int choose_chunk(int tiles, int k, int most, int num_sms) {
 }
 
 Plan make_plan(const RfMoeFewConfig& c, int t) {
-    const int num_sms = 148;
+    const int num_sms = 148;        // a B200's: a workspace's size needs no device (with another count the plan is less even)
     const int fs = c.d_expert * c.n_shared_experts, width = fs > c.d_expert ? fs : c.d_expert;
     const int hit = c.n_routed_experts < t * c.n_experts_per_token ? c.n_routed_experts : t * c.n_experts_per_token;
     const size_t pairs = (size_t)t * (c.n_experts_per_token + 1), d = c.d_hidden;

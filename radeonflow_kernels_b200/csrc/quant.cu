@@ -176,9 +176,9 @@ __device__ __forceinline__ uint2 to_e4m3x8(const float (&x)[8], float r) {
 // Memory and instructions bound it alike: a thread's 32 elements were 496 instructions when every lane reduced each of its blocks
 // by itself, found its scale and checked each element for the end, and 32768 gathered rows of 7168 bf16 took 121 us.  So the four
 // blocks are reduced together (lane l ends with block l / 4's maximum, by 5 shuffles instead of 16) and each quad of lanes finds one
-// block's factors: 98 us.  What is left of a gather waits for memory, so that resident warps count: 91 us with 8 CTAs an SM (32
-// registers) where 6 fit by themselves; two units a thread, the second's loads ahead of the first's work, or a ring of bulk copies
-// before a few warps, were slower (118 and 129), as were column panels that stay in L2 (95, at best).
+// block's factors: 98 us.  What is left of a gather waits for memory, so that resident warps count: 91 to 96 us with 8 CTAs an SM
+// (32 registers) where 6 fit by themselves; two units a thread, the second's loads ahead of the first's work, or a ring of bulk
+// copies before a few warps, were slower (118 and 129), as were column panels that stay in L2 (95 beside 91, at best).
 constexpr int kRowThreads = 256;
 template <class T, bool VEC, bool SWIGLU, int PER>                   // resident, by registers: what fits without spills, elsewhere
 constexpr int kRowCtas = PER == 1 || (VEC && !SWIGLU && sizeof(T) == 2) ? 8 : (SWIGLU && (!VEC || sizeof(T) == 4)) ? 3 : 5;
