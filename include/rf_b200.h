@@ -546,7 +546,8 @@ typedef struct {
 } RfMoeFewConfig;
 /* HOST arrays of n_routed_experts device pointers, and the shared expert's behind them if there is one; the scale arrays
  * only for RF_MOE_FEW_E4M3 (else NULL).  Weights, router_weight (fp16 [E, d_hidden]) and router_bias (fp32 [E] or NULL) are kept by
- * reference.  Allocates a table on the current device and copies to it: call it outside stream capture.  */
+ * reference.  Experts whose matrices lie at even distances (views of one stack) are read a little faster than others.
+ * Allocates a table on the current device and copies to it: call it outside stream capture.  */
 int rf_moe_few_create(const RfMoeFewConfig *config, const void *router_weight, const float *router_bias,
                       const void *const *expert_gate, const void *const *expert_up, const void *const *expert_down,
                       const float *const *gate_scale, const float *const *up_scale, const float *const *down_scale,

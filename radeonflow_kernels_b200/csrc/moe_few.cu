@@ -20,8 +20,8 @@
 // item with the last chunk of a column tile adds the chunks up in their order, and the last item of a result tile adds the
 // experts in rank order: results are the same bits whoever comes last.  A token is routed by one CTA: every CTA for itself takes one
 // hand-over less, and for 32 tokens through 128 or 256 experts 10 us more.
-// One token through 9 fp16 experts of 1024 x 512 takes 18 us, through 5 of 7168 x 2048 71 to 76 (5.8 to 6.2 TB/s); 13 tokens through 86 of
-// 256 FP8 experts 710 to 780 (5.0 to 5.4 TB/s), 32 through 164 1340 to 1400 (5.3).  What holds FP8 below fp16's rate: the MMA warps are busy for
+// One token through 9 fp16 experts of 1024 x 512 takes 18 us, through 5 of 7168 x 2048 70 to 75 (5.9 to 6.3 TB/s); 13 tokens through 86 of
+// 256 FP8 experts 730 to 760 (5.1 to 5.3 TB/s), 32 through 164 1330 to 1395 (5.3).  What holds FP8 below fp16's rate: the MMA warps are busy for
 // two thirds of the time, so that their waits and the stream's do not always overlap (the stream alone took 641 us of 729 for those 13
 // tokens); a third group of four, at 96 registers, is slower.  Warps of a CTA:
 //   0      draws tickets, issues the weight loads (16 KB stages)
@@ -422,7 +422,7 @@ __device__ __forceinline__ void build_lists(const MoeFewParams& p, Routing& rt) 
 
 template <bool FP8, int NG>
 __global__ void __launch_bounds__(THREADS, 1)
-moe_few_kernel(const MoeFewParams p) {
+moe_few_kernel(const __grid_constant__ FewMaps even, const MoeFewParams p) {
     using C = Cfg<FP8, NG>;
     constexpr int STAGES = C::kStages;
 
@@ -451,6 +451,7 @@ moe_few_kernel(const MoeFewParams p) {
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     griddep_launch_dependents();
+    if (warp == WARP_SUM && lane < (p.fs > 0 ? 6 : 3) && p.maps == nullptr) tma_prefetch_desc(even.m + lane);
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(full_bar(s), 1);
@@ -580,12 +581,12 @@ moe_few_kernel(const MoeFewParams p) {
                     ticket = atomicAdd(p.head + kFewTicket, 1);
                     continue;
                 }
-                const int e = expert_of(it);
                 int k0, len;
                 k_range(it, &k0, &len);
-                const CUtensorMap* m0 = p.maps + 3 * e + (it.x == kFirst ? 0 : 2);
+                const int which = it.x == kFirst ? 0 : 2, e = expert_of(it), matrix = p.maps == nullptr && it.y >= 0 ? e : 0;
+                const CUtensorMap* m0 = p.maps != nullptr ? p.maps + 3 * e + which : even.m + (it.y < 0 ? 3 : 0) + which;
                 const CUtensorMap* m1 = it.x == kFirst ? m0 + 1 : m0;
-                if (m0 != acquired) {
+                if (p.maps != nullptr && m0 != acquired) {
                     tma_acquire_desc(m0);
                     if (m1 != m0) tma_acquire_desc(m1);
                     acquired = m0;
@@ -599,8 +600,8 @@ moe_few_kernel(const MoeFewParams p) {
                     const uint32_t dst = smem_base + s * STAGE_BYTES;
                     const int k = k0 + i * C::kStageK;
                     mbar_expect_tx(full_bar(s), STAGE_BYTES);
-                    tma_load_2d(dst, m0, full_bar(s), FP8 ? k : n0, FP8 ? n0 : k);
-                    tma_load_2d(dst + BOX_BYTES, m1, full_bar(s), FP8 ? k : n1, FP8 ? n1 : k);
+                    tma_load_3d(dst, m0, full_bar(s), FP8 ? k : n0, FP8 ? n0 : k, matrix);
+                    tma_load_3d(dst + BOX_BYTES, m1, full_bar(s), FP8 ? k : n1, FP8 ? n1 : k, matrix);
                     if (++s == STAGES) { s = 0; ph ^= 1; }
                 }
             }
@@ -1030,7 +1031,7 @@ moe_few_kernel(const MoeFewParams p) {
 }
 
 template <bool FP8, int NG>
-cudaError_t launch_one(const MoeFewParams& p, int num_sms, cudaStream_t stream) {
+cudaError_t launch_one(const FewMaps& maps, const MoeFewParams& p, int num_sms, cudaStream_t stream) {
     static bool attr_set[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
@@ -1041,14 +1042,15 @@ cudaError_t launch_one(const MoeFewParams& p, int num_sms, cudaStream_t stream) 
         if (e != cudaSuccess) return e;
         attr_set[dev] = true;
     }
-    return launch_kernel(kernel, dim3((unsigned)num_sms), THREADS, smem, stream, true, p);
+    return launch_kernel(kernel, dim3((unsigned)num_sms), THREADS, smem, stream, true, maps, p);
 }
 
 }  // namespace
 
-cudaError_t moe_few_launch(const MoeFewParams& p, bool fp8, int num_sms, cudaStream_t stream) {
-    if (moe_few_rows(p.t) == 8) return fp8 ? launch_one<true, 1>(p, num_sms, stream) : launch_one<false, 1>(p, num_sms, stream);
-    return fp8 ? launch_one<true, 2>(p, num_sms, stream) : launch_one<false, 2>(p, num_sms, stream);
+cudaError_t moe_few_launch(const MoeFewParams& p, const FewMaps& maps, bool fp8, int num_sms, cudaStream_t stream) {
+    if (moe_few_rows(p.t) == 8)
+        return fp8 ? launch_one<true, 1>(maps, p, num_sms, stream) : launch_one<false, 1>(maps, p, num_sms, stream);
+    return fp8 ? launch_one<true, 2>(maps, p, num_sms, stream) : launch_one<false, 2>(maps, p, num_sms, stream);
 }
 
 }  // namespace rf

@@ -13,11 +13,19 @@ constexpr int kFewMaxTopK = 8;
 // Words in front of the workspace (128 bytes apart: the ticket is drawn while the others are read)
 enum { kFewTicket = 0, kFewExits = 32, kFewBad = 64, kFewCalls = 96, kFewHeadWords = 128 };
 
+// Tensor maps of weights that lie at even distances, as those of one stack do: gate, up, down of the experts, then of the shared one.
+// As kernel parameters they need no fence.  Where the experts lie anywhere, a table has a map for each of their matrices, which
+// the proxy's fence has to be run on at every change of expert: 1.5 % of the time of 1 token through 4 fp16 experts of 7168 x 2048,
+// 4 % with 13 tokens through 86 of 256 FP8 experts, 6 % with 32 through 8 of 128 of 2048 x 768.
+struct FewMaps {
+    CUtensorMap m[6];
+};
+
 struct MoeFewParams {
     const void* x;                  // fp16 [t, d]
     const void* router;             // fp16 [experts, d]
     const float* router_bias;       // fp32 [experts] or nullptr
-    const CUtensorMap* maps;        // device: gate, up, down of every expert, then of the shared one
+    const CUtensorMap* maps;        // device: gate, up, down of every expert, then of the shared one; or nullptr: FewMaps
     const float* const* scales;     // device: the same order (FP8 weights)
     void* out;                      // fp16 [t, d]
     // workspace: words of 32 bits of data and the call's number
@@ -54,6 +62,6 @@ __host__ __device__ constexpr int few_stages(bool fp8, int ng) { return ng > 1 ?
 // The first stage of an item that is `group`'s, where stage 0 lies in slot s; from there every other one is.
 __host__ __device__ constexpr int few_first_stage(int group, int s) { return (group ^ s) & 1; }
 
-cudaError_t moe_few_launch(const MoeFewParams& p, bool fp8, int num_sms, cudaStream_t stream);
+cudaError_t moe_few_launch(const MoeFewParams& p, const FewMaps& maps, bool fp8, int num_sms, cudaStream_t stream);
 
 }  // namespace rf

@@ -15,8 +15,10 @@ struct RfMoeFew {
     int device;
     const void* router;
     const float* router_bias;
-    CUtensorMap* maps;
+    void* tables;               // device: maps (if there are any), scales
+    CUtensorMap* maps;          // nullptr: the experts lie at even distances
     const float** scales;
+    rf::FewMaps even;
 };
 
 namespace {
@@ -137,9 +139,20 @@ cudaError_t zeroed(size_t bytes, void** out) {
     return e;
 }
 
-bool encode(CUtensorMap* m, bool fp8, const void* base, int k, int n) {
-    return fp8 ? rf::encode_tma_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, (uint64_t)n, (uint64_t)k, (uint64_t)k, 64, 128, true)
-               : rf::encode_tma_2d(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base, (uint64_t)k, (uint64_t)n, (uint64_t)n * 2, 64, 64, true);
+// `count` matrices of k x n weights, `apart` bytes apart
+bool encode(CUtensorMap* m, bool fp8, const void* base, int k, int n, int count, long long apart) {
+    return fp8 ? rf::encode_tma_matrices(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, (uint64_t)k, (uint64_t)n, (uint64_t)count, (uint64_t)k,
+                                         (uint64_t)apart, 128, 64)
+               : rf::encode_tma_matrices(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, base, (uint64_t)n, (uint64_t)k, (uint64_t)count,
+                                         (uint64_t)n * 2, (uint64_t)apart, 64, 64);
+}
+
+// The distance of matrices of `size` bytes that lie evenly, whole rows apart, as one tensor map holds them; else 0.
+long long distance(const void* const* p, int count, long long size, long long row_bytes) {
+    const long long apart = count > 1 ? (long long)((uintptr_t)p[1] - (uintptr_t)p[0]) : size;
+    for (int i = 2; i < count; ++i)
+        if ((long long)((uintptr_t)p[i] - (uintptr_t)p[i - 1]) != apart) return 0;
+    return apart >= size && apart % row_bytes == 0 && apart < (1LL << 40) ? apart : 0;
 }
 
 }  // namespace
@@ -168,23 +181,34 @@ int rf_moe_few_create(const RfMoeFewConfig* config, const void* router_weight, c
     }
     if (rf::misaligned({router_weight}, 16) || rf::misaligned({router_bias}, 4)) return RF_ERR_MISALIGNED;
     if (!rf::device_state()) return RF_ERR_CUDA;
+    const int experts = c.n_routed_experts, d = c.d_hidden, f = c.d_expert, fs = f * c.n_shared_experts;
+    const long long element = fp8 ? 1 : 2, size = (long long)d * f * element, shared = (long long)d * fs * element;
+    const void* const* const mats[3] = {expert_gate, expert_up, expert_down};
+    const float* const* const mat_scales[3] = {gate_scale, up_scale, down_scale};
+    rf::FewMaps even_maps = {};
     std::vector<CUtensorMap> maps;
     std::vector<const float*> scales;
+    bool even = true;
+    long long apart[3];
+    for (int i = 0; i < 3; ++i) {
+        apart[i] = distance(mats[i], experts, size, element * (fp8 == (i == 2) ? f : d));       // (rows along k in FP8, along n in fp16)
+        even = even && apart[i] != 0;
+    }
     try {
-        maps.resize((size_t)3 * sets);
+        if (!even) maps.resize((size_t)3 * sets);
         scales.resize((size_t)3 * sets, nullptr);
     } catch (const std::bad_alloc&) {
         return RF_ERR_CUDA;
     }
-    for (int e = 0; e < sets; ++e) {
-        const int f = e < c.n_routed_experts ? c.d_expert : c.d_expert * c.n_shared_experts;
-        if (!encode(&maps[3 * e], fp8, expert_gate[e], c.d_hidden, f) || !encode(&maps[3 * e + 1], fp8, expert_up[e], c.d_hidden, f) ||
-            !encode(&maps[3 * e + 2], fp8, expert_down[e], f, c.d_hidden))
-            return RF_ERR_CUDA;
-        if (fp8) {
-            scales[3 * e] = gate_scale[e];
-            scales[3 * e + 1] = up_scale[e];
-            scales[3 * e + 2] = down_scale[e];
+    for (int i = 0; i < 3; ++i) {
+        auto one = [&](CUtensorMap* m, const void* base, int width, int count, long long bytes) {
+            return i < 2 ? encode(m, fp8, base, d, width, count, bytes) : encode(m, fp8, base, width, d, count, bytes);
+        };
+        if (even && !one(&even_maps.m[i], mats[i][0], f, experts, apart[i])) return RF_ERR_CUDA;
+        if (even && fs > 0 && !one(&even_maps.m[3 + i], mats[i][experts], fs, 1, shared)) return RF_ERR_CUDA;
+        for (int e = 0; e < sets; ++e) {
+            if (!even && !one(&maps[3 * e + i], mats[i][e], e < experts ? f : fs, 1, e < experts ? size : shared)) return RF_ERR_CUDA;
+            if (fp8) scales[3 * e + i] = mat_scales[i][e];
         }
     }
     RfMoeFew* few = new (std::nothrow) RfMoeFew();
@@ -192,6 +216,7 @@ int rf_moe_few_create(const RfMoeFewConfig* config, const void* router_weight, c
     few->cfg = c;
     few->router = router_weight;
     few->router_bias = router_bias;
+    few->even = even_maps;
     cudaGetDevice(&few->device);
     const size_t map_bytes = maps.size() * sizeof(CUtensorMap), scale_bytes = scales.size() * sizeof(float*);
     char* dev = nullptr;
@@ -200,9 +225,10 @@ int rf_moe_few_create(const RfMoeFewConfig* config, const void* router_weight, c
         delete few;
         return RF_ERR_CUDA;
     }
-    few->maps = reinterpret_cast<CUtensorMap*>(dev);
+    few->tables = dev;
+    few->maps = even ? nullptr : reinterpret_cast<CUtensorMap*>(dev);
     few->scales = reinterpret_cast<const float**>(dev + map_bytes);
-    if (rf::upload(dev, maps.data(), map_bytes) != cudaSuccess ||
+    if ((!even && rf::upload(dev, maps.data(), map_bytes) != cudaSuccess) ||
         rf::upload(dev + map_bytes, scales.data(), scale_bytes) != cudaSuccess) {
         cudaFree(dev);
         delete few;
@@ -214,7 +240,7 @@ int rf_moe_few_create(const RfMoeFewConfig* config, const void* router_weight, c
 
 int rf_moe_few_destroy(RfMoeFew* few) {
     if (!few) return RF_OK;
-    const int rc = rf_moe_few_workspace_free(few->maps);       // (may come from a garbage collector during a capture)
+    const int rc = rf_moe_few_workspace_free(few->tables);       // (may come from a garbage collector during a capture)
     delete few;
     return rc;
 }
@@ -339,7 +365,7 @@ int rf_moe_few_forward(RfMoeFew* few, const void* x, int n_tokens, void* out, vo
     p.router_units = (p.experts + 15) / 16 * p.router_chunks * rf::moe_few_token_groups(p.t);
     p.status = st->status;
     p.launch_tag = rf::next_launch_tag();
-    const cudaError_t e = rf::moe_few_launch(p, c.weight_type == RF_MOE_FEW_E4M3, st->num_sms, reinterpret_cast<cudaStream_t>(stream));
+    const cudaError_t e = rf::moe_few_launch(p, few->even, c.weight_type == RF_MOE_FEW_E4M3, st->num_sms, reinterpret_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) {
         fprintf(stderr, "rf_b200: launch of the layer for a few tokens failed: %s\n", cudaGetErrorString(e));
         return RF_ERR_CUDA;

@@ -101,19 +101,20 @@ def test_maps_in_device_memory_are_acquired():
     before the first of them, and on the next one when the expert changes."""
     found = set()
     for f, name, params, body in KERNELS:
-        for maps in set(re.findall(r"const CUtensorMap\* (\w+) = p\.\w*maps\b", body)) | set(
-                re.findall(r"const CUtensorMap\* (\w+) = [^;]*\bm0 \+ 1", body)) | set(
-                re.findall(r"const CUtensorMap\* (\w+) = SWIGLU \? p\.w2_maps", body)):
+        if not re.search(r"p\.\w*maps\b", body):
+            assert not re.search(r"CUtensorMap\s*\*", params), (f, name)
+            continue
+        pointers = re.findall(r"const CUtensorMap\* (m\w+) = (?!\()", body)
+        for maps in pointers:
+            loads = [m.start() for m in re.finditer(r"tma_load_\dd\w*\([^,]+, " + maps + r",", body)]
+            if not loads or maps == "mx":           # (mx: the rows' maps, kernel parameters)
+                continue
             found.add((name, maps))
-            load = re.search(r"tma_load_2d\w*\([^,]+, " + maps + r",", body)
             fence = body.index(f"tma_acquire_desc({maps})")
-            assert load and body.rindex("if (m", 0, fence) < fence < load.start(), (f, maps)
-            assert not re.search(r"tma_prefetch_desc\((p\.|" + maps + ")", body), f      # (nor fetched before that)
+            assert re.search(r"if \((p\.maps != nullptr && )?m\w+ != acquired\) \{", body[:fence]) and fence < loads[0], (f, maps)
+        # nor is one fetched before that
+        assert not re.search(r"tma_prefetch_desc\((p\.|" + "|".join(pointers) + ")", body), f
     assert found == {("moe_few_kernel", "m0"), ("moe_few_kernel", "m1"), ("moe_gemm_kernel", "mw"), ("moe_gemm_kernel", "mw2")}
-    # nowhere else are maps read through a pointer
-    for f, name, params, body in KERNELS:
-        if name not in ("moe_few_kernel", "moe_gemm_kernel"):
-            assert not re.search(r"p\.\w*maps\b", body) and not re.search(r"CUtensorMap\s*\*", params), (f, name)
 
 
 def test_grouped_scale_slots_are_given_back_after_they_were_read():

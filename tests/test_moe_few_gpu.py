@@ -408,3 +408,85 @@ def test_a_capture_that_fails_leaves_nothing():
 def test_workspaces_of_captures_only(rf_lib):
     got = ctypes.c_void_p()
     assert rf_lib.rf_moe_few_workspace_alloc_captured(torch.cuda.Stream().cuda_stream, 1000, ctypes.byref(got)) == 7 and not got
+
+
+class Scattered(moe_few.FewTokenMoE):
+    """The same weights, each matrix in memory of its own, the experts in descending order: no distance is even."""
+
+    def _copies(self, rows):
+        gap = 48
+        buf = torch.empty(sum(t.numel() * t.element_size() + gap for row in rows for t in row) + 16, dtype=torch.uint8, device=DEV)
+        at, out = 0, [None] * len(rows)
+        for i in reversed(range(len(rows))):
+            out[i] = []
+            for t in rows[i]:
+                n = t.numel() * t.element_size()
+                out[i].append(buf[at:at + n].view(t.dtype).view(t.shape).copy_(t))
+                at += n + gap
+        return out
+
+    def _fp16_matrices(self, *args):
+        rows, scales = super()._fp16_matrices(*args)
+        return self._copies(rows), scales
+
+    def _fp8_matrices(self, *args):
+        rows, scales = super()._fp8_matrices(*args)
+        return self._copies(rows), scales
+
+
+def stacked(w, cfg, interleaved):
+    """The fp16 layer's dict as views of stacks."""
+    e, w = cfg["n_routed_experts"], dict(w)
+    mats = [torch.stack([w[f"experts.{i}.{j}.weight"] for i in range(e)]) for j in range(3)]
+    if interleaved:                 # gate and up in one stack
+        both = torch.stack(mats[:2], 1)
+        mats[:2] = both[:, 0], both[:, 1]
+    for i in range(e):
+        for j in range(3):
+            w[f"experts.{i}.{j}.weight"] = mats[j][i]
+    return w
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("t,d,f,e,k,ns", [(1, 256, 128, 16, 4, 1), (8, 640, 256, 8, 2, 2), (13, 1152, 384, 32, 8, 1), (32, 512, 128, 4, 2, 0), (5, 384, 128, 1, 1, 1)])
+def test_weights_may_lie_anywhere(t, d, f, e, k, ns, fp8):
+    """Stacks (one tensor map each), and matrices anywhere (a table of them): the same bits."""
+    x, w, cfg, dense = make(t, d, f, e, k, ns, fp8, seed=d + e)
+    ref, tol, _ = reference(x, w, cfg, dense)
+    layers = [moe_few.FewTokenMoE(w, cfg), Scattered(w, cfg)]
+    if not fp8:
+        layers += [moe_few.FewTokenMoE(stacked(w, cfg, interleaved), cfg) for interleaved in (False, True)]
+    got = [layer.forward(x) for layer in layers]
+    check(got[0], ref, tol)
+    assert all(torch.equal(g, got[0]) for g in got)
+    for _ in range(50):
+        for layer in layers:
+            assert torch.equal(layer.forward(x), got[0])
+    assert gemm.device_status() == 0
+
+
+def test_widths_of_64_in_stacks():
+    for t, d, f, e, k, ns in ((1, 64, 64, 4, 2, 1), (20, 320, 192, 16, 2, 2)):
+        x, w, cfg, dense = make(t, d, f, e, k, ns, False, seed=9)
+        ref, tol, _ = reference(x, w, cfg, dense)
+        got = moe_few.FewTokenMoE(stacked(w, cfg, False), cfg).forward(x)
+        check(got, ref, tol)
+        assert torch.equal(Scattered(w, cfg).forward(x), got)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_scattered_layers_made_one_where_the_other_was(fp8):
+    made = [make(4, 512, 256, 16, 4, 1, fp8, seed=30 + i) for i in range(2)]
+    want = [reference(x, w, cfg, dense) for x, w, cfg, dense in made]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for i in range(40):
+        x, w, cfg, _ = made[i % 2]
+        layer = Scattered(w, cfg)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            got = layer.forward(x)
+        side.synchronize()
+        check(got, *want[i % 2][:2])
+        del layer
+    assert gemm.device_status() == 0
