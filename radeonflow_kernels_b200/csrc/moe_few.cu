@@ -20,8 +20,8 @@
 // item with the last chunk of a column tile adds the chunks up in their order, and the last item of a result tile adds the
 // experts in rank order: results are the same bits whoever comes last.  A token is routed by one CTA: every CTA for itself takes one
 // hand-over less, and for 32 tokens through 128 or 256 experts 10 us more.
-// One token through 9 fp16 experts of 1024 x 512 takes 18 us, through 5 of 7168 x 2048 70 to 75 (5.9 to 6.3 TB/s); 13 tokens through 86 of
-// 256 FP8 experts 730 to 760 (5.1 to 5.3 TB/s), 32 through 164 1330 to 1395 (5.3).  What holds FP8 below fp16's rate: the MMA warps are busy for
+// One token through 9 fp16 experts of 1024 x 512 takes 18 us, through 5 of 7168 x 2048 71 to 75 (5.9 to 6.2 TB/s); 13 tokens through 86 of
+// 256 FP8 experts 700 to 760 (5.1 to 5.5 TB/s), 32 through 164 1310 to 1395 (5.5).  What holds FP8 below fp16's rate: the MMA warps are busy for
 // two thirds of the time, so that their waits and the stream's do not always overlap (the stream alone took 641 us of 729 for those 13
 // tokens); a third group of four, at 96 registers, is slower.  Warps of a CTA:
 //   0      draws tickets, issues the weight loads (16 KB stages)
@@ -451,7 +451,6 @@ moe_few_kernel(const __grid_constant__ FewMaps even, const MoeFewParams p) {
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     griddep_launch_dependents();
-    if (warp == WARP_SUM && lane < (p.fs > 0 ? 6 : 3) && p.maps == nullptr) tma_prefetch_desc(even.m + lane);
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(full_bar(s), 1);
@@ -583,7 +582,7 @@ moe_few_kernel(const __grid_constant__ FewMaps even, const MoeFewParams p) {
                 }
                 int k0, len;
                 k_range(it, &k0, &len);
-                const int which = it.x == kFirst ? 0 : 2, e = expert_of(it), matrix = p.maps == nullptr && it.y >= 0 ? e : 0;
+                const int which = it.x == kFirst ? 0 : 2, e = expert_of(it);
                 const CUtensorMap* m0 = p.maps != nullptr ? p.maps + 3 * e + which : even.m + (it.y < 0 ? 3 : 0) + which;
                 const CUtensorMap* m1 = it.x == kFirst ? m0 + 1 : m0;
                 if (p.maps != nullptr && m0 != acquired) {
@@ -591,7 +590,10 @@ moe_few_kernel(const __grid_constant__ FewMaps even, const MoeFewParams p) {
                     if (m1 != m0) tma_acquire_desc(m1);
                     acquired = m0;
                 }
+                // columns; and the rows in front of the expert's matrix in its stack
                 const int n0 = it.x == kFirst ? it.z * 64 : it.z * 128, n1 = it.x == kFirst ? n0 : n0 + 64;
+                const int in_stack = p.maps == nullptr && it.y >= 0 ? e : 0;
+                const int r0 = in_stack * even.rows[which], r1 = it.x == kFirst ? in_stack * even.rows[1] : r0;
                 const int n_stages = len / C::kStageK;
                 for (int i = 0; i < n_stages; ++i, ++st) {
                     if (i == max(n_stages - DRAW_AHEAD, 0)) ticket = atomicAdd(p.head + kFewTicket, 1);
@@ -600,8 +602,8 @@ moe_few_kernel(const __grid_constant__ FewMaps even, const MoeFewParams p) {
                     const uint32_t dst = smem_base + s * STAGE_BYTES;
                     const int k = k0 + i * C::kStageK;
                     mbar_expect_tx(full_bar(s), STAGE_BYTES);
-                    tma_load_3d(dst, m0, full_bar(s), FP8 ? k : n0, FP8 ? n0 : k, matrix);
-                    tma_load_3d(dst + BOX_BYTES, m1, full_bar(s), FP8 ? k : n1, FP8 ? n1 : k, matrix);
+                    tma_load_2d(dst, m0, full_bar(s), FP8 ? k : n0, r0 + (FP8 ? n0 : k));
+                    tma_load_2d(dst + BOX_BYTES, m1, full_bar(s), FP8 ? k : n1, r1 + (FP8 ? n1 : k));
                     if (++s == STAGES) { s = 0; ph ^= 1; }
                 }
             }

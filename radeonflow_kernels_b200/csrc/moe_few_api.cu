@@ -139,20 +139,19 @@ cudaError_t zeroed(size_t bytes, void** out) {
     return e;
 }
 
-// `count` matrices of k x n weights, `apart` bytes apart
-bool encode(CUtensorMap* m, bool fp8, const void* base, int k, int n, int count, long long apart) {
-    return fp8 ? rf::encode_tma_matrices(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, (uint64_t)k, (uint64_t)n, (uint64_t)count, (uint64_t)k,
-                                         (uint64_t)apart, 128, 64)
-               : rf::encode_tma_matrices(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, base, (uint64_t)n, (uint64_t)k, (uint64_t)count,
-                                         (uint64_t)n * 2, (uint64_t)apart, 64, 64);
+// Weights of k x n; `below`: rows that the map reaches beyond them
+bool encode(CUtensorMap* m, bool fp8, const void* base, int k, int n, long long below) {
+    return fp8 ? rf::encode_tma_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, (uint64_t)(n + below), (uint64_t)k, (uint64_t)k, 64, 128, true)
+               : rf::encode_tma_2d(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base, (uint64_t)(k + below), (uint64_t)n, (uint64_t)n * 2, 64, 64,
+                                   true);
 }
 
-// The distance of matrices of `size` bytes that lie evenly, whole rows apart, as one tensor map holds them; else 0.
-long long distance(const void* const* p, int count, long long size, long long row_bytes) {
-    const long long apart = count > 1 ? (long long)((uintptr_t)p[1] - (uintptr_t)p[0]) : size;
+// Rows from one matrix of `rows` rows to the next, where all lie evenly and a coordinate reaches the last one; else 0.
+int rows_apart(const void* const* p, int count, long long rows, long long row_bytes) {
+    const long long apart = count > 1 ? (long long)((uintptr_t)p[1] - (uintptr_t)p[0]) : rows * row_bytes;
     for (int i = 2; i < count; ++i)
         if ((long long)((uintptr_t)p[i] - (uintptr_t)p[i - 1]) != apart) return 0;
-    return apart >= size && apart % row_bytes == 0 && apart < (1LL << 40) ? apart : 0;
+    return apart >= rows * row_bytes && apart % row_bytes == 0 && apart / row_bytes <= 0x7fffffffLL / count ? (int)(apart / row_bytes) : 0;
 }
 
 }  // namespace
@@ -182,17 +181,16 @@ int rf_moe_few_create(const RfMoeFewConfig* config, const void* router_weight, c
     if (rf::misaligned({router_weight}, 16) || rf::misaligned({router_bias}, 4)) return RF_ERR_MISALIGNED;
     if (!rf::device_state()) return RF_ERR_CUDA;
     const int experts = c.n_routed_experts, d = c.d_hidden, f = c.d_expert, fs = f * c.n_shared_experts;
-    const long long element = fp8 ? 1 : 2, size = (long long)d * f * element, shared = (long long)d * fs * element;
     const void* const* const mats[3] = {expert_gate, expert_up, expert_down};
     const float* const* const mat_scales[3] = {gate_scale, up_scale, down_scale};
     rf::FewMaps even_maps = {};
     std::vector<CUtensorMap> maps;
     std::vector<const float*> scales;
     bool even = true;
-    long long apart[3];
     for (int i = 0; i < 3; ++i) {
-        apart[i] = distance(mats[i], experts, size, element * (fp8 == (i == 2) ? f : d));       // (rows along k in FP8, along n in fp16)
-        even = even && apart[i] != 0;
+        const int k = i < 2 ? d : f, n = i < 2 ? f : d;            // (FP8 rows are the n of a matrix, fp16 ones its k)
+        even_maps.rows[i] = rows_apart(mats[i], experts, fp8 ? n : k, fp8 ? k : 2LL * n);
+        even = even && even_maps.rows[i] != 0;
     }
     try {
         if (!even) maps.resize((size_t)3 * sets);
@@ -201,13 +199,13 @@ int rf_moe_few_create(const RfMoeFewConfig* config, const void* router_weight, c
         return RF_ERR_CUDA;
     }
     for (int i = 0; i < 3; ++i) {
-        auto one = [&](CUtensorMap* m, const void* base, int width, int count, long long bytes) {
-            return i < 2 ? encode(m, fp8, base, d, width, count, bytes) : encode(m, fp8, base, width, d, count, bytes);
+        auto one = [&](CUtensorMap* m, const void* base, int width, long long below) {
+            return i < 2 ? encode(m, fp8, base, d, width, below) : encode(m, fp8, base, width, d, below);
         };
-        if (even && !one(&even_maps.m[i], mats[i][0], f, experts, apart[i])) return RF_ERR_CUDA;
-        if (even && fs > 0 && !one(&even_maps.m[3 + i], mats[i][experts], fs, 1, shared)) return RF_ERR_CUDA;
+        if (even && !one(&even_maps.m[i], mats[i][0], f, (experts - 1LL) * even_maps.rows[i])) return RF_ERR_CUDA;
+        if (even && fs > 0 && !one(&even_maps.m[3 + i], mats[i][experts], fs, 0)) return RF_ERR_CUDA;
         for (int e = 0; e < sets; ++e) {
-            if (!even && !one(&maps[3 * e + i], mats[i][e], e < experts ? f : fs, 1, e < experts ? size : shared)) return RF_ERR_CUDA;
+            if (!even && !one(&maps[3 * e + i], mats[i][e], e < experts ? f : fs, 0)) return RF_ERR_CUDA;
             if (fp8) scales[3 * e + i] = mat_scales[i][e];
         }
     }
