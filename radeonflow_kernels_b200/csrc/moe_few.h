@@ -17,7 +17,7 @@ enum { kFewTicket = 0, kFewExits = 32, kFewBad = 64, kFewCalls = 96, kFewHeadWor
 // below the other, then of the shared one.  As kernel parameters they need no fence.  Where the experts lie anywhere, a table has a
 // map for each of their matrices, which the proxy's fence has to be run on at every change of expert: 1.5 % of the time of 1
 // token through 4 fp16 experts of 7168 x 2048, 4 % with 13 tokens through 86 of 256 FP8 experts, 6 % with 32 through 8 of 128 of
-// 2048 x 768.  (One 3-D map of the stack instead of 2-D ones is 3 % slower for those 13 tokens.)
+// 2048 x 768.  (One 3-D map of a stack instead of a 2-D one is 1 % slower for those 13 tokens.)
 struct FewMaps {
     CUtensorMap m[6];
     int rows[3];                    // from an expert's matrix to the next one's
